@@ -19,6 +19,8 @@ from .attention import fused_hqmq_attention_dequant_sdpa as fused_attention_refe
 from ._lib import HqmqError  # noqa: F401
 from .packed import PackedKV  # noqa: F401
 from .cache import PackedKVCache  # noqa: F401
+from .paged import PagedBatch, PagedKV, paged_attention, paged_attention_mass, paged_evict, paged_store  # noqa: F401
+from .paged_cache import PagedKVCache  # noqa: F401
 from .quantizers import HQMQQuantizer as HQMQ
 from .quantizers import KVQuantizer  # noqa: F401
 from .quantizers import OutlierAwareGenericQuantizer, OutlierAwareHQMQQuantizer
@@ -60,5 +62,6 @@ __all__ = [
     "fused_attention", "fused_attention_reference", "with_outlier_extraction", "device_info",
     "kernels_ada", "kernels_hopper", "kernels_blackwell",
     "PackedKV", "PackedKVCache", "fused_attention_packed", "combine_partials", "decode_dequant", "HqmqError",
+    "PagedKV", "PagedBatch", "PagedKVCache", "paged_attention", "paged_attention_mass", "paged_store", "paged_evict",
 ]
 __version__ = "0.1.0"

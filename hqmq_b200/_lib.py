@@ -93,6 +93,40 @@ class AttnArgs(C.Structure):
     ]
 
 
+class PagedPlan(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32)] + [(name, C.c_int32) for name in (
+        "n_seqs", "n_pages", "page_tokens", "H_q", "H_kv", "d", "window", "tab_room", "renew", "total_q", "most_q",
+        "reserved", "words", "seqs", "tabs", "n_tab", "dec_units", "dec_rows", "dec_ctas", "dec_unit", "dec_base",
+        "dec_warp", "dec_cut", "dec_tiles", "ch_units", "ch_streams", "ch_tiles", "ch_heads", "ch_whole", "ch_ctas",
+        "ch_unit", "ch_order", "ch_start", "ch_seqs", "ch_img_tiles", "ch_img", "ms_units", "ms_rows", "ms_ctas",
+        "ms_unit", "ms_base", "ms_warp", "ms_tiles", "ms_groups", "ms_group", "ms_tile_room", "ms_group_room")]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("q_dtype", C.c_int32), ("o_dtype", C.c_int32), ("r_qmax", C.c_int32),
+        ("Q", C.c_void_p), ("q_stride", C.c_int64 * 2), ("O", C.c_void_p), ("o_stride", C.c_int64 * 2),
+        ("softmax_scale", C.c_float), ("softcap", C.c_float), ("sinks", C.c_void_p), ("K", Packed), ("V", Packed),
+        ("table_K", C.c_void_p), ("table_V", C.c_void_p), ("plan", PagedPlan), ("plan_data", C.c_void_p),
+        ("prior", C.c_void_p), ("mass", C.c_void_p), ("decay", C.c_float), ("reserved", C.c_int32),
+    ]
+
+
+class PagedStoreArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("reserved", C.c_int32), ("src_K", Packed), ("src_V", Packed), ("K", Packed), ("V", Packed),
+        ("plan", PagedPlan), ("plan_data", C.c_void_p),
+    ]
+
+
+class PagedEvictArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("first", C.c_int32), ("last", C.c_int32), ("kept_stride", C.c_int32), ("K", Packed), ("V", Packed),
+        ("mass", C.c_void_p), ("new_mass", C.c_void_p), ("kept", C.c_void_p), ("src", PagedPlan), ("dst", PagedPlan),
+        ("src_data", C.c_void_p), ("dst_data", C.c_void_p), ("longest", C.c_int32), ("most_kept", C.c_int32),
+    ]
+
+
 EXCHANGE_MAX_RANKS = 16
 
 
@@ -171,6 +205,14 @@ def lib():
     L.hqmq_exchange_wait.argtypes = [C.POINTER(Exchange), C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p]
     L.hqmq_read_status.argtypes = [C.c_void_p, C.POINTER(C.c_uint32), C.c_void_p]
     L.hqmq_combine_partials.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]
+    L.hqmq_paged_plan_size.argtypes = [C.POINTER(PagedPlan), C.c_void_p, C.c_void_p]
+    L.hqmq_paged_plan_fill.argtypes = [C.POINTER(PagedPlan), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
+    for name in ("attn", "mass"):
+        size, call = getattr(L, f"hqmq_paged_{name}_workspace_bytes"), getattr(L, f"hqmq_paged_{name}")
+        size.restype, size.argtypes = C.c_size_t, [C.POINTER(PagedAttnArgs)]
+        call.argtypes = [C.POINTER(PagedAttnArgs), C.c_void_p, C.c_size_t, C.c_void_p]
+    L.hqmq_paged_store.argtypes = [C.POINTER(PagedStoreArgs), C.c_void_p]
+    L.hqmq_paged_evict.argtypes = [C.POINTER(PagedEvictArgs), C.c_void_p]
     if L.hqmq_abi_version() != ABI_VERSION:
         raise HqmqError("hqmq_b200: library ABI version mismatch; rebuild with `python -m hqmq_b200.build --force`")
     _lib = L

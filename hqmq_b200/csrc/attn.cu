@@ -236,7 +236,7 @@ static int resident_clusters(const void* kernel, size_t smem, int threads, int c
 
 cudaError_t raise_smem_limit(const void* kernel, size_t smem) {
   struct Entry { const void* k; int dev; };
-  static Entry done[64];
+  static Entry done[256];
   static int n_done = 0;
   static std::mutex mu;
   int dev = 0, optin = 0;
@@ -250,7 +250,7 @@ cudaError_t raise_smem_limit(const void* kernel, size_t smem) {
   if (rc != cudaSuccess) return rc;
   const int most = optin - (int)fa.sharedSizeBytes;
   rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most > (int)smem ? most : (int)smem);
-  if (rc == cudaSuccess && n_done < 64) done[n_done++] = {kernel, dev};
+  if (rc == cudaSuccess && n_done < 256) done[n_done++] = {kernel, dev};
   return rc;
 }
 

@@ -62,9 +62,37 @@ __host__ __device__ inline void pf_unit_tiles(const PrefillParams& p, int m, int
   n = hi > lo ? hi - lo : 1;
 }
 
+// The same of a unit of a ragged batch.
+template <int MODE>
+__device__ __forceinline__ void pf_tiles(const PrefillParams& p, int m, int& lo, int& n) {
+  if constexpr (MODE == 0) { pf_unit_tiles(p, m, lo, n); }
+  else { const int4 u = __ldg(p.units + 2 * m); lo = u.z; n = u.w; }
+}
+// The rows of a unit: number among the sequence's units, queries and keys of the sequence, offsets of its first query in Q and O.
+struct PfRows { int m, Tq, Tkv, scale, h; int64_t q0, o0; };
+template <int MODE>
+__device__ __forceinline__ PfRows pf_rows(const PrefillParams& p, int bh, int m) {
+  PfRows w;
+  if constexpr (MODE == 0) {
+    const int x = p.bh0 + bh, b = x / p.Hkv;
+    w.h = x - b * p.Hkv; w.m = m; w.Tq = p.Tq; w.Tkv = p.Tkv; w.scale = x;
+    w.q0 = (int64_t)b * p.qs_b; w.o0 = (int64_t)b * p.os_b;
+  } else {
+    const int4 u = __ldg(p.units + 2 * m), v = __ldg(p.units + 2 * m + 1);
+    w.h = p.h0 + bh; w.m = u.y; w.Tq = v.y; w.Tkv = v.x; w.scale = u.x * p.Hkv + w.h;
+    w.q0 = (int64_t)v.z * p.qs_t; w.o0 = (int64_t)v.z * p.os_t;
+  }
+  return w;
+}
+template <int MODE>
+__device__ __forceinline__ void pf_keys(const PrefillParams& p, const PfRows& w, int tq, int& beg, int& end) {
+  key_range(w.Tkv, w.Tq, MODE == 0 ? p.causal : 2, p.window, tq, beg, end);
+}
+
 struct PfPiece { int bh, m, tile0, n; bool head, tail; };
 // The pieces of one CTA.  Cut mode (p.L > 0): its stretch [c * L, (c + 1) * L) of the flat tile sequence, unit by unit.
 // Whole mode: units in order of m falling (with a causal mask: of length falling), dealt out to the CTAs to and fro.
+template <int MODE>
 struct PfIter {
   int left;                      // tiles left of the piece; whole mode: index of the next unit in the CTA's hand
   int bh, m, off, lo, n;
@@ -72,9 +100,9 @@ struct PfIter {
     if (p.L == 0) { left = 0; return; }
     const int64_t pos = (int64_t)cta * p.L;
     left = (int)(p.total - pos < p.L ? p.total - pos : p.L);
-    bh = (int)(pos / p.Wh);
-    m = p.start_m[cta]; off = p.start_off[cta];
-    pf_unit_tiles(p, m, lo, n);
+    if constexpr (MODE == 0) { bh = (int)(pos / p.Wh); m = p.start_m[cta]; off = p.start_off[cta]; }
+    else { const int4 st = __ldg(p.starts + cta); bh = st.x; m = st.y; off = st.z; }
+    pf_tiles<MODE>(p, m, lo, n);
   }
   __device__ __forceinline__ bool next(const PrefillParams& p, PfPiece& q) {
     if (p.L == 0) {
@@ -83,8 +111,8 @@ struct PfIter {
       if (i >= p.units_all) return false;
       ++left;
       const int n_bh = p.units_all / p.units_m, j = i / n_bh;
-      q.bh = i - j * n_bh; q.m = p.units_m - 1 - j;
-      pf_unit_tiles(p, q.m, q.tile0, q.n);
+      q.bh = i - j * n_bh; q.m = MODE == 0 ? p.units_m - 1 - j : __ldg(p.order + j);
+      pf_tiles<MODE>(p, q.m, q.tile0, q.n);
       q.head = q.tail = true;
       return true;
     }
@@ -92,7 +120,7 @@ struct PfIter {
     if (off >= n) {
       off = 0;
       if (++m == p.units_m) { m = 0; ++bh; }
-      pf_unit_tiles(p, m, lo, n);
+      pf_tiles<MODE>(p, m, lo, n);
     }
     q.bh = bh; q.m = m; q.tile0 = lo + off;
     q.n = n - off < left ? n - off : left;
@@ -180,8 +208,27 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// tanh for |x| <= 1/2, its series up to x^11 (the next term is under 4.4e-7), and anywhere: 1 - 2 / (e^2x + 1)
+__device__ __forceinline__ float2 cap_near(float2 x) {
+  const float2 q = mul2(x, x);
+  auto c = [](float v) { return make_float2(v, v); };
+  float2 y = fma2(q, c(-1382.f / 155925.f), c(62.f / 2835.f));
+  y = fma2(q, y, c(-17.f / 315.f));
+  y = fma2(q, y, c(2.f / 15.f));
+  y = fma2(q, y, c(-1.f / 3.f));
+  return fma2(mul2(q, y), x, x);
+}
+__device__ __forceinline__ float cap_exp(float x) { return 1.f - __fdividef(2.f, fast_exp2(2.885390081777927f * x) + 1.f); }
+// A row's sum with its head's sink (m: the row's maximum, exp2 domain); infinite where the sink is beyond all scores.
+__device__ __forceinline__ float with_sink(const PrefillParams& p, int head, float m, float l) {
+  if (m == -INFINITY) return l;
+  const float sk = __ldg(p.sinks + head) * 1.4426950408889634f - m;
+  return sk > 126.f ? INFINITY : l + fast_exp2(sk);
+}
+
 // ---- attend ----------------------------------------------------------------------------------------------------------------
-template <int D>
+// MODE 0: a batch of one length; 1: a ragged batch over pages; 2: that with capped scores.
+template <int D, int MODE>
 __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const PrefillParams p) {
   constexpr int NS = pf_stages(D);
   constexpr uint32_t TB = (uint32_t)pf_tile_bytes(D);
@@ -240,14 +287,17 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
   if (warp == 9) {
     // ================================ loader =====================================================================
     if (lane == 0) {
-      PfIter it;
+      PfIter<MODE> it;
       PfPiece q;
       it.init(p, (int)blockIdx.x);
       uint32_t g = 0;          // tiles issued
       bool ok = true;
       while (ok && it.next(p, q)) {
-        const unsigned char* kp = p.kimg + ((int64_t)q.bh * p.nt + (q.tile0 - p.kt0)) * TB;
-        const unsigned char* vp = p.vimg + ((int64_t)q.bh * p.nt + (q.tile0 - p.kt0)) * TB;
+        int64_t img;
+        if constexpr (MODE == 0) img = (int64_t)q.bh * p.nt + (q.tile0 - p.kt0);
+        else img = (int64_t)q.bh * p.img_tiles + __ldg(&p.units[2 * q.m + 1].w) + q.tile0;
+        const unsigned char* kp = p.kimg + img * TB;
+        const unsigned char* vp = p.vimg + img * TB;
         for (int i = 0; i < q.n; ++i, ++g) {
           const uint32_t st = g % NS, ph = (g / NS) & 1u;
           if (g >= NS && !wait(kempty + 8 * st, ph ^ 1u)) { ok = false; break; }
@@ -280,7 +330,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
     // ================================ MMA issuers: one warp per stream, converged ====================================
     // (A ready wait costs its warp about 200 clocks; with one warp for both streams the tensor cores ran dry meanwhile.)
     const int s = (warp - 8) / 2;
-    PfIter it;
+    PfIter<MODE> it;
     PfPiece q;
     it.init(p, (int)blockIdx.x);
     auto wait_w = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };   // one answer per warp
@@ -357,9 +407,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
     const int c_q = lane % QL;
     const uint32_t g_inv = 65536u / (uint32_t)p.G + 1u;                   // rw / G = rw * g_inv >> 16 for rw < 128
     auto load_q = [&](const PfPiece& w) {
-      const int bh = p.bh0 + w.bh, b = bh / p.Hkv, h = bh - b * p.Hkv;
-      const int64_t qb = (int64_t)b * p.qs_b + (int64_t)(h * p.G) * p.qs_h + 8 * c_q;
-      const int tq0 = (w.m * p.streams + s) * p.P;
+      const PfRows rw_ = pf_rows<MODE>(p, w.bh, w.m);
+      const int64_t qb = rw_.q0 + (int64_t)(rw_.h * p.G) * p.qs_h + 8 * c_q;
+      const int tq0 = (rw_.m * p.streams + s) * p.P, Tq = rw_.Tq;
       auto put = [&](int rw, uint4 v) {
         const uint32_t dst = sQ + s * TB + rw * 128 + (c_q >> 3) * 16384 + (((c_q & 7) ^ (rw & 7)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -368,7 +418,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
       if (p.q_vec) {
         // (offsets in the unit are 32-bit counts of 16 bytes: with 64-bit strides the addresses of eight loads took 1600 clocks)
         const uint4* qp = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.Q) + qb + (int64_t)tq0 * p.qs_t);
-        const int st_h = (int)(p.qs_h >> 3), st_t = (int)(p.qs_t >> 3), n_pos = min(p.P, p.Tq - tq0);
+        const int st_h = (int)(p.qs_h >> 3), st_t = (int)(p.qs_t >> 3), n_pos = min(p.P, Tq - tq0);
 #pragma unroll 1
         for (int k0 = 0; k0 < QL; k0 += 8) {
           uint4 v[8];
@@ -396,7 +446,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
           const int rw = rw0 + k * QR, pw = (int)((uint32_t)rw * g_inv >> 16), gw = rw - pw * p.G;
           const int64_t o = qb + (int64_t)gw * p.qs_h + (int64_t)(tq0 + pw) * p.qs_t;
           float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (pw < p.P && tq0 + pw < p.Tq) {
+          if (pw < p.P && tq0 + pw < Tq) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = load_float(p.Q, o + e, p.q_dtype);
           }
@@ -407,7 +457,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
       __syncwarp();
       if (lane == 0) mbar_arrive(qfull + 8 * s);
     };
-    PfIter it;
+    PfIter<MODE> it;
     PfPiece q, nq;
     it.init(p, (int)blockIdx.x);
     uint32_t g = 0, u = 0;
@@ -416,6 +466,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
     //  their NaN from the merge.)
     const bool lost = __ldcg(p.status) == p.epoch;
     int tq = 0;
+    PfRows w{};                                  // of the unit at hand
     bool live = false, w_live = false;
     float m_run = -INFINITY, vmul = 0.f;
     float2 l2 = make_float2(0.f, 0.f);
@@ -428,9 +479,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
         if (!ok) break;
         tc_fence_after();
         if (w_live) {
-          const int bh = p.bh0 + q.bh, b = bh / p.Hkv, h = bh - b * p.Hkv;
-          const float l = l2.x + l2.y;
+          float l = l2.x + l2.y;
           const bool whole = q.head && q.tail;
+          if constexpr (MODE != 0) { if (whole && p.sinks && live) l = with_sink(p, w.h * p.G + gh, m_run, l); }
           const float mul = whole ? (l != 0.f ? vmul / l : 0.f) : vmul;
           // a partial is stored four columns at a time ([d / 4][256 rows][4], then m and l of the rows), so that a lane stores 16 bytes
           // and its neighbours the next
@@ -441,8 +492,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int rw = (warp & 3) * 32 + 8 * k + (lane >> 2), pw = (int)((uint32_t)rw * g_inv >> 16), gw = rw - pw * p.G;
-            const int tw = (q.m * p.streams + s) * p.P + pw;
-            orow[k] = pw < p.P && tw < p.Tq ? reinterpret_cast<uint16_t*>(p.O) + (int64_t)b * p.os_b + (int64_t)(h * p.G + gw) * p.os_h +
+            const int tw = (w.m * p.streams + s) * p.P + pw;
+            orow[k] = pw < p.P && tw < w.Tq ? reinterpret_cast<uint16_t*>(p.O) + w.o0 + (int64_t)(w.h * p.G + gw) * p.os_h +
                                                   (int64_t)tw * p.os_t + (lane & 3) * 8 : nullptr;
           }
           const bool bf = p.o_dtype == HQMQ_BF16;
@@ -483,7 +534,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
               }
             } else {
               // any strides, any type: parked in shared memory (fp32) and stored an element at a time
-              const int64_t oo = (int64_t)b * p.os_b + (int64_t)(h * p.G + gh) * p.os_h + (int64_t)tq * p.os_t + c;
+              const int64_t oo = w.o0 + (int64_t)(w.h * p.G + gh) * p.os_h + (int64_t)tq * p.os_t + c;
               float* mine = reinterpret_cast<float*>(base + (stage - s_base)) + lane;      // [16][32 lanes]: half of the columns at a time
 #pragma unroll
               for (int e0 = 0; e0 < 32; e0 += 16) {
@@ -504,19 +555,22 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
       if (!more) break;
       q = nq;
       more = it.next(p, nq);
-      tq = (q.m * p.streams + s) * p.P + pl;
-      live = pl < p.P && tq < p.Tq;
+      w = pf_rows<MODE>(p, q.bh, q.m);
+      tq = (w.m * p.streams + s) * p.P + pl;
+      live = pl < p.P && tq < w.Tq;
       w_live = __any_sync(0xffffffffu, live);
       // this row's keys; the least and the most that a row of the warp sees.  (A row without a query is not written; its queries
       // are zero, and it takes whatever mask leaves the warp's loops alone.)
       int beg = 0, end = 0;
-      if (live) key_range(p.Tkv, p.Tq, p.causal, p.window, tq, beg, end);
+      if (live) pf_keys<MODE>(p, w, tq, beg, end);
       const int beg_lo = __reduce_min_sync(0xffffffffu, live ? beg : 0x7fffffff), beg_hi = __reduce_max_sync(0xffffffffu, live ? beg : 0);
       const int end_lo = __reduce_min_sync(0xffffffffu, live ? end : 0x7fffffff), end_hi = __reduce_max_sync(0xffffffffu, live ? end : 0);
       if (!live) { beg = beg_lo; end = end_hi; }
-      const float kmul = p.kmul[p.bh0 + q.bh];
-      vmul = lost ? NAN : p.vmul[p.bh0 + q.bh];
+      const float kmul = p.kmul[w.scale];
+      vmul = lost ? NAN : p.vmul[w.scale];
       const float2 kmul2 = make_float2(kmul, kmul);
+      float2 cap2 = kmul2;
+      if constexpr (MODE == 2) cap2 = make_float2(kmul * p.cap_in, kmul * p.cap_in);
       m_run = -INFINITY;
       l2 = make_float2(0.f, 0.f);
       for (int i = 0; i < q.n; ++i, ++g) {
@@ -552,7 +606,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1])));
-          const float mc = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kmul;
+          float mc = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kmul;
+          bool near = false;
+          if constexpr (MODE == 2) {
+            // the polynomial holds for scores of up to half the cap; a tile with a larger one, or a masked one, goes through exp2
+            float mn = INFINITY;
+#pragma unroll
+            for (int c = 0; c < 128; c += 2) mn = fminf(mn, fminf(__uint_as_float(r[c]), __uint_as_float(r[c + 1])));
+            near = __all_sync(0xffffffffu, fmaxf(mc, -mn * kmul) * p.cap_in <= 0.5f);
+            if (mc != -INFINITY) mc = cap_exp(mc * p.cap_in) * p.cap_log2;
+          }
           if (__any_sync(0xffffffffu, mc > m_run + kPfSlack)) {
             const float m_new = fmaxf(m_run, mc);
             const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
@@ -577,7 +640,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
           auto pairs_of = [&](int grp, uint32_t* pk) {          // 32 keys
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              float2 x = fma2(make_float2(__uint_as_float(r[32 * grp + 2 * e]), __uint_as_float(r[32 * grp + 2 * e + 1])), kmul2, nb2);
+              float2 x = make_float2(__uint_as_float(r[32 * grp + 2 * e]), __uint_as_float(r[32 * grp + 2 * e + 1]));
+              if constexpr (MODE == 2) {
+                const float2 y = mul2(x, cap2);
+                if (near) x = fma2(cap_near(y), make_float2(p.cap_log2, p.cap_log2), nb2);
+                else {
+                  x.x = x.x == -INFINITY ? x.x : fmaf(cap_exp(y.x), p.cap_log2, nb);
+                  x.y = x.y == -INFINITY ? x.y : fmaf(cap_exp(y.y), p.cap_log2, nb);
+                }
+              } else x = fma2(x, kmul2, nb2);
               x.x = fast_exp2(x.x); x.y = fast_exp2(x.y);
               const __half2 h = __float22half2_rn(x);
               // (the weights that are summed are the rounded ones the tensor cores see: the rounding cancels)
@@ -624,9 +695,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
     }
     // A wait ran out: the rows of this unit and of the CTA's others become NaN (of a unit that is cut, the merge's do).
     for (bool left = !ok; left;) {
-      const int bh = p.bh0 + q.bh, b = bh / p.Hkv, h = bh - b * p.Hkv, tn = (q.m * p.streams + s) * p.P + pl;
-      if (q.head && q.tail && pl < p.P && tn < p.Tq) {
-        const int64_t oo = (int64_t)b * p.os_b + (int64_t)(h * p.G + gh) * p.os_h + (int64_t)tn * p.os_t;
+      const PfRows lw = pf_rows<MODE>(p, q.bh, q.m);
+      const int tn = (lw.m * p.streams + s) * p.P + pl;
+      if (q.head && q.tail && pl < p.P && tn < lw.Tq) {
+        const int64_t oo = lw.o0 + (int64_t)(lw.h * p.G + gh) * p.os_h + (int64_t)tn * p.os_t;
 #pragma unroll 1
         for (int x = 0; x < D; ++x) store_float(p.O, oo + x, NAN, p.o_dtype);
       }
@@ -646,12 +718,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
 
 // ---- merge of the units that were cut between CTAs: blockIdx.x + 1 = a CTA whose piece starts inside a unit ----------------
 // blockIdx.y = 32 rows of the unit: a lane per row, a warp per D / 8 columns; the result is turned in shared memory.
-template <int D>
+template <int D, int MODE>
 __global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillParams p) {
   constexpr int E = D / 8;
   __shared__ float tile[32][D + 1];
   const int c = blockIdx.x + 1;
-  PfIter it;
+  PfIter<MODE> it;
   it.init(p, c);
   grid_dep_wait();                                          // (no CTA may outlive the kernel ahead of it)
   if (it.off == 0) return;                                  // the unit starts with the CTA
@@ -659,7 +731,7 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillParams 
   if ((int64_t)(c - 1) * p.L > s_u) return;                 // the unit's first boundary does the merge
   const int c0 = c - 1, n_parts = (int)((s_u + it.n - 1) / p.L) - c0 + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 32 + lane;
-  const int bh = p.bh0 + it.bh, b = bh / p.Hkv, h = bh - b * p.Hkv;
+  const PfRows w = pf_rows<MODE>(p, it.bh, it.m);
   // the CTA that holds the unit's first tile wrote its second slot, the others their first
   constexpr int64_t kSlot = 256 * (D + 2);
   const float* part = p.part + (int64_t)c0 * 2 * kSlot + row;
@@ -672,26 +744,30 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillParams 
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   for (int k = 0; k < n_parts; ++k) {
     const float* pp = slot(k);
-    const float w = fast_exp2(pp[D * 256] - mu);
-    l = fmaf(pp[(D + 1) * 256], w, l);
+    const float wk = fast_exp2(pp[D * 256] - mu);
+    l = fmaf(pp[(D + 1) * 256], wk, l);
     const float4* col = reinterpret_cast<const float4*>(pp - row) + warp * (E / 4) * 256 + row;
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
       const float4 v = col[e / 4 * 256];
-      acc[e] = fmaf(v.x, w, acc[e]); acc[e + 1] = fmaf(v.y, w, acc[e + 1]);
-      acc[e + 2] = fmaf(v.z, w, acc[e + 2]); acc[e + 3] = fmaf(v.w, w, acc[e + 3]);
+      acc[e] = fmaf(v.x, wk, acc[e]); acc[e + 1] = fmaf(v.y, wk, acc[e + 1]);
+      acc[e + 2] = fmaf(v.z, wk, acc[e + 2]); acc[e + 3] = fmaf(v.w, wk, acc[e + 3]);
     }
   }
   const bool failed = *p.status == p.epoch;                 // the attention kernel gave up on a wait
+  if constexpr (MODE != 0) {
+    const int pl = (row & 127) / p.G, gh = (row & 127) - pl * p.G;
+    if (p.sinks && row < 128 * p.streams && pl < p.P && (w.m * p.streams + (row >> 7)) * p.P + pl < w.Tq) l = with_sink(p, w.h * p.G + gh, m, l);
+  }
   const float inv = failed ? NAN : l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) tile[lane][warp * E + e] = acc[e] * inv;
   __syncthreads();
   for (int i = threadIdx.x; i < 32 * D / 2; i += 256) {
     const int rl = i / (D / 2), x = 2 * (i - rl * (D / 2)), r = blockIdx.y * 32 + rl, s = r >> 7, pl = (r & 127) / p.G, gh = (r & 127) - pl * p.G;
-    const int tq = (it.m * p.streams + s) * p.P + pl;
-    if (s >= p.streams || pl >= p.P || tq >= p.Tq) continue;
-    const int64_t oo = (int64_t)b * p.os_b + (int64_t)(h * p.G + gh) * p.os_h + (int64_t)tq * p.os_t + x;
+    const int tq = (w.m * p.streams + s) * p.P + pl;
+    if (s >= p.streams || pl >= p.P || tq >= w.Tq) continue;
+    const int64_t oo = w.o0 + (int64_t)(w.h * p.G + gh) * p.os_h + (int64_t)tq * p.os_t + x;
     const float f0 = tile[rl][x], f1 = tile[rl][x + 1];
     if (p.o_vec)
       *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.O) + oo) =
@@ -1022,8 +1098,8 @@ int prefill_launch(const hqmq_attn_args* a, const PrefillPlan& pl, void* workspa
   const size_t esmem = (size_t)e.table_rows * 8;
   const void* ek = N == 32 ? (a->layout == 0 ? (const void*)&prefill_expand_kernel<32, 0> : (const void*)&prefill_expand_kernel<32, 1>)
                            : (a->layout == 0 ? (const void*)&prefill_expand_kernel<16, 0> : (const void*)&prefill_expand_kernel<16, 1>);
-  const void* ak = d == 128 ? (const void*)&prefill_attn_kernel<128> : (const void*)&prefill_attn_kernel<64>;
-  const void* mk = d == 128 ? (const void*)&prefill_merge_kernel<128> : (const void*)&prefill_merge_kernel<64>;
+  const void* ak = d == 128 ? (const void*)&prefill_attn_kernel<128, 0> : (const void*)&prefill_attn_kernel<64, 0>;
+  const void* mk = d == 128 ? (const void*)&prefill_merge_kernel<128, 0> : (const void*)&prefill_merge_kernel<64, 0>;
   HQMQ_CHECK_CUDA(raise_smem_limit(ek, esmem));
   HQMQ_CHECK_CUDA(raise_smem_limit(ak, pf_smem_bytes(d)));
   for (int bh0 = 0; bh0 < bh_all; bh0 += pl.group) {
@@ -1066,3 +1142,5 @@ int prefill_launch(const hqmq_attn_args* a, const PrefillPlan& pl, void* workspa
 
 }  // namespace attn
 }  // namespace hqmq
+
+#include "paged_chunk.cuh"

@@ -34,6 +34,12 @@ struct PrefillParams {
   float* part;                                    // [CTA][2][256 rows x (d + 2)]: [d / 4][256][4], m [256], l [256]
   uint32_t* status; uint32_t epoch;
   int start_m[kPfMaxCtas], start_off[kPfMaxCtas];  // first unit of every CTA's piece, the unit's tiles before it
+  // a ragged batch over pages (paged_chunk.cuh): units from a list {sequence, m, lo, n}{kv, q, first row of Q, image tile - lo}, the
+  // (b, head)s are the heads of a group from h0 on
+  const int4* units; const int* order; const int4* starts;
+  int img_tiles, h0;
+  const float* sinks;                             // [H_q] or null
+  float cap_log2, cap_in;                         // cap on the scores in the exp2 domain, one over it (0: none)
 };
 
 struct ExpandParams {

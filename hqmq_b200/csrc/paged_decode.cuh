@@ -1,0 +1,510 @@
+// Attention of a few query rows per sequence over a paged cache: the kernel.
+//
+// The tile's arithmetic is that of the staged decode kernels (attn_kernel.cuh): S^T = K Q^T with the 16 tokens as rows and the query
+// rows as columns, O^T += V^T P^T, operands gathered from shared-memory tables straight into fragments.  What differs: a warp walks
+// its own stretch of tiles from unit to unit (paged.cuh); flagged chunks, which decode to zero, are put into the fragments before
+// their product (a lane owns 2 tokens x N / 4 chunks of K and 4 x N / 8 of V, and tests its own flag bits; which of the
+// steps have one at all is one word per tile), as fp16(x * qmax / rs), what the table would have given; V's scales enter P relative to the largest
+// one seen, a power of two that the accumulators are rescaled by like by the maximum, so that values of any size keep their bits.
+#pragma once
+#include "attn_tma.cuh"
+#include "paged_tile.cuh"
+
+namespace hqmq {
+namespace paged {
+
+struct DecodeParams {
+  PoolView pool;
+  QueryView q;
+  void* O; int o_dtype, o_vec; int64_t os_t, os_h;
+  const uint16_t* tblK; const uint16_t* tblV;
+  const float* sinks;
+  int table_rows, ib, row_bytes, repk, repv, window;
+  float kfac, cap_log2;          // kfac: what a product is multiplied by beside rs (softmax scale * log2 e / qmax, or with a cap 2 log2 e / cap times that)
+  float qmaxf, vfac;             // 1 / qmax
+  int sdt;
+  const int4* seqs; const int4* units; const int* base; const int* wunit; const int4* cuts; const int* tabs; const int* hdr;
+  int ctas;
+  float* parts;                  // [CTA][warps][2][part], then [CTA][2][part]
+};
+
+template <int N, int NB> __host__ __device__ constexpr int part_floats() { return NB * (N / 4 * 128 + 16); }
+
+// One finished row pair of a lane: value (i, e) of a part is head 2j + (e & 1), dim 4 (r NVG + i / 2) + 2 (i & 1) + e / 2.
+template <int N>
+__device__ __forceinline__ void emit_pair(const DecodeParams& p, const Seq& s, int h, int row, int rows, int r, int i, float a, float b) {
+  constexpr int NVG = Geo<N>::NVG;
+  if (row >= rows) return;
+  const int qi = row / p.q.G, g = row - qi * p.q.G, x = 4 * (r * NVG + (i >> 1)) + 2 * (i & 1);
+  const int64_t o = (int64_t)(s.q_off + qi) * p.os_t + (int64_t)(h * p.q.G + g) * p.os_h + x;
+  if (p.o_vec) {
+    *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.O) + o) =
+        (uint32_t)float_to_bits16(a, p.o_dtype) | ((uint32_t)float_to_bits16(b, p.o_dtype) << 16);
+  } else { store_float(p.O, o, a, p.o_dtype); store_float(p.O, o + 1, b, p.o_dtype); }
+}
+// What a row's sum is with its head's sink: m and l in the exp2 domain; returns 1 / l (0 for a row that saw nothing).
+__device__ __forceinline__ float inverse_sum(const DecodeParams& p, int h, int row, int rows, float m, float l) {
+  if (p.sinks && row < rows) {
+    const float sk = __ldg(p.sinks + h * p.q.G + row % p.q.G) * 1.4426950408889634f;
+    if (m == -INFINITY || sk - m > 126.f) return 0.f;
+    l += fast_exp2(sk - m);
+  }
+  return l != 0.f ? 1.f / l : 0.f;
+}
+
+// The parts of a unit, element `idx` of [NB][N / 4][32] quadruples: merged value and the row pair's maxima and sums.
+template <int N, int NB, typename PartOf>
+__device__ __forceinline__ void merge_parts(int idx, int n, const PartOf& part_of, float4& v, float2& m, float2& l) {
+  constexpr int PER = N / 4 * 32;
+  const int nb = idx / PER, j = idx & 3;
+  m = make_float2(-INFINITY, -INFINITY);
+  const int at = NB * PER * 4 + nb * 16 + 2 * j;
+  for (int k = 0; k < n; ++k) {
+    const float2 mk = __ldcg(reinterpret_cast<const float2*>(part_of(k) + at));
+    m.x = fmaxf(m.x, mk.x); m.y = fmaxf(m.y, mk.y);
+  }
+  const float ux = m.x == -INFINITY ? 0.f : m.x, uy = m.y == -INFINITY ? 0.f : m.y;
+  v = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < n; ++k) {
+    const float* pk = part_of(k);
+    const float2 mk = __ldcg(reinterpret_cast<const float2*>(pk + at)), lk = __ldcg(reinterpret_cast<const float2*>(pk + at + 8));
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(pk) + idx);
+    const float wx = fast_exp2(mk.x - ux), wy = fast_exp2(mk.y - uy);
+    l.x = fmaf(lk.x, wx, l.x); l.y = fmaf(lk.y, wy, l.y);
+    v.x = fmaf(x.x, wx, v.x); v.y = fmaf(x.y, wy, v.y); v.z = fmaf(x.z, wx, v.z); v.w = fmaf(x.w, wy, v.w);
+  }
+}
+template <int N, int NB>
+__device__ __forceinline__ void emit_merged(const DecodeParams& p, int u, int h, int idx, float4 v, float2 m, float2 l) {
+  constexpr int PER = N / 4 * 32;
+  const int4 un = __ldg(p.units + u), sq = __ldg(p.seqs + un.x);
+  const Seq s{sq.x, sq.y, sq.z, sq.w};
+  const int rows = s.q * p.q.G, nb = idx / PER, i = (idx - nb * PER) >> 5, lane = idx & 31, row = nb * 8 + 2 * (lane & 3);
+  const float ia = inverse_sum(p, h, row, rows, m.x, l.x), ib = inverse_sum(p, h, row + 1, rows, m.y, l.y);
+  emit_pair<N>(p, s, h, row, rows, lane >> 2, i, v.x * ia, v.z * ia);
+  emit_pair<N>(p, s, h, row + 1, rows, lane >> 2, i, v.y * ib, v.w * ib);
+}
+
+template <int N, int IB, int RB, int NB, bool OUTL>
+__global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1) paged_decode_kernel(const DecodeParams p) {
+  using FL = FastLoader<N, IB ? IB : 12, IB ? RB : 4, true>;
+  constexpr int NKS = Geo<N>::NKS, NVG = Geo<N>::NVG, NOT = 2 * NVG;
+  constexpr int NW = NB == 1 ? kDecWarps : kDecWarpsWide, THREADS = NW * 32, PART = part_floats<N, NB>();
+  const int ROW = IB ? row_bytes_of<N, IB, RB>() : p.row_bytes;
+  const TileLayout L = tile_layout(ROW, true, OUTL);
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const uint32_t strideK = 8u << p.repk, strideV = 8u << p.repv;
+  unsigned char* tblK = smem_raw;
+  unsigned char* tblV = smem_raw + (size_t)(p.table_rows >> 1) * strideK;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 3, r = lane >> 2;
+  unsigned char* ring = tblV + (size_t)(p.table_rows >> 1) * strideV + (size_t)warp * kTileStages * L.bytes;
+  const uint32_t ring32 = smem_u32(ring);
+  grid_dep_launch();
+  const int h = (int)blockIdx.x / p.ctas, k = (int)blockIdx.x - h * p.ctas;
+  const int n_units = p.hdr[0], total = p.hdr[1], n_warps = p.ctas * NW;
+  const int w = k * NW + warp;
+  const int f0 = stretch_begin(w, total, n_warps), f1 = stretch_begin(w + 1, total, n_warps);
+  const int c0 = stretch_begin(k * NW, total, n_warps), c1 = stretch_begin((k + 1) * NW, total, n_warps);
+  if (c0 >= c1) return;
+
+  // ---- the first tiles on their way, then the tables -----------------------------------------------------------------------
+  TileIter it;                       // the tile to be staged next
+  int n = f1 - f0;
+  it.left = n;
+  if (n > 0) {
+    it.u = __ldg(p.wunit + w);
+    it.unit(p.units, p.seqs, f0 - __ldg(p.base + it.u));
+  }
+  auto stage = [&](int i) {          // tile i of the stretch, which `it` is at
+    const int page = __ldg(p.tabs + it.tab + ((it.tile * kTile) >> p.pool.page_bits));
+    const int st = i % kTileStages;
+    stage_tile<true, OUTL>(p.pool, L, ROW, ring32 + st * L.bytes, ring + st * L.bytes, h, page, it.tile, lane);
+    it.next(p.units, p.seqs);
+  };
+  if (n > 0) stage(0);
+  if (n > 1) stage(1);
+  cp_commit();
+  load_table<THREADS>(tblK, p.tblK, h, p.table_rows, p.repk);
+  load_table<THREADS>(tblV, p.tblV, h, p.table_rows, p.repv);
+  __syncthreads();
+  if constexpr (OUTL) {
+    cp_wait_all();
+    __syncwarp();
+    if (n > 0) stage_values<true>(p.pool, L, ring32, ring, h, lane);
+    cp_commit();
+  }
+
+  const uint32_t laneK = (uint32_t)(lane & ((1 << p.repk) - 1)) * 8u, laneV = (uint32_t)(lane & ((1 << p.repv) - 1)) * 8u;
+  // (rows of 64 bytes: the odd groups of lanes take their pair of V's tokens in the other order, which spreads the loads over the banks)
+  constexpr bool kSwz = IB != 0 && row_bytes_of<N, IB, RB>() % 128 == 64;
+  const int vswz = kSwz ? (j & 1) : 0;
+  FL ld;
+  ld.row_bytes = ROW; ld.row_words = ROW / 4; ld.j = j; ld.r = r; ld.sdt = p.sdt;
+  const float kfac = p.kfac;
+  float* my_parts = p.parts + ((size_t)blockIdx.x * NW + warp) * 2 * PART;
+
+  int u = n > 0 ? __ldg(p.wunit + w) : 0, i = 0;
+  bool first_seg = true;
+  while (i < n) {
+    // ---- a unit, or what the stretch has of it ------------------------------------------------------------------------------
+    const int4 un = __ldg(p.units + u), sq4 = __ldg(p.seqs + un.x);
+    const Seq s{sq4.x, sq4.y, sq4.z, sq4.w};
+    const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
+    const int rows = s.q * p.q.G;
+    uint32_t qb[NB][NKS][2];
+    float qmul[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float mul = load_query<NKS>(qb[nb], p.q, s.q_off, h, nb * 8 + r, rows, j);
+      qmul[nb][0] = __shfl_sync(0xffffffffu, mul, 8 * j) * kfac;
+      qmul[nb][1] = __shfl_sync(0xffffffffu, mul, 8 * j + 4) * kfac;
+    }
+    const int p_first = s.kv - s.q, edge_lo = p.window > 0 ? s.kv - p.window : 0;    // (the last query sees nothing before edge_lo)
+    float m_run[NB][2], l_run[NB][2], o[NB][NOT][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      m_run[nb][0] = m_run[nb][1] = -INFINITY;
+      l_run[nb][0] = l_run[nb][1] = 0.f;
+#pragma unroll
+      for (int x = 0; x < NOT; ++x) o[nb][x][0] = o[nb][x][1] = o[nb][x][2] = o[nb][x][3] = 0.f;
+    }
+    float v_pow = 0.f, v_inv = 0.f;        // the power of two that V's scales are relative to (0: none yet), and one over it
+    const int i_end = min(n, i + (un.w - (un.z + (f0 + i - b0))));
+    int tile = un.z + (f0 + i - b0);
+    for (; i < i_end; ++i, ++tile) {
+      cp_wait_all();
+      __syncwarp();
+      if constexpr (OUTL) {
+        if (i + 1 < n) { const int st = (i + 1) % kTileStages; stage_values<true>(p.pool, L, ring32 + st * L.bytes, ring + st * L.bytes, h, lane); }
+      }
+      if (i + 2 < n) stage(i + 2);
+      cp_commit();
+      const unsigned char* sp = ring + (i % kTileStages) * L.bytes;
+      const int t0 = tile * kTile;
+      const bool edge = t0 + kTile > p_first + 1 || t0 < edge_lo;
+
+      // ---- this lane's fields, scales and flags ------------------------------------------------------------------------------
+      uint32_t kw[2][FL::KW + 1], vw[4][FL::VW + 1];
+      float ksc[2], vsc[2];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int t = nt * 8 + r;
+        if constexpr (IB != 0) ld.template load_span<FL::KW, FL::LK>(kw[nt], sp + t * ROW, j, true);
+        ksc[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt);
+        vsc[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsv)[t], p.sdt) * p.vfac;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = 2 * j + ((x & 1) ^ vswz) + (x >> 1) * 8;
+        if constexpr (IB != 0) ld.template load_span<FL::VW, FL::LV>(vw[x], sp + L.v + t * ROW, r, !edge || t0 + t < s.kv);
+      }
+      uint32_t kstep = 0u, vstep = 0u;       // bit x: some lane has a flagged chunk in step x
+      uint32_t fk[2] = {0u, 0u}, fk_pre[2] = {0u, 0u}, before = 0u;
+      if constexpr (OUTL) {
+        uint32_t fk_t = 0u, fv_t = 0u;
+        if (lane < kTile && t0 + lane < s.kv) {
+          if (p.pool.K.flags) fk_t = reinterpret_cast<const uint32_t*>(sp + L.flk)[lane];
+          if (p.pool.V.flags) fv_t = reinterpret_cast<const uint32_t*>(sp + L.flv)[lane];
+        }
+        kstep = __reduce_or_sync(0xffffffffu, fk_t);
+        vstep = __reduce_or_sync(0xffffffffu, fv_t);
+        if (kstep | vstep) {
+          before = counts_before(__popc(fk_t) | (__popc(fv_t) << 16), lane);
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            fk[nt] = __shfl_sync(0xffffffffu, fk_t, nt * 8 + r);
+            fk_pre[nt] = __shfl_sync(0xffffffffu, before, nt * 8 + r) & 0xffffu;
+          }
+        }
+        // chunks j * NKS + ks / r * NVG + g: which ks, which g
+        if constexpr (NKS == 8) { kstep |= kstep >> 16; kstep |= kstep >> 8; kstep &= 0xffu; }
+        else { kstep |= kstep >> 8; kstep |= kstep >> 4; kstep &= 0xfu; }
+        if constexpr (NVG == 4) { vstep |= vstep >> 16; vstep |= vstep >> 8; vstep |= vstep >> 4; vstep &= 0xfu; }
+        else { vstep |= vstep >> 8; vstep |= vstep >> 4; vstep |= vstep >> 2; vstep &= 3u; }
+      }
+      const int64_t ph = OUTL ? (int64_t)*reinterpret_cast<const int*>(sp + L.off + 16) * p.pool.Hkv + h : 0;
+
+      // ---- S^T = K Q^T ---------------------------------------------------------------------------------------------------------
+      float sc[NB][4], s2[NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[nb][x] = s2[nb][x] = 0.f;
+      float kinv[2];
+      if constexpr (OUTL) {
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) kinv[nt] = ksc[nt] != 0.f ? __fdividef(p.qmaxf, ksc[nt]) : 0.f;
+      }
+      static_for<0, NKS>([&](auto ks_) {
+        constexpr int ks = decltype(ks_)::value;
+        uint32_t a[4];
+        static_for<0, 2>([&](auto nt_) {
+          constexpr int nt = decltype(nt_)::value;
+          uint32_t idx; __half2 rr;
+          if constexpr (IB != 0) FL::template cut<ks>(kw[nt], idx, rr);
+          else cut_any(reinterpret_cast<const uint32_t*>(sp + (nt * 8 + r) * ROW), j * NKS + ks, p.ib, p.ib + p.pool.K.radius_bits, idx, rr);
+          const uint2 cw = *reinterpret_cast<const uint2*>(tblK + (idx * strideK + laneK));
+          a[nt] = hmul2_u32(cw.x, rr);
+          a[2 + nt] = hmul2_u32(cw.y, rr);
+        });
+        if constexpr (OUTL) {
+          if (kstep & (1u << ks)) {
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+              const int c = j * NKS + ks;
+              if ((fk[nt] >> c) & 1u) {
+                const uint32_t rel = fk_pre[nt] + __popc(fk[nt] & ((1u << c) - 1u));
+                const float4 x = values_of(flagged_value(p.pool.K, sp, L.payk, reinterpret_cast<const uint32_t*>(sp + L.off)[0], rel, ph), p.pool.K.out_dtype);
+                a[nt] = pack_half2(x.x * kinv[nt], x.y * kinv[nt]);
+                a[2 + nt] = pack_half2(x.z * kinv[nt], x.w * kinv[nt]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma16816((ks & 1) ? s2[nb] : sc[nb], a[0], a[1], a[2], a[3], qb[nb][ks][0], qb[nb][ks][1]);
+      });
+
+      // ---- scale, cap, mask -----------------------------------------------------------------------------------------------------
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[nb][x] = (sc[nb][x] + s2[nb][x]) * (ksc[x >> 1] * qmul[nb][x & 1]);
+      if (p.cap_log2 > 0.f) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[nb][x] = capped(sc[nb][x], p.cap_log2);
+      }
+      if (edge) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int t = t0 + (x >> 1) * 8 + r, pos = min(p_first + (nb * 8 + 2 * j + (x & 1)) / p.q.G, s.kv - 1);
+            if (t > pos || (p.window > 0 && t <= pos - p.window)) sc[nb][x] = -INFINITY;
+          }
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+          if (t0 + nt * 8 + r >= s.kv) vsc[nt] = 0.f;
+      }
+
+      // ---- maxima: raised, with the accumulators, only where a score exceeds one by 2^4, or V's scale its power ---------------------
+      constexpr float kSlack = 4.f;
+      bool need = fmaxf(vsc[0], vsc[1]) > v_pow;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) need |= fmaxf(sc[nb][e], sc[nb][2 + e]) > m_run[nb][e] + kSlack;
+      if (__any_sync(0xffffffffu, need)) {
+        float big = fmaxf(vsc[0], vsc[1]);
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 4));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 8));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
+        float vs = 1.f;
+        if (big > v_pow) {
+          // the next power of two, within 2^-100 .. 2^100
+          const int e = min(100, max(-100, (int)(__float_as_uint(big) >> 23) - 126));
+          const float np = __uint_as_float((uint32_t)(127 + e) << 23);
+          vs = v_pow * __uint_as_float((uint32_t)(127 - e) << 23);
+          v_pow = np;
+          v_inv = __uint_as_float((uint32_t)(127 - e) << 23);
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float m = fmaxf(sc[nb][e], sc[nb][2 + e]);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            const float m_new = fmaxf(m_run[nb][e], m);
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[nb][e] - m_new);
+            m_run[nb][e] = m_new;
+            l_run[nb][e] *= alpha;
+            const float oa = alpha * vs;
+#pragma unroll
+            for (int x = 0; x < NOT; ++x) { o[nb][x][e] *= oa; o[nb][x][2 + e] *= oa; }
+          }
+      }
+
+      // ---- P: fp16(p * scale of V); the weights summed are those rounded products divided by the scale, so the rounding cancels ------
+      uint32_t pb[NB][2];
+      const float vn[2] = {vsc[0] * v_inv, vsc[1] * v_inv};
+      const float iv[2] = {vn[0] > 0.f ? rcp_approx(vn[0]) : 0.f, vn[1] > 0.f ? rcp_approx(vn[1]) : 0.f};
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float pr[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) pr[x] = fast_exp2(sc[nb][x] - (m_run[nb][x & 1] == -INFINITY ? 0.f : m_run[nb][x & 1]));
+        const __half2 h0 = __floats2half2_rn(pr[0] * vn[0], pr[1] * vn[0]), h1 = __floats2half2_rn(pr[2] * vn[1], pr[3] * vn[1]);
+        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
+        // (a token whose scale is far below the largest one has products that fp16 does not hold: its weight is taken as it is)
+        const bool ok0 = vn[0] > 0.0009765625f, ok1 = vn[1] > 0.0009765625f;
+        l_run[nb][0] += (ok0 ? g0.x * iv[0] : pr[0]) + (ok1 ? g1.x * iv[1] : pr[2]);
+        l_run[nb][1] += (ok0 ? g0.y * iv[0] : pr[1]) + (ok1 ? g1.y * iv[1] : pr[3]);
+        pb[nb][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h0));
+        pb[nb][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h1));
+        if (vswz) { pb[nb][0] = __byte_perm(pb[nb][0], 0u, 0x1032); pb[nb][1] = __byte_perm(pb[nb][1], 0u, 0x1032); }
+      }
+
+      // ---- O^T += V^T P^T ---------------------------------------------------------------------------------------------------------
+      uint32_t fv[4] = {0u, 0u, 0u, 0u}, fv_pre[4] = {0u, 0u, 0u, 0u};
+      float vi[4] = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (OUTL) {
+        if (vstep) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int t = 2 * j + ((x & 1) ^ vswz) + (x >> 1) * 8;
+            fv_pre[x] = __shfl_sync(0xffffffffu, before, t) >> 16;
+            fv[x] = t0 + t < s.kv ? reinterpret_cast<const uint32_t*>(sp + L.flv)[t] : 0u;
+            const float rs = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsv)[t], p.sdt);
+            vi[x] = rs != 0.f ? __fdividef(p.qmaxf, rs) : 0.f;
+          }
+        }
+      }
+      static_for<0, NVG>([&](auto g_) {
+        constexpr int g = decltype(g_)::value;
+        uint32_t lo[4], hi[4];
+        static_for<0, 4>([&](auto x_) {
+          constexpr int x = decltype(x_)::value;
+          uint32_t idx; __half2 rr;
+          if constexpr (IB != 0) FL::template cut<g>(vw[x], idx, rr);
+          else {
+            const int t = 2 * j + (x & 1) + (x >> 1) * 8;
+            cut_any(reinterpret_cast<const uint32_t*>(sp + L.v + t * ROW), r * NVG + g, p.ib, p.ib + p.pool.V.radius_bits, idx, rr);
+            if (edge && t0 + t >= s.kv) { idx = 0u; rr = __float2half2_rn(0.f); }
+          }
+          const uint2 cw = *reinterpret_cast<const uint2*>(tblV + (idx * strideV + laneV));
+          lo[x] = hmul2_u32(cw.x, rr);
+          hi[x] = hmul2_u32(cw.y, rr);
+        });
+        if constexpr (OUTL) {
+          if (vstep & (1u << g)) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int c = r * NVG + g;
+              if ((fv[x] >> c) & 1u) {
+                const uint32_t rel = fv_pre[x] + __popc(fv[x] & ((1u << c) - 1u));
+                const float4 y = values_of(flagged_value(p.pool.V, sp, L.payv, reinterpret_cast<const uint32_t*>(sp + L.off)[2], rel, ph), p.pool.V.out_dtype);
+                lo[x] = pack_half2(y.x * vi[x], y.y * vi[x]);
+                hi[x] = pack_half2(y.z * vi[x], y.w * vi[x]);
+              }
+            }
+          }
+        }
+        const uint32_t a0 = __byte_perm(lo[0], lo[1], 0x5410), a1 = __byte_perm(lo[0], lo[1], 0x7632);
+        const uint32_t a2 = __byte_perm(lo[2], lo[3], 0x5410), a3 = __byte_perm(lo[2], lo[3], 0x7632);
+        const uint32_t e0 = __byte_perm(hi[0], hi[1], 0x5410), e1 = __byte_perm(hi[0], hi[1], 0x7632);
+        const uint32_t e2 = __byte_perm(hi[2], hi[3], 0x5410), e3 = __byte_perm(hi[2], hi[3], 0x7632);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          mma16816(o[nb][2 * g], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
+          mma16816(o[nb][2 * g + 1], e0, e1, e2, e3, pb[nb][0], pb[nb][1]);
+        }
+      });
+    }
+
+    // ---- the unit's result, or a part of it --------------------------------------------------------------------------------------
+    const bool whole = b0 >= f0 && b1 <= f1;
+    float* part = my_parts + (first_seg ? 0 : PART);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float li[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l = l_run[nb][e];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        l_run[nb][e] = l;
+        li[e] = whole ? inverse_sum(p, h, nb * 8 + 2 * j + e, rows, m_run[nb][e], l) * v_pow : v_pow;
+      }
+#pragma unroll
+      for (int x = 0; x < NOT; ++x) {
+        const float4 v = make_float4(o[nb][x][0] * li[0], o[nb][x][1] * li[1], o[nb][x][2] * li[0], o[nb][x][3] * li[1]);
+        if (whole) {
+          emit_pair<N>(p, s, h, nb * 8 + 2 * j, rows, r, x, v.x, v.z);
+          emit_pair<N>(p, s, h, nb * 8 + 2 * j + 1, rows, r, x, v.y, v.w);
+        } else {
+          reinterpret_cast<float4*>(part)[(nb * NOT + x) * 32 + lane] = v;
+        }
+      }
+      if (!whole && r == 0) {
+        float* ml = part + NB * NOT * 128 + nb * 16 + 2 * j;
+        ml[0] = m_run[nb][0]; ml[1] = m_run[nb][1]; ml[8] = l_run[nb][0]; ml[9] = l_run[nb][1];
+      }
+    }
+    first_seg = false;
+    ++u;
+  }
+  __syncthreads();
+
+  // ---- units cut between this CTA's warps -----------------------------------------------------------------------------------------
+  // (every warp's first segment left its part in slot 0, a later one that is cut, the stretch's last, in slot 1)
+  const float* cta_parts = p.parts + (size_t)blockIdx.x * NW * 2 * PART;
+  float* out_parts = p.parts + ((size_t)gridDim.x * NW + blockIdx.x) * 2 * PART;
+  for (int v = __ldg(p.wunit + k * NW); v < n_units; ++v) {
+    const int b0 = __ldg(p.base + v), b1 = __ldg(p.base + v + 1);
+    if (b0 >= c1) break;
+    const int wa = warp_of(b0, total, n_warps), wb = warp_of(b1 - 1, total, n_warps);
+    if (wa == wb) continue;
+    const int la = max(wa - k * NW, 0), lb = min(wb - k * NW, NW - 1);
+    const int first_slot = b0 > stretch_begin(k * NW + la, total, n_warps) ? 1 : 0;
+    auto part_of = [&](int x) { return cta_parts + ((la + x) * 2 + (x == 0 ? first_slot : 0)) * PART; };
+    const bool done = wa >= k * NW && wb < (k + 1) * NW;
+    for (int idx = threadIdx.x; idx < NB * NOT * 32; idx += THREADS) {
+      float4 x; float2 m, l;
+      merge_parts<N, NB>(idx, lb - la + 1, part_of, x, m, l);
+      if (done) emit_merged<N, NB>(p, v, h, idx, x, m, l);
+      else {
+        float* dst = out_parts + (b0 > c0 ? PART : 0);
+        reinterpret_cast<float4*>(dst)[idx] = x;
+        const int nb = idx / (NOT * 32), i_ = (idx - nb * NOT * 32) >> 5;
+        if (i_ == 0 && (idx & 31) < 4) {
+          float* ml = dst + NB * NOT * 128 + nb * 16 + 2 * (idx & 3);
+          ml[0] = m.x; ml[1] = m.y; ml[8] = l.x; ml[9] = l.y;
+        }
+      }
+    }
+  }
+}
+
+// Units cut between CTAs: blockIdx.x = the cut, blockIdx.y = KV head.
+template <int N, int NB>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const DecodeParams p) {
+  constexpr int NW = NB == 1 ? kDecWarps : kDecWarpsWide, PART = part_floats<N, NB>();
+  grid_dep_wait();
+  if ((int)blockIdx.x >= p.hdr[5]) return;
+  const int4 c = __ldg(p.cuts + blockIdx.x);
+  const int h = blockIdx.y, grid = p.ctas * (int)gridDim.y;
+  const float* base = p.parts + ((size_t)grid * NW + (size_t)h * p.ctas) * 2 * PART;
+  auto part_of = [&](int x) { return base + ((size_t)(c.y + x) * 2 + (x == 0 ? c.w : 0)) * PART; };
+  for (int idx = threadIdx.x; idx < NB * N / 4 * 32; idx += 256) {
+    float4 x; float2 m, l;
+    merge_parts<N, NB>(idx, c.z - c.y + 1, part_of, x, m, l);
+    emit_merged<N, NB>(p, c.x, h, idx, x, m, l);
+  }
+}
+
+struct DecodeKernels { const void* decode; const void* merge; };
+DecodeKernels decode_kernels_128(int ib, int rb, int nb, bool outl);
+DecodeKernels decode_kernels_64(int ib, int rb, int nb, bool outl);
+
+template <int N, int NB, bool OUTL>
+const void* pick_decode(int ib, int rb) {
+  if (ib == 10 && rb == 3) return (const void*)&paged_decode_kernel<N, 10, 3, NB, OUTL>;
+  if (ib == 12 && rb == 4) return (const void*)&paged_decode_kernel<N, 12, 4, NB, OUTL>;
+  if (ib == 13 && rb == 6) return (const void*)&paged_decode_kernel<N, 13, 6, NB, OUTL>;
+  return (const void*)&paged_decode_kernel<N, 0, 0, NB, OUTL>;
+}
+template <int N>
+DecodeKernels pick_kernels(int ib, int rb, int nb, bool outl) {
+  if (nb == 1) return {outl ? pick_decode<N, 1, true>(ib, rb) : pick_decode<N, 1, false>(ib, rb), (const void*)&paged_merge_kernel<N, 1>};
+  return {outl ? pick_decode<N, 2, true>(ib, rb) : pick_decode<N, 2, false>(ib, rb), (const void*)&paged_merge_kernel<N, 2>};
+}
+
+}  // namespace paged
+}  // namespace hqmq

@@ -1,0 +1,344 @@
+// The softmax weight that every key of a paged cache receives: kernels.
+//
+//   scores  the decode kernel's K side (paged_decode.cuh): every warp walks its stretch of tiles, writes the scores of its rows, in the
+//           exp2 domain and fp32, and keeps their running maxima and sums.  A weight is compared and accumulated over many steps, so
+//           products are kept whole: a codeword times its radius code has 17 bits and a flagged value times qmax / rs 24; each is the sum
+//           of two fp16 operands, hi + lo, of two products (fp16 alone: relative error of a weight 1e-3; so 1e-6).  Q is fp16 after
+//           division by a power of two: exact for fp16 and bf16, but for what is 2^-24 of the row's largest.
+//   sum     per 512 tokens of a sequence: exp2(score - m) / l over the rows, on top of decay * prior.  Every token has one owner, so
+//           nothing is added in an order of its own (no atomics).
+// The scores go through memory between the two (R rows x 4 bytes a token, against 50 to 80 bytes of codes): a second decoding pass
+// would cost the gathers and products again, which bound the first.
+#pragma once
+#include "attn_tma.cuh"
+#include "paged_tile.cuh"
+
+namespace hqmq {
+namespace paged {
+
+struct MassParams {
+  PoolView pool;
+  QueryView q;
+  const uint16_t* tblK;
+  const float* sinks;
+  int table_rows, ib, row_bytes, repk, window;
+  float kfac, cap, cap_in;       // cap (exp2 domain) * tanh(x * cap_in)
+  float qmaxf;
+  int sdt;
+  const int4* seqs; const int4* units; const int* base; const int* wunit; const int4* groups; const int* tabs; const int* hdr;
+  int ctas;
+  float* scores;                 // [head][tile of the flat sequence][16][rows of a unit]
+  float2* parts;                 // [CTA][warps][2][rows]
+  float2* cta_parts;             // [CTA][2][rows]
+  float2* stats;                 // [head][unit][rows]: units that no CTA boundary cuts
+  const float* prior; float* mass; float decay;
+};
+
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {        // (m, l) of two parts
+  const float m = fmaxf(a.x, b.x), u = m == -INFINITY ? 0.f : m;
+  return make_float2(m, a.y * fast_exp2(a.x - u) + b.y * fast_exp2(b.x - u));
+}
+
+template <int N, int IB, int RB, int NB, bool OUTL>
+__global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const MassParams p) {
+  using FL = FastLoader<N, IB ? IB : 12, IB ? RB : 4, true>;
+  constexpr int NKS = Geo<N>::NKS, NW = kMassWarps, THREADS = NW * 32, R = 8 * NB;
+  const int ROW = IB ? row_bytes_of<N, IB, RB>() : p.row_bytes;
+  const TileLayout L = tile_layout(ROW, false, OUTL);
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const uint32_t strideK = 8u << p.repk;
+  unsigned char* tblK = smem_raw;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 3, r = lane >> 2;
+  unsigned char* ring = tblK + (size_t)(p.table_rows >> 1) * strideK + (size_t)warp * kTileStages * L.bytes;
+  const uint32_t ring32 = smem_u32(ring);
+  grid_dep_launch();
+  const int h = (int)blockIdx.x / p.ctas, k = (int)blockIdx.x - h * p.ctas;
+  const int n_units = p.hdr[2], total = p.hdr[3], n_warps = p.ctas * NW;
+  const int w = k * NW + warp;
+  const int f0 = stretch_begin(w, total, n_warps), f1 = stretch_begin(w + 1, total, n_warps);
+  const int c0 = stretch_begin(k * NW, total, n_warps), c1 = stretch_begin((k + 1) * NW, total, n_warps);
+  if (c0 >= c1) return;
+
+  TileIter it;
+  int n = f1 - f0;
+  it.left = n;
+  if (n > 0) {
+    it.u = __ldg(p.wunit + w);
+    it.unit(p.units, p.seqs, f0 - __ldg(p.base + it.u));
+  }
+  auto stage = [&](int i) {
+    const int page = __ldg(p.tabs + it.tab + ((it.tile * kTile) >> p.pool.page_bits));
+    const int st = i % kTileStages;
+    stage_tile<false, OUTL>(p.pool, L, ROW, ring32 + st * L.bytes, ring + st * L.bytes, h, page, it.tile, lane);
+    it.next(p.units, p.seqs);
+  };
+  if (n > 0) stage(0);
+  if (n > 1) stage(1);
+  cp_commit();
+  load_table<THREADS>(tblK, p.tblK, h, p.table_rows, p.repk);
+  __syncthreads();
+  if constexpr (OUTL) {
+    cp_wait_all();
+    __syncwarp();
+    if (n > 0) stage_values<false>(p.pool, L, ring32, ring, h, lane);
+    cp_commit();
+  }
+  const uint32_t laneK = (uint32_t)(lane & ((1 << p.repk) - 1)) * 8u;
+  FL ld;
+  ld.row_bytes = ROW; ld.row_words = ROW / 4; ld.j = j; ld.r = r; ld.sdt = p.sdt;
+  float2* my_parts = p.parts + ((size_t)blockIdx.x * NW + warp) * 2 * R;
+
+  int u = n > 0 ? __ldg(p.wunit + w) : 0, i = 0;
+  bool first_seg = true;
+  while (i < n) {
+    const int4 un = __ldg(p.units + u), sq4 = __ldg(p.seqs + un.x);
+    const Seq s{sq4.x, sq4.y, sq4.z, sq4.w};
+    const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
+    const int rows = s.q * p.q.G, row0 = un.y;
+    uint32_t qb[NB][NKS][2];
+    float qmul[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float mul = load_query<NKS>(qb[nb], p.q, s.q_off, h, row0 + nb * 8 + r, rows, j);
+      qmul[nb][0] = __shfl_sync(0xffffffffu, mul, 8 * j);
+      qmul[nb][1] = __shfl_sync(0xffffffffu, mul, 8 * j + 4);
+    }
+    const int p_first = s.kv - s.q + row0 / p.q.G, p_last = s.kv - s.q + (min(row0 + R, rows) - 1) / p.q.G;
+    const int edge_lo = p.window > 0 ? p_last + 1 - p.window : 0;
+    float2 ml[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) ml[nb][0] = ml[nb][1] = make_float2(-INFINITY, 0.f);
+    const int i_end = min(n, i + (b1 - (f0 + i)));
+    int tile = un.z + (f0 + i - b0);
+    for (; i < i_end; ++i, ++tile) {
+      cp_wait_all();
+      __syncwarp();
+      if constexpr (OUTL) {
+        if (i + 1 < n) { const int st = (i + 1) % kTileStages; stage_values<false>(p.pool, L, ring32 + st * L.bytes, ring + st * L.bytes, h, lane); }
+      }
+      if (i + 2 < n) stage(i + 2);
+      cp_commit();
+      const unsigned char* sp = ring + (i % kTileStages) * L.bytes;
+      const int t0 = tile * kTile;
+      const bool edge = t0 + kTile > p_first + 1 || t0 < edge_lo;
+      uint32_t kw[2][FL::KW + 1];
+      float rs[2];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int t = nt * 8 + r;
+        if constexpr (IB != 0) ld.template load_span<FL::KW, FL::LK>(kw[nt], sp + t * ROW, j, true);
+        rs[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt);
+      }
+      uint32_t kstep = 0u, fk[2] = {0u, 0u}, fk_pre[2] = {0u, 0u};
+      float kinv[2] = {0.f, 0.f};
+      if constexpr (OUTL) {
+        uint32_t fk_t = 0u;
+        if (lane < kTile && t0 + lane < s.kv) fk_t = reinterpret_cast<const uint32_t*>(sp + L.flk)[lane];
+        kstep = __reduce_or_sync(0xffffffffu, fk_t);
+        if (kstep) {
+          const uint32_t before = counts_before(__popc(fk_t), lane);
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            fk[nt] = __shfl_sync(0xffffffffu, fk_t, nt * 8 + r);
+            fk_pre[nt] = __shfl_sync(0xffffffffu, before, nt * 8 + r);
+            kinv[nt] = rs[nt] != 0.f ? __fdiv_rn(p.qmaxf, rs[nt]) : 0.f;
+          }
+        }
+        if constexpr (NKS == 8) { kstep |= kstep >> 16; kstep |= kstep >> 8; kstep &= 0xffu; }
+        else { kstep |= kstep >> 8; kstep |= kstep >> 4; kstep &= 0xfu; }
+      }
+      const int64_t ph = OUTL ? (int64_t)*reinterpret_cast<const int*>(sp + L.off + 16) * p.pool.Hkv + h : 0;
+      // two chains of the high halves' products and one of the low ones': the tensor cores cut a sum's bits with every step
+      float sc[NB][4], s2[NB][4], s3[NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[nb][x] = s2[nb][x] = s3[nb][x] = 0.f;
+      static_for<0, NKS>([&](auto ks_) {
+        constexpr int ks = decltype(ks_)::value;
+        uint32_t a[4], b[4];
+        static_for<0, 2>([&](auto nt_) {
+          constexpr int nt = decltype(nt_)::value;
+          uint32_t idx; __half2 rr;
+          if constexpr (IB != 0) FL::template cut<ks>(kw[nt], idx, rr);
+          else cut_any(reinterpret_cast<const uint32_t*>(sp + (nt * 8 + r) * ROW), j * NKS + ks, p.ib, p.ib + p.pool.K.radius_bits, idx, rr);
+          const uint2 cw = *reinterpret_cast<const uint2*>(tblK + (idx * strideK + laneK));
+          // hi = fl(c * r), lo = c * r - hi, which an fma gives exactly
+          auto split = [&](uint32_t c, uint32_t& hi, uint32_t& lo) {
+            const __half2 ch = *reinterpret_cast<const __half2*>(&c), hh = __hmul2(ch, rr), lh = __hfma2(ch, rr, __hneg2(hh));
+            hi = *reinterpret_cast<const uint32_t*>(&hh); lo = *reinterpret_cast<const uint32_t*>(&lh);
+          };
+          split(cw.x, a[nt], b[nt]);
+          split(cw.y, a[2 + nt], b[2 + nt]);
+        });
+        if constexpr (OUTL) {
+          if (kstep & (1u << ks)) {
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+              const int c = j * NKS + ks;
+              if ((fk[nt] >> c) & 1u) {
+                const uint32_t rel = fk_pre[nt] + __popc(fk[nt] & ((1u << c) - 1u));
+                const float4 x = values_of(flagged_value(p.pool.K, sp, L.payk, reinterpret_cast<const uint32_t*>(sp + L.off)[0], rel, ph), p.pool.K.out_dtype);
+                auto split = [&](float v0, float v1, uint32_t& hi, uint32_t& lo) {
+                  v0 *= kinv[nt]; v1 *= kinv[nt];
+                  hi = pack_half2(v0, v1);
+                  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                  lo = pack_half2(v0 - g.x, v1 - g.y);
+                };
+                split(x.x, x.y, a[nt], b[nt]);
+                split(x.z, x.w, a[2 + nt], b[2 + nt]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          mma16816((ks & 1) ? s2[nb] : sc[nb], a[0], a[1], a[2], a[3], qb[nb][ks][0], qb[nb][ks][1]);
+          mma16816(s3[nb], b[0], b[1], b[2], b[3], qb[nb][ks][0], qb[nb][ks][1]);
+        }
+      });
+      float* dst = p.scores + ((int64_t)h * total + f0 + i) * (kTile * R) + r * R + 2 * j;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float v = (sc[nb][x] + s2[nb][x] + s3[nb][x]) * (rs[x >> 1] * (p.kfac * qmul[nb][x & 1]));
+          if (p.cap > 0.f) v = p.cap * tanhf(v * p.cap_in);
+          if (edge) {
+            const int t = t0 + (x >> 1) * 8 + r, pos = min(p_first + (row0 % p.q.G + nb * 8 + 2 * j + (x & 1)) / p.q.G, s.kv - 1);
+            if (t > pos || (p.window > 0 && t <= pos - p.window)) v = -INFINITY;
+          }
+          sc[nb][x] = v;
+        }
+        // (each lane keeps the maximum and sum of its own tokens)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float m = fmaxf(sc[nb][e], sc[nb][2 + e]);
+          if (m > ml[nb][e].x) { ml[nb][e].y *= fast_exp2(ml[nb][e].x - m); ml[nb][e].x = m; }
+          const float b = ml[nb][e].x == -INFINITY ? 0.f : ml[nb][e].x;
+          ml[nb][e].y += fast_exp2(sc[nb][e] - b) + fast_exp2(sc[nb][2 + e] - b);
+        }
+        *reinterpret_cast<float2*>(dst + nb * 8) = make_float2(sc[nb][0], sc[nb][1]);
+        *reinterpret_cast<float2*>(dst + 8 * R + nb * 8) = make_float2(sc[nb][2], sc[nb][3]);
+      }
+    }
+    const bool whole = b0 >= f0 && b1 <= f1;
+    float2* dst = whole ? p.stats + ((int64_t)h * n_units + u) * R : my_parts + (first_seg ? 0 : R);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float2 v = ml[nb][e];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) v = joined(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+        if (r == 0) dst[nb * 8 + 2 * j + e] = v;
+      }
+    first_seg = false;
+    ++u;
+  }
+  __syncthreads();
+  // units cut between the CTA's warps
+  const float2* cta = p.parts + (size_t)blockIdx.x * NW * 2 * R;
+  for (int v = __ldg(p.wunit + k * NW); v < n_units; ++v) {
+    const int b0 = __ldg(p.base + v), b1 = __ldg(p.base + v + 1);
+    if (b0 >= c1) break;
+    const int wa = warp_of(b0, total, n_warps), wb = warp_of(b1 - 1, total, n_warps);
+    if (wa == wb) continue;
+    const int la = max(wa - k * NW, 0), lb = min(wb - k * NW, NW - 1);
+    const int first_slot = b0 > stretch_begin(k * NW + la, total, n_warps) ? 1 : 0;
+    float2* dst = wa >= k * NW && wb < (k + 1) * NW ? p.stats + ((int64_t)h * n_units + v) * R
+                                                    : p.cta_parts + ((size_t)blockIdx.x * 2 + (b0 > c0 ? 1 : 0)) * R;
+    for (int row = threadIdx.x; row < R; row += THREADS) {
+      float2 a = make_float2(-INFINITY, 0.f);
+      for (int x = la; x <= lb; ++x) a = joined(a, __ldcg(cta + (x * 2 + (x == la ? first_slot : 0)) * R + row));
+      dst[row] = a;
+    }
+  }
+}
+
+// blockIdx.x = 512 tokens of a sequence, blockIdx.y = KV head.
+template <int NB>
+__global__ void __launch_bounds__(256) paged_mass_kernel(const MassParams p) {
+  constexpr int R = 8 * NB, LPT = R / 4, PER = kMassGroup * LPT / 256;
+  __shared__ float2 s_stat[R];
+  grid_dep_wait();
+  const int n_units = p.hdr[2], total = p.hdr[3];
+  if ((int)blockIdx.x >= p.hdr[4]) return;
+  const int h = blockIdx.y, n_warps = p.ctas * kMassWarps;
+  const int4 gr = __ldg(p.groups + blockIdx.x), sq4 = __ldg(p.seqs + gr.x);
+  const Seq s{sq4.x, sq4.y, sq4.z, sq4.w};
+  const int rows = s.q * p.q.G, tid = threadIdx.x;
+  float acc[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+  for (int u = gr.z; u < gr.w; ++u) {
+    const int4 un = __ldg(p.units + u);
+    if (un.w * kTile <= gr.y || un.z * kTile >= gr.y + kMassGroup) continue;      // (the same for all threads)
+    const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
+    __syncthreads();
+    if (tid < R) {
+      const int k0 = warp_of(b0, total, n_warps) / kMassWarps, k1 = warp_of(b1 - 1, total, n_warps) / kMassWarps;
+      float2 a = make_float2(-INFINITY, 0.f);
+      if (k0 == k1) a = __ldcg(p.stats + ((int64_t)h * n_units + u) * R + tid);
+      else
+        for (int k = k0; k <= k1; ++k) {
+          const int slot = k == k0 && b0 > stretch_begin(k * kMassWarps, total, n_warps) ? 1 : 0;
+          a = joined(a, __ldcg(p.cta_parts + ((size_t)(h * p.ctas + k) * 2 + slot) * R + tid));
+        }
+      const int row = un.y + tid;
+      float inv = 0.f;
+      if (row < rows) {
+        bool none = a.x == -INFINITY;
+        if (p.sinks && !none) {
+          const float sk = __ldg(p.sinks + h * p.q.G + row % p.q.G) * 1.4426950408889634f;
+          none = sk - a.x > 126.f;
+          a.y += fast_exp2(sk - a.x);
+        }
+        inv = none ? 0.f : 1.f / a.y;
+      }
+      s_stat[tid] = make_float2(a.x == -INFINITY ? 0.f : a.x, inv);
+    }
+    __syncthreads();
+    const float4* sc = reinterpret_cast<const float4*>(p.scores + ((int64_t)h * total + b0 - un.z) * (kTile * R));      // of token 0
+    const int q4 = (tid % LPT) * 4;
+    const float2 s0 = s_stat[q4], s1 = s_stat[q4 + 1], s2 = s_stat[q4 + 2], s3 = s_stat[q4 + 3];
+    const int lo = un.z * kTile, hi = min(un.w * kTile, s.kv);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int t = gr.y + (tid + i * 256) / LPT;
+      if (t >= lo && t < hi) {
+        const float4 v = __ldcg(sc + (int64_t)t * LPT + tid % LPT);
+        acc[i] += fast_exp2(v.x - s0.x) * s0.y + fast_exp2(v.y - s1.x) * s1.y + fast_exp2(v.z - s2.x) * s2.y + fast_exp2(v.w - s3.x) * s3.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+#pragma unroll
+    for (int o = 1; o < LPT; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+    const int t = gr.y + (tid + i * 256) / LPT;
+    if (tid % LPT == 0 && t < s.kv) {
+      const int page = __ldg(p.tabs + s.tab + (t >> p.pool.page_bits));
+      const int64_t at = (((int64_t)page * p.pool.Hkv + h) << p.pool.page_bits) + (t & ((1 << p.pool.page_bits) - 1));
+      p.mass[at] = p.prior ? fmaf(p.decay, p.prior[at], acc[i]) : acc[i];
+    }
+  }
+}
+
+const void* scores_kernel_128(int ib, int rb, int nb, bool outl);
+const void* scores_kernel_64(int ib, int rb, int nb, bool outl);
+template <int N, int NB, bool OUTL>
+const void* pick_scores(int ib, int rb) {
+  if (ib == 10 && rb == 3) return (const void*)&paged_scores_kernel<N, 10, 3, NB, OUTL>;
+  if (ib == 12 && rb == 4) return (const void*)&paged_scores_kernel<N, 12, 4, NB, OUTL>;
+  if (ib == 13 && rb == 6) return (const void*)&paged_scores_kernel<N, 13, 6, NB, OUTL>;
+  return (const void*)&paged_scores_kernel<N, 0, 0, NB, OUTL>;
+}
+template <int N>
+const void* pick_scores_kernel(int ib, int rb, int nb, bool outl) {
+  if (nb == 1) return outl ? pick_scores<N, 1, true>(ib, rb) : pick_scores<N, 1, false>(ib, rb);
+  return outl ? pick_scores<N, 4, true>(ib, rb) : pick_scores<N, 4, false>(ib, rb);
+}
+
+}  // namespace paged
+}  // namespace hqmq

@@ -1,0 +1,212 @@
+// A 16-token tile of a paged cache on its way into shared memory and out of it as tensor-core operands.
+//
+// Every warp has a ring of three stages of its own, filled with 16-byte asynchronous copies by all of its lanes: while tile i is
+// computed, the rows, scales, flag words and block offsets of tile i + 2 are on their way, and the flagged chunks' values of tile
+// i + 1, whose place in the side buffer the tile's offsets say.  Tiles lie inside a page (pages hold 64 tokens or more), so a tile
+// is contiguous whatever the table says.
+#pragma once
+#include "paged.cuh"
+
+namespace hqmq {
+namespace paged {
+
+constexpr int kPay = 48;       // values of flagged chunks staged per tile and tensor; further ones are read from global memory
+constexpr int kTileStages = 3;
+
+// Rows of IB + RB bits per chunk; IB = 0: any width, at run time.
+template <int N, int IB, int RB>
+__host__ __device__ constexpr int row_bytes_of() { return (N * (IB + RB) + 31) / 32 * 4; }
+
+// Where the parts of a stage lie.
+struct TileLayout { int v, rsk, rsv, flk, flv, off, payk, payv, bytes; };
+__host__ __device__ constexpr TileLayout tile_layout(int row, bool hasv, bool outl) {
+  TileLayout l{};
+  int at = kTile * row;
+  l.v = at; at += hasv ? kTile * row : 0;
+  l.rsk = at; at += kTile * 2;
+  l.rsv = at; at += hasv ? kTile * 2 : 0;
+  l.flk = at; at += outl ? kTile * 4 : 0;
+  l.flv = at; at += outl && hasv ? kTile * 4 : 0;
+  l.off = at; at += outl ? 32 : 0;          // K: before, behind; V: before, behind; page
+  l.payk = at; at += outl ? kPay * 8 : 0;
+  l.payv = at; at += outl && hasv ? kPay * 8 : 0;
+  l.bytes = (at + 15) & ~15;
+  return l;
+}
+
+// What the copies need to know of a pool; page_bits = log2(tokens of a page).
+struct PoolView {
+  hqmq_packed K, V;
+  int Hkv, page_bits;
+};
+
+// The tiles of a warp's stretch, in order.
+struct TileIter {
+  int u, tile, hi, tab, left;
+  __device__ __forceinline__ void unit(const int4* units, const int4* seqs, int skip) {
+    const int4 un = __ldg(units + u);
+    tile = un.z + skip; hi = un.w;
+    tab = __ldg(&seqs[un.x].w);
+  }
+  __device__ __forceinline__ void next(const int4* units, const int4* seqs) {
+    if (--left <= 0) return;
+    if (++tile == hi) { ++u; unit(units, seqs, 0); }
+  }
+};
+
+template <bool HASV, bool OUTL>
+__device__ __forceinline__ void stage_tile(const PoolView& p, const TileLayout& l, int row_bytes, uint32_t sb, unsigned char* sp, int h, int page,
+                                           int tile, int lane) {
+  const int in_page = (tile * kTile) & ((1 << p.page_bits) - 1);
+  const int64_t ph = (int64_t)page * p.Hkv + h;
+  const int64_t row = (ph << p.page_bits) + in_page;
+  const int n16 = row_bytes;                                  // 16 rows of row_bytes, 16 bytes at a time
+  const unsigned char* k = p.K.codes + row * row_bytes;
+  for (int c = lane; c < n16; c += 32) cp_async16(sb + 16 * c, k + 16 * c);
+  if constexpr (HASV) {
+    const unsigned char* v = p.V.codes + row * row_bytes;
+    for (int c = lane; c < n16; c += 32) cp_async16(sb + l.v + 16 * c, v + 16 * c);
+  }
+  // the small parts: a lane each
+  const unsigned char* src = nullptr;
+  uint32_t dst = 0;
+  if (lane < 2) { src = reinterpret_cast<const unsigned char*>(p.K.rs) + row * 2 + lane * 16; dst = l.rsk + lane * 16; }
+  else if (HASV && lane < 4) { src = reinterpret_cast<const unsigned char*>(p.V.rs) + row * 2 + (lane - 2) * 16; dst = l.rsv + (lane - 2) * 16; }
+  else if (OUTL && lane >= 4 && lane < 8) { if (p.K.flags) { src = reinterpret_cast<const unsigned char*>(p.K.flags + row) + (lane - 4) * 16; dst = l.flk + (lane - 4) * 16; } }
+  else if (OUTL && HASV && lane >= 8 && lane < 12) { if (p.V.flags) { src = reinterpret_cast<const unsigned char*>(p.V.flags + row) + (lane - 8) * 16; dst = l.flv + (lane - 8) * 16; } }
+  if (src) cp_async16(sb + dst, src);
+  if constexpr (OUTL) {
+    const int64_t o = ph * ((1 << p.page_bits) / HQMQ_OUT_BLOCK + 1) + in_page / HQMQ_OUT_BLOCK;
+    if (lane >= 12 && lane < 14 && p.K.flags) cp_async4(sb + l.off + (lane - 12) * 4, p.K.out_off + o + (lane - 12));
+    if (HASV && lane >= 14 && lane < 16 && p.V.flags) cp_async4(sb + l.off + (lane - 12) * 4, p.V.out_off + o + (lane - 14));
+    if (lane == 16) *reinterpret_cast<int*>(sp + l.off + 16) = page;
+  }
+}
+
+// The values of a staged tile's flagged chunks (an entry the side buffer had no room for reads as 0).
+template <bool HASV>
+__device__ __forceinline__ void stage_values(const PoolView& p, const TileLayout& l, uint32_t sb, unsigned char* sp, int h, int lane) {
+  const uint32_t* off = reinterpret_cast<const uint32_t*>(sp + l.off);
+  const int64_t ph = (int64_t)(int)off[4] * p.Hkv + h;
+  auto side = [&](const hqmq_packed& x, uint32_t lo, uint32_t hi, int at) {
+    const uint32_t n = hi - lo < (uint32_t)kPay ? hi - lo : (uint32_t)kPay;
+    const unsigned char* v = reinterpret_cast<const unsigned char*>(x.out_vals) + ph * x.out_cap * 8;
+    for (uint32_t i = lane; i < n; i += 32) {
+      const uint32_t e = lo + i;
+      if (e < (uint32_t)x.out_cap) cp_async8(sb + at + 8 * i, v + (int64_t)e * 8);
+      else *reinterpret_cast<uint2*>(sp + at + 8 * i) = make_uint2(0u, 0u);
+    }
+  };
+  if (p.K.flags) side(p.K, off[0], off[1], l.payk);
+  if (HASV && p.V.flags) side(p.V, off[2], off[3], l.payv);
+}
+
+// The value of a flagged chunk: entry `rel` of the tile's, two words of two 16-bit values.
+__device__ __forceinline__ uint2 flagged_value(const hqmq_packed& x, const unsigned char* sp, int at, uint32_t lo, uint32_t rel, int64_t ph) {
+  if (rel < (uint32_t)kPay) return *reinterpret_cast<const uint2*>(sp + at + 8 * rel);
+  const uint32_t e = lo + rel;
+  if (e >= (uint32_t)x.out_cap) return make_uint2(0u, 0u);
+  return __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned char*>(x.out_vals) + (ph * x.out_cap + e) * 8));
+}
+__device__ __forceinline__ float4 values_of(uint2 v, int dtype) {
+  float2 a, b;
+  if (dtype == HQMQ_BF16) {
+    a = make_float2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u));
+    b = make_float2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+  } else {
+    a = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+    b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+  }
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// Sums of two 16-bit counts per lane over the lanes before it (lanes 0..15 of the tile's tokens).
+__device__ __forceinline__ uint32_t counts_before(uint32_t own, int lane) {
+  uint32_t x = own;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x - own;
+}
+
+// The codeword and radius of field `c` of a row of `cb`-bit fields (sign-folded index, the sign in the radius).
+__device__ __forceinline__ void cut_any(const uint32_t* row, int c, int ib, int cb, uint32_t& idx, __half2& rr) {
+  const uint32_t v = row_field(row, c, cb);
+  const __half2 r2 = radius_half2(v >> ib);
+  idx = (v & ((1u << ib) - 1u)) >> 1;
+  const uint32_t ru = *reinterpret_cast<const uint32_t*>(&r2) ^ ((0u - (v & 1u)) & 0x80008000u);
+  rr = *reinterpret_cast<const __half2*>(&ru);
+}
+
+// One head's table, sign-folded and replicated: entry i of the even codewords `reps` times in a row.
+template <int THREADS>
+__device__ __forceinline__ void load_table(unsigned char* tbl, const uint16_t* src16, int h, int rows, int rep_log2) {
+  const uint2* src = reinterpret_cast<const uint2*>(src16) + (int64_t)h * rows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows_f = rows >> 1;
+  for (int i0 = warp * 32; i0 < rows_f; i0 += THREADS) {
+    uint2 e = make_uint2(0u, 0u);
+    if (i0 + lane < rows_f) e = __ldg(src + 2 * (i0 + lane));
+    uint2* d = reinterpret_cast<uint2*>(tbl) + ((size_t)i0 << rep_log2);
+    for (int k = 0; k < 1 << rep_log2; ++k) {
+      const int s = k * 32 + lane, from = s >> rep_log2;
+      const uint2 v = make_uint2(__shfl_sync(0xffffffffu, e.x, from), __shfl_sync(0xffffffffu, e.y, from));
+      if (i0 + from < rows_f) d[s] = v;
+    }
+  }
+}
+
+// ---- the queries of a unit: rows as columns of the product ----------------------------------------------------------------------
+struct QueryView { const void* Q; int dtype, vec; int64_t st_t, st_h; int G; };
+
+// Row `row` (query * G + head) of a unit, this lane's dims [4 NKS j, 4 NKS (j + 1)), in fp16 after division by a power of two that
+// brings the row's largest value to [1, 2); returns that power.  A row that is not there is zeros.
+template <int NKS>
+__device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& q, int q_off, int h, int row, int rows, int j) {
+  float f[4 * NKS];
+  const int qi = row / q.G, g = row - qi * q.G;
+  const bool real = row < rows;
+  const int64_t o = (int64_t)(q_off + qi) * q.st_t + (int64_t)(h * q.G + g) * q.st_h + 4 * NKS * j;
+#pragma unroll
+  for (int i = 0; i < 4 * NKS; ++i) f[i] = 0.f;
+  if (real) {
+    if (q.vec) {
+#pragma unroll
+      for (int i = 0; i < 4 * NKS; i += 8) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q.Q) + o + i));
+        const float4 a = values_of(make_uint2(v.x, v.y), q.dtype), b = values_of(make_uint2(v.z, v.w), q.dtype);
+        f[i] = a.x; f[i + 1] = a.y; f[i + 2] = a.z; f[i + 3] = a.w;
+        f[i + 4] = b.x; f[i + 5] = b.y; f[i + 6] = b.z; f[i + 7] = b.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4 * NKS; ++i) f[i] = load_float(q.Q, o + i, q.dtype);
+    }
+  }
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4 * NKS; ++i) m = fmaxf(m, fabsf(f[i]));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  int e = (int)(__float_as_uint(m) >> 23) - 127;               // (subnormal: -127; infinite: 128)
+  e = min(126, max(-126, e));
+  const float div = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    qb[ks][0] = pack_half2(f[4 * ks] * div, f[4 * ks + 1] * div);
+    qb[ks][1] = pack_half2(f[4 * ks + 2] * div, f[4 * ks + 3] * div);
+  }
+  return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// softcap * tanh(x / softcap) in the exp2 domain, from x * 2 log2(e) / softcap: 1 - 2 / (2^y + 1)
+__device__ __forceinline__ float capped(float y, float cap_log2) { return cap_log2 - __fdividef(2.f * cap_log2, fast_exp2(y) + 1.f); }
+
+}  // namespace paged
+}  // namespace hqmq

@@ -456,6 +456,103 @@ int hqmq_exchange_wait(const hqmq_exchange* x, uint32_t epoch, uint32_t max_poll
  * launches that wait for EACH OTHER must not share one GPU (ranks are GPUs). */
 int hqmq_exchange_step(const hqmq_exchange* x, const float* local, uint32_t epoch, uint32_t max_polls, uint32_t* status,
                        int64_t rows, int d, int out_dtype, void* out, void* stream);
+/* ---- a paged compressed cache ---------------------------------------------------------------------------------
+ * A pool of pages is one hqmq_packed per tensor with B = pages and T_cap = tokens per page (a power of two, at least
+ * 64): page p, KV head h holds rows, scales, flags, payload, block offsets and counter of its T_cap tokens exactly as a
+ * (b, h) of the contiguous layout does.  Scales and payload are 16-bit; there are no fragment records.  Sequences are
+ * rows of a table of pages: token t of sequence s lives in page table[s][t / T_cap], row t % T_cap.
+ *
+ * A plan says how the calls over one batch split their work.  It is made on the host from the lengths (every new token is
+ * part of its sequence: q_len <= kv_len), copied to the device by the caller and used by any number of calls, one layer after
+ * the other.  `total_q` and what follows it is filled in by the library. */
+#define HQMQ_PAGED_MAX_CTAS 148
+typedef struct hqmq_paged_plan {
+  uint32_t struct_size;
+  int32_t n_seqs, n_pages, page_tokens;
+  int32_t H_q, H_kv, d;        /* H_q = 0: tables and lengths only (hqmq_paged_store, hqmq_paged_evict) */
+  int32_t window;              /* > 0: a query sees the last `window` positions up to its own */
+  int32_t tab_room;            /* > 0: the plan has room for this many table entries, and lengths may change in place: */
+  int32_t renew;               /* 1: same q_lens, other kv_lens and tables for a plan sized before with tab_room; no count, place or
+                                  launch changes (prompt chunks: HQMQ_ERR_UNSUPPORTED), so captured calls follow the plan's words */
+  int32_t total_q;             /* rows of Q: the sum of q_lens */
+  int32_t most_q, reserved;    /* the largest q_len */
+  /* words (4 bytes) of the plan, and in words where its parts begin */
+  int32_t words, seqs, tabs, n_tab;
+  /* decode: sequences of few rows */
+  int32_t dec_units, dec_rows, dec_ctas, dec_unit, dec_base, dec_warp, dec_cut, dec_tiles;
+  /* prompt chunks */
+  int32_t ch_units, ch_streams, ch_tiles, ch_heads, ch_whole, ch_ctas, ch_unit, ch_order, ch_start, ch_seqs, ch_img_tiles, ch_img;
+  /* attention weights */
+  int32_t ms_units, ms_rows, ms_ctas, ms_unit, ms_base, ms_warp, ms_tiles, ms_groups, ms_group, ms_tile_room, ms_group_room;
+} hqmq_paged_plan;
+/* Counts and places for these lengths (host arrays of n_seqs); then the plan itself: `tables` is a host array of n_seqs rows,
+ * `table_stride` apart, of which ceil(kv_len / page_tokens) entries are read; every entry is checked against n_pages. */
+int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_lens, const int32_t* q_lens);
+int hqmq_paged_plan_fill(const hqmq_paged_plan* plan, const int32_t* kv_lens, const int32_t* q_lens, const int32_t* tables,
+                         int64_t table_stride, int32_t* out);
+
+/* Attention of the last q_len tokens of every sequence over its pages: query i of sequence s stands at position
+ * kv_len - q_len + i and sees the keys up to its own position (the last `window` of them).  Scores are
+ * softmax_scale * <q, k>, with softcap > 0 capped to softcap * tanh(score / softcap); `sinks` (optional, fp32 [H_q]) is a
+ * logit per query head that takes part in the softmax and has no value.  d_head 64 or 128, H_q / H_kv <= 16, 24 * S <= 6144. */
+typedef struct hqmq_paged_attn_args {
+  uint32_t struct_size;
+  int32_t q_dtype, o_dtype, r_qmax;
+  const void* Q;               /* [total_q][H_q][d], unit stride on the last */
+  int64_t q_stride[2];
+  void* O;
+  int64_t o_stride[2];
+  float softmax_scale, softcap;
+  const float* sinks;
+  hqmq_packed K, V;            /* V is not read by hqmq_paged_mass */
+  const uint16_t* table_K;     /* fp16 [H_kv][24 S][4], see hqmq_codebook_tables */
+  const uint16_t* table_V;
+  hqmq_paged_plan plan;
+  const int32_t* plan_data;    /* the plan on the device, 16-byte aligned */
+  /* hqmq_paged_mass: out = decay * prior + weights; fp32 [pages][H_kv][page_tokens], prior may be NULL or out */
+  const float* prior;
+  float* mass;
+  float decay;
+  int32_t reserved;
+} hqmq_paged_attn_args;
+size_t hqmq_paged_attn_workspace_bytes(const hqmq_paged_attn_args* args);
+int hqmq_paged_attn(const hqmq_paged_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+/* The softmax weight of every key, summed over the queries that see it and over the query heads of its KV head.  Products are
+ * kept to 22 bits and sums in fp32; Q in fp16 or bf16.  Only tokens of the batch's sequences are written. */
+size_t hqmq_paged_mass_workspace_bytes(const hqmq_paged_attn_args* args);
+int hqmq_paged_mass(const hqmq_paged_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Encoded tokens go to their pages: the tokens of `src` (B = 1, T_cap >= total_q), in the order of the batch's queries, become
+ * the last q_len tokens of their sequences.  A page's first token resets its side buffer; the pages written must belong to one
+ * sequence each.  Entries beyond out_cap are dropped and counted, as in hqmq_encode. */
+typedef struct hqmq_paged_store_args {
+  uint32_t struct_size;
+  int32_t reserved;
+  hqmq_packed src_K, src_V, K, V;
+  hqmq_paged_plan plan;
+  const int32_t* plan_data;
+} hqmq_paged_store_args;
+int hqmq_paged_store(const hqmq_paged_store_args* args, void* stream);
+
+/* Cuts sequences down: of every sequence and KV head the last `last` tokens, the first `first` ones and, of the others, those
+ * with the largest mass (of equal ones, and of those that are no number and count as the smallest, the earlier) move, in order, from the pages of
+ * plan `src` to those of plan `dst`, whose kv_len says how many tokens are kept (at least first + last unless all are).  K, V
+ * and mass are the pool's; pages of dst must be in use by neither plan otherwise.  kept: int32 [n_seqs][H_kv][kept_stride],
+ * the kept positions, -1 behind the last.  new_mass may be mass. */
+typedef struct hqmq_paged_evict_args {
+  uint32_t struct_size;
+  int32_t first, last, kept_stride;
+  hqmq_packed K, V;
+  const float* mass;
+  float* new_mass;
+  int32_t* kept;
+  hqmq_paged_plan src, dst;
+  const int32_t* src_data;
+  const int32_t* dst_data;
+  int32_t longest, most_kept;  /* the largest kv_len of src and of dst */
+} hqmq_paged_evict_args;
+int hqmq_paged_evict(const hqmq_paged_evict_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

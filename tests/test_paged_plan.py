@@ -1,0 +1,267 @@
+"""Plans of calls over a paged cache (host code), their refusals, and those of the calls, without a GPU."""
+import ctypes as C
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import hqmq_b200 as hqmq
+from hqmq_b200 import _lib
+
+DEC_WARPS, DEC_WARPS_WIDE, MASS_WARPS, GROUP = 16, 8, 12, 512
+
+
+def make_pool(n_pages=64, H=2, d=128, S=24, rb=3, page=64, **kw):
+    return hqmq.PagedKV(n_pages, H, d, S, rb, "cpu", page_tokens=page, **kw)
+
+
+def tables_for(kv, page, n_pages, rng):
+    order = list(range(n_pages))
+    rng.shuffle(order)
+    out, at = [], 0
+    for n in kv:
+        k = -(-n // page)
+        out.append(order[at:at + k])
+        at += k
+    return out
+
+
+def keys_of(kv, q, G, window, row0, row1):
+    first, last = kv - q + row0 // G, kv - q + (row1 - 1) // G
+    return (max(0, first + 1 - window) if window else 0), last + 1
+
+
+def stretch(w, total, n):
+    n = min(n, total)
+    return w * total // n if w < n else total
+
+
+def check_flat(words, units, bases, warps, total, ctas, per_cta, want):
+    """Units in order with their tile ranges, prefix sums, and the unit that every warp's stretch begins in."""
+    got = [tuple(words[units + 4 * i:units + 4 * i + 4].tolist()) for i in range(len(want))]
+    assert got == want
+    base = np.cumsum([0] + [u[3] - u[2] for u in want])
+    assert words[bases:bases + len(want) + 1].tolist() == base.tolist() and base[-1] == total
+    n = ctas * per_cta
+    for w in range(n):
+        f = stretch(w, total, n)
+        if f < total:
+            u = words[warps + w]
+            assert base[u] <= f < base[u + 1]
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_plan_covers_every_tile_once(seed):
+    rng = random.Random(seed)
+    H, G, d = rng.choice([(1, 1, 64), (2, 4, 128), (4, 7, 128), (8, 8, 64), (3, 16, 64)])
+    page, window = rng.choice([64, 128, 256]), rng.choice([0, 1, 100, 128])
+    B = rng.randint(1, 9)
+    kv = [rng.choice([0, 1, rng.randint(1, 40), rng.randint(1, 900)]) for _ in range(B)]
+    q = [min(n, rng.choice([0, 1, 1, 2, 5, 130, 400])) for n in kv]
+    n_pages = sum(-(-n // page) for n in kv) + 2
+    pool = make_pool(n_pages, H, d, page=page)
+    tables = tables_for(kv, page, n_pages, rng)
+    b = hqmq.PagedBatch(pool, tables, kv, q, n_heads=H * G, window=window or None)
+    p, w = b.plan, b.data.numpy()
+    assert p.total_q == sum(q) and len(w) == p.words
+    # sequences and tables
+    at = 0
+    for s in range(B):
+        n, nq, off, tab = w[p.seqs + 4 * s:p.seqs + 4 * s + 4]
+        assert (n, nq, off) == (kv[s], q[s], at)
+        assert w[p.tabs + tab:p.tabs + tab + len(tables[s])].tolist() == tables[s]
+        at += q[s]
+    tiles = lambda lo, hi: (lo // 16, -(-hi // 16))
+    few = [s for s in range(B) if 0 < q[s] * G <= 16]
+    dec = [(s, 0, *tiles(*keys_of(kv[s], q[s], G, window, 0, q[s] * G))) for s in few]
+    assert p.dec_units == len(dec) and p.dec_rows == (16 if any(q[s] * G > 8 for s in few) else 8)
+    if dec:
+        per = DEC_WARPS_WIDE if p.dec_rows > 8 else DEC_WARPS
+        check_flat(w, p.dec_unit, p.dec_base, p.dec_warp, p.dec_tiles, p.dec_ctas, per, dec)
+        # units between CTAs: every cut names its first and last CTA
+        base = w[p.dec_base:p.dec_base + len(dec) + 1]
+        n = p.dec_ctas * per
+        edges = [stretch(c * per, p.dec_tiles, n) for c in range(p.dec_ctas + 1)]
+        cta = lambda f: max(c for c in range(p.dec_ctas) if edges[c] <= f and edges[c] < edges[c + 1])
+        cuts = [(u, cta(base[u]), cta(base[u + 1] - 1)) for u in range(len(dec))]
+        want = [(u, a, z, int(base[u] > edges[a])) for u, a, z in cuts if a != z]
+        assert [tuple(w[p.dec_cut + 4 * i:p.dec_cut + 4 * i + 4].tolist()) for i in range(w[5])] == want
+    # attention weights: row blocks of every sequence, groups of tokens
+    rows = p.ms_rows
+    ms = [(s, r, *tiles(*keys_of(kv[s], q[s], G, window, r, min(q[s] * G, r + rows)))) for s in range(B) for r in range(0, q[s] * G, rows)]
+    assert p.ms_units == len(ms)
+    if ms:
+        check_flat(w, p.ms_unit, p.ms_base, p.ms_warp, p.ms_tiles, p.ms_ctas, MASS_WARPS, ms)
+    groups = [w[p.ms_group + 4 * i:p.ms_group + 4 * i + 4].tolist() for i in range(p.ms_groups)]
+    assert [g[:2] for g in groups] == [[s, t] for s in range(B) for t in range(0, kv[s], GROUP)]
+    for s, t, u0, u1 in groups:
+        assert [u for u in range(len(ms)) if ms[u][0] == s] == list(range(u0, u1))
+    # prompt chunks: units of a sequence in order, images of the tiles that any of them sees, pieces of equal size
+    P, units = 128 // G, []
+    chunks = [s for s in range(B) if q[s] * G > 16]
+    per = p.ch_streams * P
+    img = 0
+    for i, s in enumerate(chunks):
+        mine = []
+        for m in range(-(-q[s] // per)):
+            lo, hi = keys_of(kv[s], q[s], 1, window, m * per, min(q[s], (m + 1) * per))
+            mine.append((s, m, lo // 128, max(1, -(-hi // 128) - lo // 128)))
+        first, last = min(u[2] for u in mine), max(u[2] + u[3] for u in mine)
+        assert w[p.ch_img + 4 * i:p.ch_img + 4 * i + 4].tolist() == [s, first, last - first, img]
+        off = sum(q[:s])
+        units += [[*u, kv[s], q[s], off, img - first] for u in mine]
+        img += last - first
+    assert [w[p.ch_unit + 8 * i:p.ch_unit + 8 * i + 8].tolist() for i in range(p.ch_units)] == units
+    assert p.ch_img_tiles == img and p.ch_tiles == sum(u[3] for u in units) and (not units or p.H_kv % p.ch_heads == 0)
+    if units and p.ch_whole:
+        order = w[p.ch_order:p.ch_order + len(units)].tolist()
+        assert sorted(order) == list(range(len(units))) and all(units[a][3] >= units[z][3] for a, z in zip(order, order[1:]))
+    elif units:
+        flat = [(h, m, o) for h in range(p.ch_heads) for m in range(len(units)) for o in range(units[m][3])]
+        L = -(-len(flat) // p.ch_ctas)
+        assert [tuple(w[p.ch_start + 4 * c:p.ch_start + 4 * c + 3].tolist()) for c in range(p.ch_ctas)] == [flat[c * L] for c in range(p.ch_ctas)]
+
+
+@pytest.mark.parametrize("kv,q,kw", [
+    ([10], [11], {}),                                # more new tokens than tokens
+    ([-1], [0], {}),
+    ([10, 10], [1], {}),
+    ([10], [1], dict(window=0)),
+    ([10], [1], dict(n_heads=3)),
+    ([65], [1], {}),                                 # one page named, two needed
+])
+def test_batches_that_are_refused(kv, q, kw):
+    pool = make_pool()
+    with pytest.raises(ValueError):
+        hqmq.PagedBatch(pool, [[0]] * len(kv), kv, q, **{"n_heads": 4, **kw})
+
+
+@pytest.mark.parametrize("page", [-1, 64, 1 << 20])
+def test_pages_outside_of_the_pool_are_refused(page):
+    pool = make_pool(64)
+    with pytest.raises(ValueError):
+        hqmq.PagedBatch(pool, [[0, page]], [100], [1], n_heads=4)
+    hqmq.PagedBatch(pool, [[0, page]], [64], [1], n_heads=4)        # (an entry behind the last page is not read)
+    plan = _lib.PagedPlan(struct_size=C.sizeof(_lib.PagedPlan), n_seqs=1, n_pages=64, page_tokens=64, H_q=4, H_kv=2, d=128)
+    kv, q, tab = (np.array(x, dtype=np.int32) for x in ([100], [1], [0, page]))
+    L = _lib.lib()
+    assert L.hqmq_paged_plan_size(C.byref(plan), kv.ctypes.data, q.ctypes.data) == 0
+    out = np.zeros(plan.words, dtype=np.int32)
+    assert L.hqmq_paged_plan_fill(C.byref(plan), kv.ctypes.data, q.ctypes.data, tab.ctypes.data, 2, out.ctypes.data) == -2
+
+
+def test_more_refusals_of_batches():
+    pool = make_pool()
+    with pytest.raises(TypeError):
+        hqmq.PagedBatch(pool, [[0]], [1.5], [1], n_heads=4)
+    with pytest.raises(ValueError):
+        hqmq.PagedBatch(pool, [[0]], [1 << 40], [1], n_heads=4)
+    with pytest.raises(ValueError):
+        hqmq.PagedBatch(pool, [], [], [])
+    with pytest.raises(_lib.HqmqError):
+        hqmq.PagedBatch(pool, [[0, 1]], [100], [1], n_heads=4, reserve_pages=1)
+    with pytest.raises(_lib.HqmqError):
+        hqmq.PagedBatch(pool, [[0]], [10], [1], n_heads=2 * 17)       # 17 query heads per KV head
+    with pytest.raises(_lib.HqmqError):
+        hqmq.PagedBatch(pool, [[0]], [10], [1], n_heads=4).renew([[0]], [11])
+    for bad in (dict(page_tokens=96), dict(page_tokens=2048), dict(dtype=torch.float32)):
+        with pytest.raises((ValueError, TypeError)):
+            hqmq.PagedKV(4, 2, 128, 24, 3, "cpu", **bad)
+    with pytest.raises(ValueError):
+        hqmq.PagedKV(4, 2, 96, 24, 3, "cpu")
+
+
+def test_tables_in_any_form():
+    pool = make_pool()
+    want = hqmq.PagedBatch(pool, [[5, 3], [7]], [100, 9], n_heads=4).data
+    for t in (np.array([[5, 3], [7, 99]]), torch.tensor([[5, 3, -1], [7, -1, -1]]), ((5, 3, 8), (7,)), [torch.tensor([5, 3]), torch.tensor([7, 0])]):
+        assert torch.equal(hqmq.PagedBatch(pool, t, torch.tensor([100, 9]), n_heads=4).data, want)
+
+
+def test_a_plan_with_room_keeps_its_places():
+    pool = make_pool(200, H=2)
+    rng = random.Random(3)
+    b = hqmq.PagedBatch(pool, tables_for([300, 40], 64, 200, rng), [300, 40], [1, 2], n_heads=8, window=None, reserve_pages=60)
+    before = {n: getattr(b.plan, n) for n, _ in _lib.PagedPlan._fields_}
+    p = _lib.PagedPlan.from_buffer_copy(b.plan)
+    p.renew = 1
+    same = set(before) - {"n_tab", "dec_tiles", "ms_tiles", "ms_groups", "renew"}
+    for kv in ([301, 41], [3000, 700], [1, 2]):
+        t = tables_for(kv, 64, 200, rng)
+        host, *_ = b._lay_out(p, t, kv, [1, 2])
+        assert all(getattr(p, n) == before[n] for n in same)
+        w = host.numpy()
+        assert w[1] == p.dec_tiles == sum(-(-n // 16) for n in kv) and w[p.tabs:p.tabs + len(t[0])].tolist() == t[0]
+    with pytest.raises(_lib.HqmqError):
+        b._lay_out(p, tables_for([3000, 900], 64, 200, rng), [3000, 900], [1, 2])       # 62 pages
+    with pytest.raises(_lib.HqmqError):
+        b._lay_out(p, [[0], [1]], [20, 20], [1, 1])
+    c = hqmq.PagedBatch(pool, [[1, 2]], [100], [50], n_heads=8, reserve_pages=10)       # a prompt chunk
+    p = _lib.PagedPlan.from_buffer_copy(c.plan)
+    p.renew = 1
+    with pytest.raises(_lib.HqmqError):
+        c._lay_out(p, [[1, 2]], [101], [50])
+
+
+def test_pages_shared_and_written():
+    pool = make_pool()
+    shared = hqmq.PagedBatch(pool, [[1, 2], [1, 3]], [100, 90], [1, 1])      # a common prefix; new tokens in pages of their own
+    assert shared.stores_alone() and not shared._unshared
+    assert not hqmq.PagedBatch(pool, [[1, 2], [1, 2]], [100, 90], [1, 1]).stores_alone()
+    assert not hqmq.PagedBatch(pool, [[1, 1]], [100], [1]).stores_alone()
+    assert hqmq.PagedBatch(pool, [[1, 2], [2]], [100, 0], [1, 0]).stores_alone()
+
+
+def test_calls_refuse_host_memory():
+    pool = make_pool()
+    b = hqmq.PagedBatch(pool, [[0]], [10], [1], n_heads=4)
+    t = torch.zeros(2, 24 * 24, 4, dtype=torch.float16)
+    for call in (lambda: hqmq.paged_attention(torch.zeros(1, 4, 128), pool, b, t, t),
+                 lambda: hqmq.paged_attention_mass(torch.zeros(1, 4, 128), pool, b, t),
+                 lambda: hqmq.paged_evict(pool, b, b, pool.new_mass()),
+                 lambda: hqmq.paged_store(pool, pool.K, pool.V, b)):
+        with pytest.raises(_lib.HqmqError):
+            call()
+
+
+def _args(pool, batch, G=2):
+    a = _lib.PagedAttnArgs(struct_size=C.sizeof(_lib.PagedAttnArgs), q_dtype=_lib.BF16, o_dtype=_lib.BF16, r_qmax=7, softmax_scale=0.1)
+    a.Q = a.O = a.plan_data = a.table_K = a.table_V = a.mass = 1 << 20
+    a.K, a.V, a.plan = pool.K.c_struct(), pool.V.c_struct(), batch.plan
+    return a
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(struct_size=8), -1), (dict(Q=None), -1), (dict(O=None), -1), (dict(plan_data=None), -1), (dict(table_K=None), -1),
+    (dict(q_dtype=_lib.I32), -3), (dict(o_dtype=_lib.I8), -3), (dict(plan_data=(1 << 20) + 4), -4), (dict(r_qmax=15), -2),
+    (dict(softcap=-1.0), -1), (dict(softcap=float("nan")), -1), (dict(softmax_scale=float("nan")), -1), ({}, -5),
+])
+def test_abi_refuses_arguments(built_lib, change, code):
+    pool = make_pool(outliers_K=True)
+    a = _args(pool, hqmq.PagedBatch(pool, [[0, 1], [2]], [100, 50], [1, 1], n_heads=4))
+    for k, v in change.items():
+        setattr(a, k, v)
+    L = _lib.lib()
+    assert L.hqmq_paged_attn(C.byref(a), None, 0, None) == code
+    assert (L.hqmq_paged_attn_workspace_bytes(C.byref(a)) == 0) == bool(change)
+
+
+def test_abi_refuses_pools_of_another_kind(built_lib):
+    pool = make_pool(outliers_K=True)
+    b = hqmq.PagedBatch(pool, [[0, 1], [2]], [100, 50], [1, 1], n_heads=4)
+    L = _lib.lib()
+    for field, value, code in (("B", 63, -2), ("H", 4, -2), ("T_cap", 128, -2), ("scale_dtype", _lib.F32, -8), ("out_dtype", _lib.F32, -8)):
+        a = _args(pool, b)
+        setattr(a.K, field, value)
+        assert L.hqmq_paged_attn(C.byref(a), None, 0, None) == code, field
+    a = _args(pool, b)
+    a.q_dtype = _lib.F32
+    assert L.hqmq_paged_mass(C.byref(a), None, 0, None) == -8
+    store = hqmq.PagedBatch(pool, [[0, 1]], [100], [1])                # without query heads
+    assert L.hqmq_paged_attn(C.byref(_args(pool, store)), None, 0, None) == -1
+    for change in (dict(page_tokens=32), dict(n_seqs=0), dict(d=96), dict(H_q=3)):
+        a = _args(pool, b)
+        for k, v in change.items():
+            setattr(a.plan, k, v)
+        assert L.hqmq_paged_attn(C.byref(a), None, 0, None) in (-2, -8)
