@@ -12,6 +12,7 @@ namespace paged {
 namespace {
 
 constexpr size_t kSmemMax = 232448;          // 227 KB
+constexpr size_t kPastPay = 16;              // (a lane without a flagged chunk reads the place behind a stage's last value)
 constexpr float kLog2e = 1.4426950408889634f;
 
 int log2_of(int x) { int b = 0; while ((1 << b) < x) ++b; return b; }
@@ -68,8 +69,12 @@ size_t part_bytes(const hqmq_paged_plan& p) {
   const int nb = p.dec_rows > 8 ? 2 : 1;
   return (size_t)nb * (p.d / 16 * 128 + 16) * 4;
 }
-size_t decode_workspace(const hqmq_paged_plan& p) {
-  return p.dec_units ? (size_t)p.dec_ctas * p.H_kv * (dec_warps(p.dec_rows) + 1) * 2 * part_bytes(p) : 0;
+size_t decode_parts(const hqmq_paged_plan& p) { return up256((size_t)p.dec_ctas * p.H_kv * (dec_warps(p.dec_rows) + 1) * 2 * part_bytes(p)); }
+size_t decode_workspace(const hqmq_paged_attn_args* a) {
+  const hqmq_paged_plan& p = a->plan;
+  if (!p.dec_units) return 0;
+  const size_t wide = a->K.flags || a->V.flags ? (size_t)p.dec_ctas * p.H_kv * dec_warps(p.dec_rows) * 32 * (p.d / 4) * 8 : 0;
+  return decode_parts(p) + wide;
 }
 
 int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
@@ -92,9 +97,10 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   p.base = a->plan_data + pl.dec_base; p.wunit = a->plan_data + pl.dec_warp; p.tabs = a->plan_data + pl.tabs;
   p.ctas = pl.dec_ctas;
   p.parts = reinterpret_cast<float*>(ws);
+  p.wide = reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(ws) + decode_parts(pl));
   const bool outl = a->K.flags || a->V.flags;
   const int nb = pl.dec_rows > 8 ? 2 : 1, warps = dec_warps(pl.dec_rows);
-  const size_t rings = (size_t)warps * kTileStages * tile_layout(p.row_bytes, true, outl).bytes, table = (size_t)(p.table_rows >> 1) * 8;
+  const size_t rings = (size_t)warps * kTileStages * tile_layout(p.row_bytes, true, outl).bytes + kPastPay, table = (size_t)(p.table_rows >> 1) * 8;
   // (a field that no encoder writes may index up to 2^ib / 2 entries: what that reaches lies in the block's shared memory, too)
   const size_t any = (size_t)4 << p.ib;
   auto need = [&](int rk, int rv) { return std::max(rings + (table << rk) + (table << rv), std::max(any << rk, (table << rk) + (any << rv))); };
@@ -111,18 +117,20 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   HQMQ_CHECK_CUDA(raise_smem_limit(k.decode, smem));
   void* args[] = {&p};
   HQMQ_CHECK_CUDA(launch(k.decode, dim3(p.ctas * pl.H_kv), warps * 32, args, smem, st, false));
-  if (p.ctas > 1) HQMQ_CHECK_CUDA(launch(k.merge, dim3(p.ctas - 1, pl.H_kv), 256, args, 0, st, true));
+  if (p.ctas > 1) HQMQ_CHECK_CUDA(launch(k.merge, dim3(p.ctas - 1, pl.H_kv, nb * pl.d / 16 * 32 / 64), 64, args, 0, st, true));
   return HQMQ_OK;
 }
 
-struct MassPlaces { size_t parts, cta, stats, scores, bytes; };
-MassPlaces mass_places(const hqmq_paged_plan& p) {
+struct MassPlaces { size_t parts, cta, stats, wide, scores, bytes; };
+MassPlaces mass_places(const hqmq_paged_attn_args* a) {
+  const hqmq_paged_plan& p = a->plan;
   MassPlaces m;
   const size_t r = p.ms_rows, ctas = (size_t)p.ms_ctas * p.H_kv;
   m.parts = 0;
   m.cta = up256(ctas * kMassWarps * 2 * r * 8);
   m.stats = m.cta + up256(ctas * 2 * r * 8);
-  m.scores = m.stats + up256((size_t)p.H_kv * p.ms_units * r * 8);
+  m.wide = m.stats + up256((size_t)p.H_kv * p.ms_units * r * 8);
+  m.scores = m.wide + (a->K.flags ? up256(ctas * kMassWarps * 16 * (p.d / 4) * 16) : 0);
   m.bytes = m.scores + (size_t)p.H_kv * p.ms_tile_room * kTile * r * 4 + 256;
   return m;
 }
@@ -136,7 +144,7 @@ using namespace hqmq::paged;
 
 extern "C" size_t hqmq_paged_attn_workspace_bytes(const hqmq_paged_attn_args* args) {
   if (check_args(args, false)) return 0;
-  return up256(decode_workspace(args->plan)) + chunk_workspace(args) + 256;
+  return up256(decode_workspace(args)) + chunk_workspace(args) + 256;
 }
 
 extern "C" int hqmq_paged_attn(const hqmq_paged_attn_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -148,20 +156,20 @@ extern "C" int hqmq_paged_attn(const hqmq_paged_attn_args* args, void* workspace
     const int e = decode_launch(args, workspace, (cudaStream_t)stream);
     if (e) return e;
   }
-  if (args->plan.ch_units) return chunk_launch(args, reinterpret_cast<unsigned char*>(workspace) + up256(decode_workspace(args->plan)), (cudaStream_t)stream);
+  if (args->plan.ch_units) return chunk_launch(args, reinterpret_cast<unsigned char*>(workspace) + up256(decode_workspace(args)), (cudaStream_t)stream);
   return HQMQ_OK;
 }
 
 extern "C" size_t hqmq_paged_mass_workspace_bytes(const hqmq_paged_attn_args* args) {
   if (check_args(args, true)) return 0;
-  return mass_places(args->plan).bytes;
+  return mass_places(args).bytes;
 }
 
 extern "C" int hqmq_paged_mass(const hqmq_paged_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_args(a, true);
   if (rc) return rc;
   const hqmq_paged_plan& pl = a->plan;
-  const MassPlaces m = mass_places(pl);
+  const MassPlaces m = mass_places(a);
   if (!workspace || workspace_bytes < m.bytes) return HQMQ_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return HQMQ_ERR_ALIGN;
   cudaStream_t st = (cudaStream_t)stream;
@@ -183,13 +191,14 @@ extern "C" int hqmq_paged_mass(const hqmq_paged_attn_args* a, void* workspace, s
   p.ctas = pl.ms_ctas;
   p.parts = reinterpret_cast<float2*>(ws + m.parts); p.cta_parts = reinterpret_cast<float2*>(ws + m.cta);
   p.stats = reinterpret_cast<float2*>(ws + m.stats); p.scores = reinterpret_cast<float*>(ws + m.scores);
+  p.wide = reinterpret_cast<uint4*>(ws + m.wide);
   p.prior = a->prior; p.mass = a->mass; p.decay = a->decay;
   if (pl.ms_group_room == 0) return HQMQ_OK;
   const bool outl = a->K.flags != nullptr;
   const int nb = pl.ms_rows / 8;
   void* args[] = {&p};
   if (pl.ms_units) {
-    const size_t rings = (size_t)kMassWarps * kTileStages * tile_layout(p.row_bytes, false, outl).bytes, table = (size_t)(p.table_rows >> 1) * 8;
+    const size_t rings = (size_t)kMassWarps * kTileStages * tile_layout(p.row_bytes, false, outl).bytes + kPastPay, table = (size_t)(p.table_rows >> 1) * 8;
     auto need = [&](int rk) { return std::max(rings + (table << rk), ((size_t)4 << p.ib) << rk); };
     if (need(0) > kSmemMax) return HQMQ_ERR_UNSUPPORTED;
     while (p.repk < 4 && need(p.repk + 1) <= kSmemMax) ++p.repk;

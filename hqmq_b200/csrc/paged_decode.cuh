@@ -3,8 +3,10 @@
 // The tile's arithmetic is that of the staged decode kernels (attn_kernel.cuh): S^T = K Q^T with the 16 tokens as rows and the query
 // rows as columns, O^T += V^T P^T, operands gathered from shared-memory tables straight into fragments.  What differs: a warp walks
 // its own stretch of tiles from unit to unit (paged.cuh); flagged chunks, which decode to zero, are put into the fragments before
-// their product (a lane owns 2 tokens x N / 4 chunks of K and 4 x N / 8 of V, and tests its own flag bits; which of the
-// steps have one at all is one word per tile), as fp16(x * qmax / rs), what the table would have given; V's scales enter P relative to the largest
+// their product: a lane per entry turns the tile's values into fp16(x * qmax / rs), what the table would have given, once; a lane owns
+// 2 tokens x N / 4 chunks of K and 4 x N / 8 of V, its entries are neighbours in the side buffer's order, so that it walks a pointer along
+// them, in the steps (one word per tile says which) that have any.  (With the value looked up, counted for and converted by every lane in
+// every step: 1370 instructions a tile against 745 without outliers, and the loop outgrew the instruction cache.)  V's scales enter P relative to the largest
 // one seen, a power of two that the accumulators are rescaled by like by the maximum, so that values of any size keep their bits.
 #pragma once
 #include "attn_tma.cuh"
@@ -26,6 +28,7 @@ struct DecodeParams {
   const int4* seqs; const int4* units; const int* base; const int* wunit; const int4* cuts; const int* tabs; const int* hdr;
   int ctas;
   float* parts;                  // [CTA][warps][2][part], then [CTA][2][part]
+  uint2* wide;                   // [CTA][warps][K, V][16 N]: values of a tile with more flagged chunks than a stage holds
 };
 
 template <int N, int NB> __host__ __device__ constexpr int part_floats() { return NB * (N / 4 * 128 + 16); }
@@ -59,28 +62,28 @@ __device__ __forceinline__ void merge_parts(int idx, int n, const PartOf& part_o
   const int nb = idx / PER, j = idx & 3;
   m = make_float2(-INFINITY, -INFINITY);
   const int at = NB * PER * 4 + nb * 16 + 2 * j;
-  for (int k = 0; k < n; ++k) {
-    const float2 mk = __ldcg(reinterpret_cast<const float2*>(part_of(k) + at));
-    m.x = fmaxf(m.x, mk.x); m.y = fmaxf(m.y, mk.y);
-  }
-  const float ux = m.x == -INFINITY ? 0.f : m.x, uy = m.y == -INFINITY ? 0.f : m.y;
   v = make_float4(0.f, 0.f, 0.f, 0.f);
   l = make_float2(0.f, 0.f);
-#pragma unroll 4
+  // (one pass with a running maximum: no load waits for another)
+#pragma unroll 8
   for (int k = 0; k < n; ++k) {
     const float* pk = part_of(k);
     const float2 mk = __ldcg(reinterpret_cast<const float2*>(pk + at)), lk = __ldcg(reinterpret_cast<const float2*>(pk + at + 8));
     const float4 x = __ldcg(reinterpret_cast<const float4*>(pk) + idx);
-    const float wx = fast_exp2(mk.x - ux), wy = fast_exp2(mk.y - uy);
-    l.x = fmaf(lk.x, wx, l.x); l.y = fmaf(lk.y, wy, l.y);
-    v.x = fmaf(x.x, wx, v.x); v.y = fmaf(x.y, wy, v.y); v.z = fmaf(x.z, wx, v.z); v.w = fmaf(x.w, wy, v.w);
+    const float nx = fmaxf(m.x, mk.x), ny = fmaxf(m.y, mk.y), ux = nx == -INFINITY ? 0.f : nx, uy = ny == -INFINITY ? 0.f : ny;
+    const float ax = fast_exp2(m.x - ux), ay = fast_exp2(m.y - uy), wx = fast_exp2(mk.x - ux), wy = fast_exp2(mk.y - uy);
+    l.x = fmaf(lk.x, wx, l.x * ax); l.y = fmaf(lk.y, wy, l.y * ay);
+    v.x = fmaf(x.x, wx, v.x * ax); v.y = fmaf(x.y, wy, v.y * ay); v.z = fmaf(x.z, wx, v.z * ax); v.w = fmaf(x.w, wy, v.w * ay);
+    m.x = nx; m.y = ny;
   }
 }
+__device__ __forceinline__ Seq seq_of(const DecodeParams& p, int u) {
+  const int4 sq = __ldg(p.seqs + __ldg(&p.units[u].x));
+  return Seq{sq.x, sq.y, sq.z, sq.w};
+}
 template <int N, int NB>
-__device__ __forceinline__ void emit_merged(const DecodeParams& p, int u, int h, int idx, float4 v, float2 m, float2 l) {
+__device__ __forceinline__ void emit_merged(const DecodeParams& p, const Seq& s, int h, int idx, float4 v, float2 m, float2 l) {
   constexpr int PER = N / 4 * 32;
-  const int4 un = __ldg(p.units + u), sq = __ldg(p.seqs + un.x);
-  const Seq s{sq.x, sq.y, sq.z, sq.w};
   const int rows = s.q * p.q.G, nb = idx / PER, i = (idx - nb * PER) >> 5, lane = idx & 31, row = nb * 8 + 2 * (lane & 3);
   const float ia = inverse_sum(p, h, row, rows, m.x, l.x), ib = inverse_sum(p, h, row + 1, rows, m.y, l.y);
   emit_pair<N>(p, s, h, row, rows, lane >> 2, i, v.x * ia, v.z * ia);
@@ -117,14 +120,16 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
     it.u = __ldg(p.wunit + w);
     it.unit(p.units, p.seqs, f0 - __ldg(p.base + it.u));
   }
-  auto stage = [&](int i) {          // tile i of the stretch, which `it` is at
+  Stager<true, OUTL> sg;
+  sg.init(p.pool, L, lane);
+  auto stage = [&](uint32_t at) {    // the tile that `it` is at, to the stage at `at`
     const int page = __ldg(p.tabs + it.tab + ((it.tile * kTile) >> p.pool.page_bits));
-    const int st = i % kTileStages;
-    stage_tile<true, OUTL>(p.pool, L, ROW, ring32 + st * L.bytes, ring + st * L.bytes, h, page, it.tile, lane);
+    sg.template tile<IB ? row_bytes_of<N, IB, RB>() : 0>(p.pool, L, ROW, ring32 + at, ring + at, h, page, it.tile, lane);
     it.next(p.units, p.seqs);
   };
-  if (n > 0) stage(0);
-  if (n > 1) stage(1);
+  uint32_t at0 = 0u, at1 = L.bytes, at2 = 2 * L.bytes;       // stages of the tile at hand, of the next two
+  if (n > 0) stage(at0);
+  if (n > 1) stage(at1);
   cp_commit();
   load_table<THREADS>(tblK, p.tblK, h, p.table_rows, p.repk);
   load_table<THREADS>(tblV, p.tblV, h, p.table_rows, p.repv);
@@ -132,7 +137,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   if constexpr (OUTL) {
     cp_wait_all();
     __syncwarp();
-    if (n > 0) stage_values<true>(p.pool, L, ring32, ring, h, lane);
+    if (n > 0) stage_values<true>(p.pool, L, ring32, ring, lane);
     cp_commit();
   }
 
@@ -143,6 +148,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   FL ld;
   ld.row_bytes = ROW; ld.row_words = ROW / 4; ld.j = j; ld.r = r; ld.sdt = p.sdt;
   const float kfac = p.kfac;
+  auto my_wide = [&] { return p.wide + ((size_t)blockIdx.x * NW + (threadIdx.x >> 5)) * (32 * N); };     // (hardly ever asked for: not held)
   float* my_parts = p.parts + ((size_t)blockIdx.x * NW + warp) * 2 * PART;
 
   int u = n > 0 ? __ldg(p.wunit + w) : 0, i = 0;
@@ -154,13 +160,9 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
     const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
     const int rows = s.q * p.q.G;
     uint32_t qb[NB][NKS][2];
-    float qmul[NB][2];
+    float qmul[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const float mul = load_query<NKS>(qb[nb], p.q, s.q_off, h, nb * 8 + r, rows, j);
-      qmul[nb][0] = __shfl_sync(0xffffffffu, mul, 8 * j) * kfac;
-      qmul[nb][1] = __shfl_sync(0xffffffffu, mul, 8 * j + 4) * kfac;
-    }
+    for (int nb = 0; nb < NB; ++nb) qmul[nb] = load_query<NKS, true>(qb[nb], p.q, s.q_off, h, nb * 8 + r, rows, j) * kfac;
     const int p_first = s.kv - s.q, edge_lo = p.window > 0 ? s.kv - p.window : 0;    // (the last query sees nothing before edge_lo)
     float m_run[NB][2], l_run[NB][2], o[NB][NOT][4];
 #pragma unroll
@@ -177,11 +179,12 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       cp_wait_all();
       __syncwarp();
       if constexpr (OUTL) {
-        if (i + 1 < n) { const int st = (i + 1) % kTileStages; stage_values<true>(p.pool, L, ring32 + st * L.bytes, ring + st * L.bytes, h, lane); }
+        if (i + 1 < n) stage_values<true>(p.pool, L, ring32 + at1, ring + at1, lane);
       }
-      if (i + 2 < n) stage(i + 2);
+      if (i + 2 < n) stage(at2);
       cp_commit();
-      const unsigned char* sp = ring + (i % kTileStages) * L.bytes;
+      unsigned char* sp = ring + at0;
+      { const uint32_t x = at0; at0 = at1; at1 = at2; at2 = x; }
       const int t0 = tile * kTile;
       const bool edge = t0 + kTile > p_first + 1 || t0 < edge_lo;
 
@@ -201,21 +204,45 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         if constexpr (IB != 0) ld.template load_span<FL::VW, FL::LV>(vw[x], sp + L.v + t * ROW, r, !edge || t0 + t < s.kv);
       }
       uint32_t kstep = 0u, vstep = 0u;       // bit x: some lane has a flagged chunk in step x
-      uint32_t fk[2] = {0u, 0u}, fk_pre[2] = {0u, 0u}, before = 0u;
+      uint32_t fk[2] = {0u, 0u}, pk[2] = {0u, 0u};        // flags of this lane's chunks from bit 0 on, place of the first one's value
+      uint32_t fl = 0u, before = 0u, at_v = 0u;
+      bool wide = false;
       if constexpr (OUTL) {
-        uint32_t fk_t = 0u, fv_t = 0u;
-        if (lane < kTile && t0 + lane < s.kv) {
-          if (p.pool.K.flags) fk_t = reinterpret_cast<const uint32_t*>(sp + L.flk)[lane];
-          if (p.pool.V.flags) fv_t = reinterpret_cast<const uint32_t*>(sp + L.flv)[lane];
-        }
-        kstep = __reduce_or_sync(0xffffffffu, fk_t);
-        vstep = __reduce_or_sync(0xffffffffu, fv_t);
+        // lanes 0..15: K's tokens, 16..31: V's
+        if (t0 + (lane & 15) < s.kv && (lane < 16 ? p.pool.K.flags : p.pool.V.flags)) fl = reinterpret_cast<const uint32_t*>(sp + L.flk)[lane];
+        kstep = __reduce_or_sync(0xffffffffu, lane < 16 ? fl : 0u);
+        vstep = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : fl);
         if (kstep | vstep) {
-          before = counts_before(__popc(fk_t) | (__popc(fv_t) << 16), lane);
+          const uint32_t own = __popc(fl);
+          const Entries en = entries_of<true>(p.pool, L, sp);
+          before = counts_before(own, lane);
+          wide = __any_sync(0xffffffffu, before + own > (lane < 16 ? en.nk : en.nv));
+          at_v = wide ? 16u * N * 8u : en.nk * 8u;
+          // every lane its token's values, in place
+          const float rs = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[lane], p.sdt);
+          const float inv = rs != 0.f ? __fdividef(p.qmaxf, rs) : 0.f;
+          const int dt = lane < 16 ? p.pool.K.out_dtype : p.pool.V.out_dtype;
+          auto operand = [&](uint2 v) {
+            const float4 x = values_of(v, dt);
+            return make_uint2(pack_half2(x.x * inv, x.y * inv), pack_half2(x.z * inv, x.w * inv));
+          };
+          if (!wide) {
+            uint2* e = reinterpret_cast<uint2*>(sp + L.pay + (lane < 16 ? 0u : at_v)) + before;
+            for (uint32_t x = 0; x < own; ++x, ++e) *e = operand(*e);
+          } else {
+            const int64_t ph = *reinterpret_cast<const int*>(sp + L.off + 16);
+            const hqmq_packed& pk_ = lane < 16 ? p.pool.K : p.pool.V;
+            uint2* e = my_wide() + (lane < 16 ? 0 : 16 * N) + before;
+            uint32_t from = (lane < 16 ? en.k0 : en.v0) + before;
+            for (uint32_t x = 0; x < own; ++x, ++e, ++from)
+              *e = operand(from < (uint32_t)pk_.out_cap ? __ldg(reinterpret_cast<const uint2*>(pk_.out_vals) + ph * pk_.out_cap + from) : make_uint2(0u, 0u));
+          }
+          __syncwarp();
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) {
-            fk[nt] = __shfl_sync(0xffffffffu, fk_t, nt * 8 + r);
-            fk_pre[nt] = __shfl_sync(0xffffffffu, before, nt * 8 + r) & 0xffffu;
+            const uint32_t f = __shfl_sync(0xffffffffu, fl, nt * 8 + r);
+            fk[nt] = f >> (j * NKS);
+            pk[nt] = 8u * (__shfl_sync(0xffffffffu, before, nt * 8 + r) + __popc(f & ((1u << (j * NKS)) - 1u)));
           }
         }
         // chunks j * NKS + ks / r * NVG + g: which ks, which g
@@ -224,7 +251,16 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         if constexpr (NVG == 4) { vstep |= vstep >> 16; vstep |= vstep >> 8; vstep |= vstep >> 4; vstep &= 0xfu; }
         else { vstep |= vstep >> 8; vstep |= vstep >> 4; vstep |= vstep >> 2; vstep &= 3u; }
       }
-      const int64_t ph = OUTL ? (int64_t)*reinterpret_cast<const int*>(sp + L.off + 16) * p.pool.Hkv + h : 0;
+      auto values_at = [&](uint2* v, const uint32_t* at, int n_) {     // operands of flagged chunks
+        if (!wide) {
+#pragma unroll
+          for (int x = 0; x < n_; ++x) v[x] = *reinterpret_cast<const uint2*>(sp + L.pay + at[x]);
+        } else {
+          const unsigned char* far = reinterpret_cast<const unsigned char*>(my_wide());
+#pragma unroll
+          for (int x = 0; x < n_; ++x) v[x] = __ldcg(reinterpret_cast<const uint2*>(far + at[x]));
+        }
+      };
 
       // ---- S^T = K Q^T ---------------------------------------------------------------------------------------------------------
       float sc[NB][4], s2[NB][4];
@@ -232,11 +268,6 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int x = 0; x < 4; ++x) sc[nb][x] = s2[nb][x] = 0.f;
-      float kinv[2];
-      if constexpr (OUTL) {
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) kinv[nt] = ksc[nt] != 0.f ? __fdividef(p.qmaxf, ksc[nt]) : 0.f;
-      }
       static_for<0, NKS>([&](auto ks_) {
         constexpr int ks = decltype(ks_)::value;
         uint32_t a[4];
@@ -251,15 +282,14 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         });
         if constexpr (OUTL) {
           if (kstep & (1u << ks)) {
+            // (no branch per lane: the place is a place of this tile, or the one behind its last, whoever has a value there or not)
+            uint2 v[2];
+            values_at(v, pk, 2);
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
-              const int c = j * NKS + ks;
-              if ((fk[nt] >> c) & 1u) {
-                const uint32_t rel = fk_pre[nt] + __popc(fk[nt] & ((1u << c) - 1u));
-                const float4 x = values_of(flagged_value(p.pool.K, sp, L.payk, reinterpret_cast<const uint32_t*>(sp + L.off)[0], rel, ph), p.pool.K.out_dtype);
-                a[nt] = pack_half2(x.x * kinv[nt], x.y * kinv[nt]);
-                a[2 + nt] = pack_half2(x.z * kinv[nt], x.w * kinv[nt]);
-              }
+              const bool f = (fk[nt] & (1u << ks)) != 0u;
+              a[nt] = f ? v[nt].x : a[nt]; a[2 + nt] = f ? v[nt].y : a[2 + nt];
+              pk[nt] += f ? 8u : 0u;
             }
           }
         }
@@ -271,7 +301,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sc[nb][x] = (sc[nb][x] + s2[nb][x]) * (ksc[x >> 1] * qmul[nb][x & 1]);
+        for (int x = 0; x < 4; ++x) sc[nb][x] = (sc[nb][x] + s2[nb][x]) * (ksc[x >> 1] * qmul[nb]);
       if (p.cap_log2 > 0.f) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -330,38 +360,31 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
           }
       }
 
-      // ---- P: fp16(p * scale of V); the weights summed are those rounded products divided by the scale, so the rounding cancels ------
+      // ---- P: fp16(p * scale of V) -----------------------------------------------------------------------------------------------------
       uint32_t pb[NB][2];
       const float vn[2] = {vsc[0] * v_inv, vsc[1] * v_inv};
-      const float iv[2] = {vn[0] > 0.f ? rcp_approx(vn[0]) : 0.f, vn[1] > 0.f ? rcp_approx(vn[1]) : 0.f};
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         float pr[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) pr[x] = fast_exp2(sc[nb][x] - (m_run[nb][x & 1] == -INFINITY ? 0.f : m_run[nb][x & 1]));
-        const __half2 h0 = __floats2half2_rn(pr[0] * vn[0], pr[1] * vn[0]), h1 = __floats2half2_rn(pr[2] * vn[1], pr[3] * vn[1]);
-        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
-        // (a token whose scale is far below the largest one has products that fp16 does not hold: its weight is taken as it is)
-        const bool ok0 = vn[0] > 0.0009765625f, ok1 = vn[1] > 0.0009765625f;
-        l_run[nb][0] += (ok0 ? g0.x * iv[0] : pr[0]) + (ok1 ? g1.x * iv[1] : pr[2]);
-        l_run[nb][1] += (ok0 ? g0.y * iv[0] : pr[1]) + (ok1 ? g1.y * iv[1] : pr[3]);
-        pb[nb][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h0));
-        pb[nb][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h1));
+        pb[nb][0] = movmatrix_trans(pack_half2(pr[0] * vn[0], pr[1] * vn[0]));
+        pb[nb][1] = movmatrix_trans(pack_half2(pr[2] * vn[1], pr[3] * vn[1]));
+        l_run[nb][0] += pr[0] + pr[2];
+        l_run[nb][1] += pr[1] + pr[3];
         if (vswz) { pb[nb][0] = __byte_perm(pb[nb][0], 0u, 0x1032); pb[nb][1] = __byte_perm(pb[nb][1], 0u, 0x1032); }
       }
 
       // ---- O^T += V^T P^T ---------------------------------------------------------------------------------------------------------
-      uint32_t fv[4] = {0u, 0u, 0u, 0u}, fv_pre[4] = {0u, 0u, 0u, 0u};
-      float vi[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t fv[4] = {0u, 0u, 0u, 0u}, pv[4] = {0u, 0u, 0u, 0u};
       if constexpr (OUTL) {
         if (vstep) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int t = 2 * j + ((x & 1) ^ vswz) + (x >> 1) * 8;
-            fv_pre[x] = __shfl_sync(0xffffffffu, before, t) >> 16;
-            fv[x] = t0 + t < s.kv ? reinterpret_cast<const uint32_t*>(sp + L.flv)[t] : 0u;
-            const float rs = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsv)[t], p.sdt);
-            vi[x] = rs != 0.f ? __fdividef(p.qmaxf, rs) : 0.f;
+            const uint32_t f = __shfl_sync(0xffffffffu, fl, 16 + t);
+            fv[x] = f >> (r * NVG);
+            pv[x] = at_v + 8u * (__shfl_sync(0xffffffffu, before, 16 + t) + __popc(f & ((1u << (r * NVG)) - 1u)));
           }
         }
       }
@@ -383,15 +406,13 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         });
         if constexpr (OUTL) {
           if (vstep & (1u << g)) {
+            uint2 v[4];
+            values_at(v, pv, 4);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int c = r * NVG + g;
-              if ((fv[x] >> c) & 1u) {
-                const uint32_t rel = fv_pre[x] + __popc(fv[x] & ((1u << c) - 1u));
-                const float4 y = values_of(flagged_value(p.pool.V, sp, L.payv, reinterpret_cast<const uint32_t*>(sp + L.off)[2], rel, ph), p.pool.V.out_dtype);
-                lo[x] = pack_half2(y.x * vi[x], y.y * vi[x]);
-                hi[x] = pack_half2(y.z * vi[x], y.w * vi[x]);
-              }
+              const bool f = (fv[x] & (1u << g)) != 0u;
+              lo[x] = f ? v[x].x : lo[x]; hi[x] = f ? v[x].y : hi[x];
+              pv[x] += f ? 8u : 0u;
             }
           }
         }
@@ -458,7 +479,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
     for (int idx = threadIdx.x; idx < NB * NOT * 32; idx += THREADS) {
       float4 x; float2 m, l;
       merge_parts<N, NB>(idx, lb - la + 1, part_of, x, m, l);
-      if (done) emit_merged<N, NB>(p, v, h, idx, x, m, l);
+      if (done) emit_merged<N, NB>(p, seq_of(p, v), h, idx, x, m, l);
       else {
         float* dst = out_parts + (b0 > c0 ? PART : 0);
         reinterpret_cast<float4*>(dst)[idx] = x;
@@ -472,21 +493,23 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   }
 }
 
-// Units cut between CTAs: blockIdx.x = the cut, blockIdx.y = KV head.
+// Units cut between CTAs: blockIdx.x = the cut, blockIdx.y = KV head, blockIdx.z = 64 of the part's quadruples.
 template <int N, int NB>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(64) paged_merge_kernel(const DecodeParams p) {
   constexpr int NW = NB == 1 ? kDecWarps : kDecWarpsWide, PART = part_floats<N, NB>();
+  // (the plan was there before the kernel ahead of this one)
+  const bool mine = (int)blockIdx.x < p.hdr[5];
+  const int4 c = __ldg(p.cuts + (mine ? blockIdx.x : 0));
+  const Seq s = seq_of(p, mine ? c.x : 0);
   grid_dep_wait();
-  if ((int)blockIdx.x >= p.hdr[5]) return;
-  const int4 c = __ldg(p.cuts + blockIdx.x);
+  if (!mine) return;
   const int h = blockIdx.y, grid = p.ctas * (int)gridDim.y;
   const float* base = p.parts + ((size_t)grid * NW + (size_t)h * p.ctas) * 2 * PART;
   auto part_of = [&](int x) { return base + ((size_t)(c.y + x) * 2 + (x == 0 ? c.w : 0)) * PART; };
-  for (int idx = threadIdx.x; idx < NB * N / 4 * 32; idx += 256) {
-    float4 x; float2 m, l;
-    merge_parts<N, NB>(idx, c.z - c.y + 1, part_of, x, m, l);
-    emit_merged<N, NB>(p, c.x, h, idx, x, m, l);
-  }
+  const int idx = blockIdx.z * 64 + threadIdx.x;
+  float4 x; float2 m, l;
+  merge_parts<N, NB>(idx, c.z - c.y + 1, part_of, x, m, l);
+  emit_merged<N, NB>(p, s, h, idx, x, m, l);
 }
 
 struct DecodeKernels { const void* decode; const void* merge; };

@@ -32,6 +32,7 @@ struct MassParams {
   float2* cta_parts;             // [CTA][2][rows]
   float2* stats;                 // [head][unit][rows]: units that no CTA boundary cuts
   const float* prior; float* mass; float decay;
+  uint4* wide;                   // [CTA][warps][16 N]: values of a tile with more flagged chunks than a stage holds
 };
 
 __device__ __forceinline__ float2 joined(float2 a, float2 b) {        // (m, l) of two parts
@@ -66,26 +67,29 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
     it.u = __ldg(p.wunit + w);
     it.unit(p.units, p.seqs, f0 - __ldg(p.base + it.u));
   }
-  auto stage = [&](int i) {
+  Stager<false, OUTL> sg;
+  sg.init(p.pool, L, lane);
+  auto stage = [&](uint32_t at) {
     const int page = __ldg(p.tabs + it.tab + ((it.tile * kTile) >> p.pool.page_bits));
-    const int st = i % kTileStages;
-    stage_tile<false, OUTL>(p.pool, L, ROW, ring32 + st * L.bytes, ring + st * L.bytes, h, page, it.tile, lane);
+    sg.template tile<IB ? row_bytes_of<N, IB, RB>() : 0>(p.pool, L, ROW, ring32 + at, ring + at, h, page, it.tile, lane);
     it.next(p.units, p.seqs);
   };
-  if (n > 0) stage(0);
-  if (n > 1) stage(1);
+  uint32_t at0 = 0u, at1 = L.bytes, at2 = 2 * L.bytes;
+  if (n > 0) stage(at0);
+  if (n > 1) stage(at1);
   cp_commit();
   load_table<THREADS>(tblK, p.tblK, h, p.table_rows, p.repk);
   __syncthreads();
   if constexpr (OUTL) {
     cp_wait_all();
     __syncwarp();
-    if (n > 0) stage_values<false>(p.pool, L, ring32, ring, h, lane);
+    if (n > 0) stage_values<false>(p.pool, L, ring32, ring, lane);
     cp_commit();
   }
   const uint32_t laneK = (uint32_t)(lane & ((1 << p.repk) - 1)) * 8u;
   FL ld;
   ld.row_bytes = ROW; ld.row_words = ROW / 4; ld.j = j; ld.r = r; ld.sdt = p.sdt;
+  auto my_wide = [&] { return p.wide + ((size_t)blockIdx.x * NW + (threadIdx.x >> 5)) * (16 * N); };
   float2* my_parts = p.parts + ((size_t)blockIdx.x * NW + warp) * 2 * R;
 
   int u = n > 0 ? __ldg(p.wunit + w) : 0, i = 0;
@@ -99,7 +103,7 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
     float qmul[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float mul = load_query<NKS>(qb[nb], p.q, s.q_off, h, row0 + nb * 8 + r, rows, j);
+      const float mul = load_query<NKS, false>(qb[nb], p.q, s.q_off, h, row0 + nb * 8 + r, rows, j);
       qmul[nb][0] = __shfl_sync(0xffffffffu, mul, 8 * j);
       qmul[nb][1] = __shfl_sync(0xffffffffu, mul, 8 * j + 4);
     }
@@ -114,11 +118,12 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
       cp_wait_all();
       __syncwarp();
       if constexpr (OUTL) {
-        if (i + 1 < n) { const int st = (i + 1) % kTileStages; stage_values<false>(p.pool, L, ring32 + st * L.bytes, ring + st * L.bytes, h, lane); }
+        if (i + 1 < n) stage_values<false>(p.pool, L, ring32 + at1, ring + at1, lane);
       }
-      if (i + 2 < n) stage(i + 2);
+      if (i + 2 < n) stage(at2);
       cp_commit();
-      const unsigned char* sp = ring + (i % kTileStages) * L.bytes;
+      unsigned char* sp = ring + at0;
+      { const uint32_t x = at0; at0 = at1; at1 = at2; at2 = x; }
       const int t0 = tile * kTile;
       const bool edge = t0 + kTile > p_first + 1 || t0 < edge_lo;
       uint32_t kw[2][FL::KW + 1];
@@ -129,25 +134,55 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
         if constexpr (IB != 0) ld.template load_span<FL::KW, FL::LK>(kw[nt], sp + t * ROW, j, true);
         rs[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt);
       }
-      uint32_t kstep = 0u, fk[2] = {0u, 0u}, fk_pre[2] = {0u, 0u};
-      float kinv[2] = {0.f, 0.f};
+      uint32_t kstep = 0u, fk[2] = {0u, 0u}, pk[2] = {0u, 0u};
+      bool wide = false;
       if constexpr (OUTL) {
         uint32_t fk_t = 0u;
         if (lane < kTile && t0 + lane < s.kv) fk_t = reinterpret_cast<const uint32_t*>(sp + L.flk)[lane];
         kstep = __reduce_or_sync(0xffffffffu, fk_t);
         if (kstep) {
-          const uint32_t before = counts_before(__popc(fk_t), lane);
+          // Every lane its token's values times qmax / rs in two halves (see paged_decode.cuh).  An entry takes 16 bytes then, so a stage
+          // holds half as many, and they are read before any is written.
+          const uint32_t own = __popc(fk_t), before = counts_before(own, lane);
+          const Entries en = entries_of<false>(p.pool, L, sp);
+          wide = __any_sync(0xffffffffu, own != 0u && before + own > min(en.nk, (uint32_t)kPay / 2)) || __reduce_max_sync(0xffffffffu, own) > 4u;
+          const float rs_t = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[lane & 15], p.sdt);
+          const float inv = rs_t != 0.f ? __fdiv_rn(p.qmaxf, rs_t) : 0.f;
+          auto operand = [&](uint2 v) {
+            float4 x = values_of(v, p.pool.K.out_dtype);
+            x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+            uint4 o;
+            o.x = pack_half2(x.x, x.y); o.y = pack_half2(x.z, x.w);
+            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&o.x)), g2 = __half22float2(*reinterpret_cast<const __half2*>(&o.y));
+            o.z = pack_half2(x.x - g.x, x.y - g.y); o.w = pack_half2(x.z - g2.x, x.w - g2.y);
+            return o;
+          };
+          if (!wide) {
+            uint2 v[4];
+            const uint2* e = reinterpret_cast<const uint2*>(sp + L.pay) + before;
+            uint4* d = reinterpret_cast<uint4*>(sp + L.pay) + before;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) if (x < (int)own) v[x] = e[x];
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 4; ++x) if (x < (int)own) d[x] = operand(v[x]);
+          } else {
+            const int64_t ph = *reinterpret_cast<const int*>(sp + L.off + 16);
+            uint32_t from = en.k0 + before;
+            for (uint32_t x = 0; x < own; ++x, ++from)
+              my_wide()[before + x] = operand(from < (uint32_t)p.pool.K.out_cap ? __ldg(reinterpret_cast<const uint2*>(p.pool.K.out_vals) + ph * p.pool.K.out_cap + from) : make_uint2(0u, 0u));
+          }
+          __syncwarp();
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) {
-            fk[nt] = __shfl_sync(0xffffffffu, fk_t, nt * 8 + r);
-            fk_pre[nt] = __shfl_sync(0xffffffffu, before, nt * 8 + r);
-            kinv[nt] = rs[nt] != 0.f ? __fdiv_rn(p.qmaxf, rs[nt]) : 0.f;
+            const uint32_t f = __shfl_sync(0xffffffffu, fk_t, nt * 8 + r);
+            fk[nt] = f >> (j * NKS);
+            pk[nt] = 16u * (__shfl_sync(0xffffffffu, before, nt * 8 + r) + __popc(f & ((1u << (j * NKS)) - 1u)));
           }
         }
         if constexpr (NKS == 8) { kstep |= kstep >> 16; kstep |= kstep >> 8; kstep &= 0xffu; }
         else { kstep |= kstep >> 8; kstep |= kstep >> 4; kstep &= 0xfu; }
       }
-      const int64_t ph = OUTL ? (int64_t)*reinterpret_cast<const int*>(sp + L.off + 16) * p.pool.Hkv + h : 0;
       // two chains of the high halves' products and one of the low ones': the tensor cores cut a sum's bits with every step
       float sc[NB][4], s2[NB][4], s3[NB][4];
 #pragma unroll
@@ -173,21 +208,21 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
         });
         if constexpr (OUTL) {
           if (kstep & (1u << ks)) {
+            uint4 v[2];
+            if (!wide) {
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt) v[nt] = *reinterpret_cast<const uint4*>(sp + L.pay + pk[nt]);
+            } else {
+              const unsigned char* far = reinterpret_cast<const unsigned char*>(my_wide());
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt) v[nt] = __ldcg(reinterpret_cast<const uint4*>(far + pk[nt]));
+            }
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
-              const int c = j * NKS + ks;
-              if ((fk[nt] >> c) & 1u) {
-                const uint32_t rel = fk_pre[nt] + __popc(fk[nt] & ((1u << c) - 1u));
-                const float4 x = values_of(flagged_value(p.pool.K, sp, L.payk, reinterpret_cast<const uint32_t*>(sp + L.off)[0], rel, ph), p.pool.K.out_dtype);
-                auto split = [&](float v0, float v1, uint32_t& hi, uint32_t& lo) {
-                  v0 *= kinv[nt]; v1 *= kinv[nt];
-                  hi = pack_half2(v0, v1);
-                  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                  lo = pack_half2(v0 - g.x, v1 - g.y);
-                };
-                split(x.x, x.y, a[nt], b[nt]);
-                split(x.z, x.w, a[2 + nt], b[2 + nt]);
-              }
+              const bool f = (fk[nt] & (1u << ks)) != 0u;
+              a[nt] = f ? v[nt].x : a[nt]; a[2 + nt] = f ? v[nt].y : a[2 + nt];
+              b[nt] = f ? v[nt].z : b[nt]; b[2 + nt] = f ? v[nt].w : b[2 + nt];
+              pk[nt] += f ? 16u : 0u;
             }
           }
         }

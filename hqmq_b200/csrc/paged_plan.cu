@@ -11,6 +11,7 @@ bool chunked(int q, int G) { return q * G > 16; }
 
 int check_plan(const hqmq_paged_plan& p) {
   if (p.struct_size != sizeof(hqmq_paged_plan)) return HQMQ_ERR_ARG;
+  if ((int64_t)p.n_pages * p.H_kv > 0x7fffffff) return HQMQ_ERR_SHAPE;
   if (p.n_seqs < 1 || p.n_seqs > (1 << 20) || p.n_pages < 1 || p.H_kv < 1 || p.H_kv > 1024 || p.window < 0) return HQMQ_ERR_SHAPE;
   if (p.page_tokens < HQMQ_T_ALIGN || (p.page_tokens & (p.page_tokens - 1)) || p.page_tokens > kMaxPage) return HQMQ_ERR_SHAPE;
   if (p.d != 64 && p.d != 128) return HQMQ_ERR_UNSUPPORTED;

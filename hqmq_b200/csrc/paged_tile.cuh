@@ -10,26 +10,25 @@
 namespace hqmq {
 namespace paged {
 
-constexpr int kPay = 48;       // values of flagged chunks staged per tile and tensor; further ones are read from global memory
+constexpr int kPay = 96;       // values of flagged chunks staged per tile, of both tensors (of a tile with more, all go through global memory)
 constexpr int kTileStages = 3;
 
 // Rows of IB + RB bits per chunk; IB = 0: any width, at run time.
 template <int N, int IB, int RB>
 __host__ __device__ constexpr int row_bytes_of() { return (N * (IB + RB) + 31) / 32 * 4; }
 
-// Where the parts of a stage lie.
-struct TileLayout { int v, rsk, rsv, flk, flv, off, payk, payv, bytes; };
+// Where the parts of a stage lie.  Values of flagged chunks: K's, then V's (each 8 bytes, or 16 where a value is kept in two halves).
+struct TileLayout { int v, rsk, rsv, flk, flv, off, pay, bytes; };
 __host__ __device__ constexpr TileLayout tile_layout(int row, bool hasv, bool outl) {
   TileLayout l{};
   int at = kTile * row;
   l.v = at; at += hasv ? kTile * row : 0;
-  l.rsk = at; at += kTile * 2;
+  l.rsk = at; at += kTile * 2;              // (V's follow K's: the two are read as one array of 32)
   l.rsv = at; at += hasv ? kTile * 2 : 0;
   l.flk = at; at += outl ? kTile * 4 : 0;
   l.flv = at; at += outl && hasv ? kTile * 4 : 0;
-  l.off = at; at += outl ? 32 : 0;          // K: before, behind; V: before, behind; page
-  l.payk = at; at += outl ? kPay * 8 : 0;
-  l.payv = at; at += outl && hasv ? kPay * 8 : 0;
+  l.off = at; at += outl ? 32 : 0;          // K's entries before the tile and behind it; V's; page
+  l.pay = at; at += outl ? kPay * 8 : 0;
   l.bytes = (at + 15) & ~15;
   return l;
 }
@@ -54,60 +53,83 @@ struct TileIter {
   }
 };
 
+// A lane's share of the copies of a tile: its 16 bytes of the code rows, and one piece of the scales, flag words or offsets.
 template <bool HASV, bool OUTL>
-__device__ __forceinline__ void stage_tile(const PoolView& p, const TileLayout& l, int row_bytes, uint32_t sb, unsigned char* sp, int h, int page,
-                                           int tile, int lane) {
-  const int in_page = (tile * kTile) & ((1 << p.page_bits) - 1);
-  const int64_t ph = (int64_t)page * p.Hkv + h;
-  const int64_t row = (ph << p.page_bits) + in_page;
-  const int n16 = row_bytes;                                  // 16 rows of row_bytes, 16 bytes at a time
-  const unsigned char* k = p.K.codes + row * row_bytes;
-  for (int c = lane; c < n16; c += 32) cp_async16(sb + 16 * c, k + 16 * c);
-  if constexpr (HASV) {
-    const unsigned char* v = p.V.codes + row * row_bytes;
-    for (int c = lane; c < n16; c += 32) cp_async16(sb + l.v + 16 * c, v + 16 * c);
-  }
-  // the small parts: a lane each
-  const unsigned char* src = nullptr;
-  uint32_t dst = 0;
-  if (lane < 2) { src = reinterpret_cast<const unsigned char*>(p.K.rs) + row * 2 + lane * 16; dst = l.rsk + lane * 16; }
-  else if (HASV && lane < 4) { src = reinterpret_cast<const unsigned char*>(p.V.rs) + row * 2 + (lane - 2) * 16; dst = l.rsv + (lane - 2) * 16; }
-  else if (OUTL && lane >= 4 && lane < 8) { if (p.K.flags) { src = reinterpret_cast<const unsigned char*>(p.K.flags + row) + (lane - 4) * 16; dst = l.flk + (lane - 4) * 16; } }
-  else if (OUTL && HASV && lane >= 8 && lane < 12) { if (p.V.flags) { src = reinterpret_cast<const unsigned char*>(p.V.flags + row) + (lane - 8) * 16; dst = l.flv + (lane - 8) * 16; } }
-  if (src) cp_async16(sb + dst, src);
-  if constexpr (OUTL) {
-    const int64_t o = ph * ((1 << p.page_bits) / HQMQ_OUT_BLOCK + 1) + in_page / HQMQ_OUT_BLOCK;
-    if (lane >= 12 && lane < 14 && p.K.flags) cp_async4(sb + l.off + (lane - 12) * 4, p.K.out_off + o + (lane - 12));
-    if (HASV && lane >= 14 && lane < 16 && p.V.flags) cp_async4(sb + l.off + (lane - 12) * 4, p.V.out_off + o + (lane - 14));
-    if (lane == 16) *reinterpret_cast<int*>(sp + l.off + 16) = page;
-  }
-}
-
-// The values of a staged tile's flagged chunks (an entry the side buffer had no room for reads as 0).
-template <bool HASV>
-__device__ __forceinline__ void stage_values(const PoolView& p, const TileLayout& l, uint32_t sb, unsigned char* sp, int h, int lane) {
-  const uint32_t* off = reinterpret_cast<const uint32_t*>(sp + l.off);
-  const int64_t ph = (int64_t)(int)off[4] * p.Hkv + h;
-  auto side = [&](const hqmq_packed& x, uint32_t lo, uint32_t hi, int at) {
-    const uint32_t n = hi - lo < (uint32_t)kPay ? hi - lo : (uint32_t)kPay;
-    const unsigned char* v = reinterpret_cast<const unsigned char*>(x.out_vals) + ph * x.out_cap * 8;
-    for (uint32_t i = lane; i < n; i += 32) {
-      const uint32_t e = lo + i;
-      if (e < (uint32_t)x.out_cap) cp_async8(sb + at + 8 * i, v + (int64_t)e * 8);
-      else *reinterpret_cast<uint2*>(sp + at + 8 * i) = make_uint2(0u, 0u);
+struct Stager {
+  const unsigned char* k; const unsigned char* v; const unsigned char* small; const uint32_t* off;
+  uint32_t small_mul, small_dst, off_dst;      // bytes per row of the small piece (0: none), places in the stage
+  __device__ __forceinline__ void init(const PoolView& p, const TileLayout& l, int lane) {
+    k = p.K.codes + 16 * lane;
+    v = HASV ? p.V.codes + 16 * lane : nullptr;
+    small = nullptr; small_mul = small_dst = 0u; off = nullptr; off_dst = 0u;
+    auto piece = [&](const void* base, int i, int mul, int dst) {
+      if (base) { small = reinterpret_cast<const unsigned char*>(base) + 16 * i; small_mul = mul; small_dst = dst + 16 * i; }
+    };
+    if (lane < 2) piece(p.K.rs, lane, 2, l.rsk);
+    else if (HASV && lane < 4) piece(p.V.rs, lane - 2, 2, l.rsv);
+    else if (OUTL && lane >= 4 && lane < 8) piece(p.K.flags, lane - 4, 4, l.flk);
+    else if (OUTL && HASV && lane >= 8 && lane < 12) piece(p.V.flags, lane - 8, 4, l.flv);
+    if constexpr (OUTL) {
+      if (lane >= 12 && lane < 14 && p.K.flags) { off = p.K.out_off + (lane - 12); off_dst = l.off + (lane - 12) * 4; }
+      if (HASV && lane >= 14 && lane < 16 && p.V.flags) { off = p.V.out_off + (lane - 14); off_dst = l.off + (lane - 12) * 4; }
     }
-  };
-  if (p.K.flags) side(p.K, off[0], off[1], l.payk);
-  if (HASV && p.V.flags) side(p.V, off[2], off[3], l.payv);
+  }
+  template <int ROWC>
+  __device__ __forceinline__ void tile(const PoolView& p, const TileLayout& l, int row_bytes, uint32_t sb, unsigned char* sp, int h, int page,
+                                       int tile, int lane) const {
+    const int in_page = (tile * kTile) & ((1 << p.page_bits) - 1), ph = page * p.Hkv + h;
+    const int64_t row = ((int64_t)ph << p.page_bits) + in_page;
+    const unsigned char* ks = k + row * row_bytes;
+    const unsigned char* vs = HASV ? v + row * row_bytes : nullptr;
+    // (16 rows of row_bytes are row_bytes pieces of 16 bytes)
+    if constexpr (ROWC != 0) {
+#pragma unroll
+      for (int c = 0; c < (ROWC + 31) / 32; ++c) {
+        if (32 * c + 32 <= ROWC || lane < ROWC - 32 * c) {
+          cp_async16(sb + 16 * lane + 512 * c, ks + 512 * c);
+          if constexpr (HASV) cp_async16(sb + l.v + 16 * lane + 512 * c, vs + 512 * c);
+        }
+      }
+    } else {
+      for (int c = 0; c * 32 + lane < row_bytes; ++c) {
+        cp_async16(sb + 16 * lane + 512 * c, ks + 512 * c);
+        if constexpr (HASV) cp_async16(sb + l.v + 16 * lane + 512 * c, vs + 512 * c);
+      }
+    }
+    if (small_mul) cp_async16(sb + small_dst, small + row * small_mul);
+    if constexpr (OUTL) {
+      if (off_dst) cp_async4(sb + off_dst, off + (int64_t)ph * ((1 << p.page_bits) / HQMQ_OUT_BLOCK + 1) + in_page / HQMQ_OUT_BLOCK);
+      if (lane == 16) *reinterpret_cast<int*>(sp + l.off + 16) = ph;
+    }
+  }
+};
+
+// The values of a staged tile's flagged chunks, 8 bytes each: K's first, then V's, as many as there is room for (an entry the side
+// buffer had no room for reads as 0).  Ranges: entries before the tile and behind it.
+struct Entries { uint32_t k0, nk, v0, nv; };
+template <bool HASV>
+__device__ __forceinline__ Entries entries_of(const PoolView& p, const TileLayout& l, const unsigned char* sp) {
+  const uint4 o = *reinterpret_cast<const uint4*>(sp + l.off);
+  Entries e;
+  e.k0 = o.x; e.v0 = o.z;
+  e.nk = p.K.flags ? min(o.y - o.x, (uint32_t)kPay) : 0u;
+  e.nv = HASV && p.V.flags ? min(o.w - o.z, (uint32_t)kPay - e.nk) : 0u;
+  return e;
+}
+template <bool HASV>
+__device__ __forceinline__ void stage_values(const PoolView& p, const TileLayout& l, uint32_t sb, unsigned char* sp, int lane) {
+  const Entries e = entries_of<HASV>(p, l, sp);
+  if (e.nk + e.nv == 0u) return;
+  const int64_t ph = *reinterpret_cast<const int*>(sp + l.off + 16);
+  for (uint32_t i = lane; i < e.nk + e.nv; i += 32) {
+    const bool is_v = HASV && i >= e.nk;
+    const uint32_t at = is_v ? e.v0 + (i - e.nk) : e.k0 + i, cap = is_v ? (uint32_t)p.V.out_cap : (uint32_t)p.K.out_cap;
+    const unsigned char* v = reinterpret_cast<const unsigned char*>(is_v ? p.V.out_vals : p.K.out_vals);
+    if (at < cap) cp_async8(sb + l.pay + 8 * i, v + (ph * cap + at) * 8);
+    else *reinterpret_cast<uint2*>(sp + l.pay + 8 * i) = make_uint2(0u, 0u);
+  }
 }
 
-// The value of a flagged chunk: entry `rel` of the tile's, two words of two 16-bit values.
-__device__ __forceinline__ uint2 flagged_value(const hqmq_packed& x, const unsigned char* sp, int at, uint32_t lo, uint32_t rel, int64_t ph) {
-  if (rel < (uint32_t)kPay) return *reinterpret_cast<const uint2*>(sp + at + 8 * rel);
-  const uint32_t e = lo + rel;
-  if (e >= (uint32_t)x.out_cap) return make_uint2(0u, 0u);
-  return __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned char*>(x.out_vals) + (ph * x.out_cap + e) * 8));
-}
 __device__ __forceinline__ float4 values_of(uint2 v, int dtype) {
   float2 a, b;
   if (dtype == HQMQ_BF16) {
@@ -120,13 +142,13 @@ __device__ __forceinline__ float4 values_of(uint2 v, int dtype) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// Sums of two 16-bit counts per lane over the lanes before it (lanes 0..15 of the tile's tokens).
+// Sum over the lanes before this one in its half of the warp.
 __device__ __forceinline__ uint32_t counts_before(uint32_t own, int lane) {
   uint32_t x = own;
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o, 16);
+    if ((lane & 15) >= o) x += y;
   }
   return x - own;
 }
@@ -161,8 +183,9 @@ __device__ __forceinline__ void load_table(unsigned char* tbl, const uint16_t* s
 struct QueryView { const void* Q; int dtype, vec; int64_t st_t, st_h; int G; };
 
 // Row `row` (query * G + head) of a unit, this lane's dims [4 NKS j, 4 NKS (j + 1)), in fp16 after division by a power of two that
-// brings the row's largest value to [1, 2); returns that power.  A row that is not there is zeros.
-template <int NKS>
+// brings the row's largest value to [1, 2); returns that power.  (SHARED: the largest of the warp's eight rows, one power for all.)  A
+// row that is not there is zeros.
+template <int NKS, bool SHARED>
 __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& q, int q_off, int h, int row, int rows, int j) {
   float f[4 * NKS];
   const int qi = row / q.G, g = row - qi * q.G;
@@ -189,6 +212,10 @@ __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& 
   for (int i = 0; i < 4 * NKS; ++i) m = fmaxf(m, fabsf(f[i]));
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  if constexpr (SHARED) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  }
   int e = (int)(__float_as_uint(m) >> 23) - 127;               // (subnormal: -127; infinite: 128)
   e = min(126, max(-126, e));
   const float div = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -200,11 +227,6 @@ __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& 
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // softcap * tanh(x / softcap) in the exp2 domain, from x * 2 log2(e) / softcap: 1 - 2 / (2^y + 1)
 __device__ __forceinline__ float capped(float y, float cap_log2) { return cap_log2 - __fdividef(2.f * cap_log2, fast_exp2(y) + 1.f); }
 
