@@ -2,12 +2,11 @@
 //
 // The tile's arithmetic is that of the staged decode kernels (attn_kernel.cuh): S^T = K Q^T with the 16 tokens as rows and the query
 // rows as columns, O^T += V^T P^T, operands gathered from shared-memory tables straight into fragments.  What differs: a warp walks
-// its own stretch of tiles from unit to unit (paged.cuh); flagged chunks, which decode to zero, are put into the fragments before
-// their product: a lane per entry turns the tile's values into fp16(x * qmax / rs), what the table would have given, once; a lane owns
-// 2 tokens x N / 4 chunks of K and 4 x N / 8 of V, its entries are neighbours in the side buffer's order, so that it walks a pointer along
-// them, in the steps (one word per tile says which) that have any.  (With the value looked up, counted for and converted by every lane in
-// every step: 1370 instructions a tile against 745 without outliers, and the loop outgrew the instruction cache.)  V's scales enter P relative to the largest
-// one seen, a power of two that the accumulators are rescaled by like by the maximum, so that values of any size keep their bits.
+// its own stretch of tiles from unit to unit (paged.cuh); flagged chunks, which decode to zero, are products of their own behind the
+// others': a lane per token turns its values into fp16(x * qmax / rs), what the table would have given, and a lane, which owns 2 tokens
+// x N / 4 chunks of K and 4 x N / 8 of V, finds its own in the side buffer's order by counting the flags before them; V's scales enter P
+// relative to the largest one seen, a power of two that the accumulators are rescaled by like by the maximum, so that values of any size
+// keep their bits.
 #pragma once
 #include "attn_tma.cuh"
 #include "paged_tile.cuh"
@@ -119,13 +118,13 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   if (n > 0) {
     it.u = __ldg(p.wunit + w);
     it.unit(p.units, p.seqs, f0 - __ldg(p.base + it.u));
+    it.find_page(p.tabs, p.pool.page_bits);
   }
   Stager<true, OUTL> sg;
   sg.init(p.pool, L, lane);
   auto stage = [&](uint32_t at) {    // the tile that `it` is at, to the stage at `at`
-    const int page = __ldg(p.tabs + it.tab + ((it.tile * kTile) >> p.pool.page_bits));
-    sg.template tile<IB ? row_bytes_of<N, IB, RB>() : 0>(p.pool, L, ROW, ring32 + at, ring + at, h, page, it.tile, lane);
-    it.next(p.units, p.seqs);
+    sg.template tile<IB ? row_bytes_of<N, IB, RB>() : 0>(p.pool, L, ROW, ring32 + at, ring + at, h, it.page, it.tile, lane);
+    it.next(p.units, p.seqs, p.tabs, p.pool.page_bits);
   };
   uint32_t at0 = 0u, at1 = L.bytes, at2 = 2 * L.bytes;       // stages of the tile at hand, of the next two
   if (n > 0) stage(at0);
@@ -203,21 +202,17 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         const int t = 2 * j + ((x & 1) ^ vswz) + (x >> 1) * 8;
         if constexpr (IB != 0) ld.template load_span<FL::VW, FL::LV>(vw[x], sp + L.v + t * ROW, r, !edge || t0 + t < s.kv);
       }
-      uint32_t kstep = 0u, vstep = 0u;       // bit x: some lane has a flagged chunk in step x
-      uint32_t fk[2] = {0u, 0u}, pk[2] = {0u, 0u};        // flags of this lane's chunks from bit 0 on, place of the first one's value
-      uint32_t fl = 0u, before = 0u, at_v = 0u;
+      uint32_t kcols = 0u, vcols = 0u;       // the columns of chunks in which some token of the tile has a flagged one
+      uint32_t fl = 0u, before = 0u;         // lanes 0..15: K's tokens, 16..31: V's: flags, and entries of the tile's earlier tokens
       bool wide = false;
       if constexpr (OUTL) {
-        // lanes 0..15: K's tokens, 16..31: V's
         if (t0 + (lane & 15) < s.kv && (lane < 16 ? p.pool.K.flags : p.pool.V.flags)) fl = reinterpret_cast<const uint32_t*>(sp + L.flk)[lane];
-        kstep = __reduce_or_sync(0xffffffffu, lane < 16 ? fl : 0u);
-        vstep = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : fl);
-        if (kstep | vstep) {
+        kcols = __reduce_or_sync(0xffffffffu, lane < 16 ? fl : 0u);
+        vcols = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : fl);
+        if (kcols | vcols) {
           const uint32_t own = __popc(fl);
-          const Entries en = entries_of<true>(p.pool, L, sp);
           before = counts_before(own, lane);
-          wide = __any_sync(0xffffffffu, before + own > (lane < 16 ? en.nk : en.nv));
-          at_v = wide ? 16u * N * 8u : en.nk * 8u;
+          wide = __any_sync(0xffffffffu, before + own > (lane < 16 ? kPayK : kPayV));
           // every lane its token's values, in place
           const float rs = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[lane], p.sdt);
           const float inv = rs != 0.f ? __fdividef(p.qmaxf, rs) : 0.f;
@@ -227,38 +222,28 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
             return make_uint2(pack_half2(x.x * inv, x.y * inv), pack_half2(x.z * inv, x.w * inv));
           };
           if (!wide) {
-            uint2* e = reinterpret_cast<uint2*>(sp + L.pay + (lane < 16 ? 0u : at_v)) + before;
+            uint2* e = reinterpret_cast<uint2*>(sp + L.pay + (lane < 16 ? 0 : kPayK * 8)) + before;
             for (uint32_t x = 0; x < own; ++x, ++e) *e = operand(*e);
           } else {
             const int64_t ph = *reinterpret_cast<const int*>(sp + L.off + 16);
-            const hqmq_packed& pk_ = lane < 16 ? p.pool.K : p.pool.V;
+            const hqmq_packed& pk = lane < 16 ? p.pool.K : p.pool.V;
             uint2* e = my_wide() + (lane < 16 ? 0 : 16 * N) + before;
-            uint32_t from = (lane < 16 ? en.k0 : en.v0) + before;
+            uint32_t from = reinterpret_cast<const uint32_t*>(sp + L.off)[lane < 16 ? 0 : 2] + before;
             for (uint32_t x = 0; x < own; ++x, ++e, ++from)
-              *e = operand(from < (uint32_t)pk_.out_cap ? __ldg(reinterpret_cast<const uint2*>(pk_.out_vals) + ph * pk_.out_cap + from) : make_uint2(0u, 0u));
+              *e = operand(from < (uint32_t)pk.out_cap ? __ldg(reinterpret_cast<const uint2*>(pk.out_vals) + ph * pk.out_cap + from) : make_uint2(0u, 0u));
           }
           __syncwarp();
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const uint32_t f = __shfl_sync(0xffffffffu, fl, nt * 8 + r);
-            fk[nt] = f >> (j * NKS);
-            pk[nt] = 8u * (__shfl_sync(0xffffffffu, before, nt * 8 + r) + __popc(f & ((1u << (j * NKS)) - 1u)));
-          }
         }
-        // chunks j * NKS + ks / r * NVG + g: which ks, which g
-        if constexpr (NKS == 8) { kstep |= kstep >> 16; kstep |= kstep >> 8; kstep &= 0xffu; }
-        else { kstep |= kstep >> 8; kstep |= kstep >> 4; kstep &= 0xfu; }
-        if constexpr (NVG == 4) { vstep |= vstep >> 16; vstep |= vstep >> 8; vstep |= vstep >> 4; vstep &= 0xfu; }
-        else { vstep |= vstep >> 8; vstep |= vstep >> 4; vstep |= vstep >> 2; vstep &= 3u; }
       }
-      auto values_at = [&](uint2* v, const uint32_t* at, int n_) {     // operands of flagged chunks
+      // Operands of flagged chunks at places counted in entries.  No branch per lane: a place is one of this tile's, or the one behind
+      // the last, whether the lane has a value there or not.
+      auto values_at = [&](uint2* v, const uint32_t* at, int n_, bool of_v) {
         if (!wide) {
 #pragma unroll
-          for (int x = 0; x < n_; ++x) v[x] = *reinterpret_cast<const uint2*>(sp + L.pay + at[x]);
+          for (int x = 0; x < n_; ++x) v[x] = reinterpret_cast<const uint2*>(sp + L.pay + (of_v ? kPayK * 8 : 0))[at[x]];
         } else {
-          const unsigned char* far = reinterpret_cast<const unsigned char*>(my_wide());
 #pragma unroll
-          for (int x = 0; x < n_; ++x) v[x] = __ldcg(reinterpret_cast<const uint2*>(far + at[x]));
+          for (int x = 0; x < n_; ++x) v[x] = __ldcg(my_wide() + (of_v ? 16 * N : 0) + at[x]);
         }
       };
 
@@ -280,22 +265,41 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
           a[nt] = hmul2_u32(cw.x, rr);
           a[2 + nt] = hmul2_u32(cw.y, rr);
         });
-        if constexpr (OUTL) {
-          if (kstep & (1u << ks)) {
-            // (no branch per lane: the place is a place of this tile, or the one behind its last, whoever has a value there or not)
-            uint2 v[2];
-            values_at(v, pk, 2);
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-              const bool f = (fk[nt] & (1u << ks)) != 0u;
-              a[nt] = f ? v[nt].x : a[nt]; a[2 + nt] = f ? v[nt].y : a[2 + nt];
-              pk[nt] += f ? 8u : 0u;
-            }
-          }
-        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) mma16816((ks & 1) ? s2[nb] : sc[nb], a[0], a[1], a[2], a[3], qb[nb][ks][0], qb[nb][ks][1]);
       });
+
+      // Flagged chunks of K: the four groups of lanes that share a j take a column of theirs each, one more product.  (Put into the
+      // fragments above instead, the branches of every step kept the look-ups from being issued ahead: 381 us against 170 without
+      // outliers for 16 x 32k, 287 with that part left out.)
+      if constexpr (OUTL) {
+        if (kcols) {
+          uint32_t left = (kcols >> (j * NKS)) & ((1u << NKS) - 1u), f[2], at[2];
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            const uint32_t w_ = __shfl_sync(0xffffffffu, fl, nt * 8 + r);
+            f[nt] = w_ >> (j * NKS);
+            at[nt] = __shfl_sync(0xffffffffu, before, nt * 8 + r) + __popc(w_ & ((1u << (j * NKS)) - 1u));
+          }
+          do {
+            const int ks = left ? __ffs(left) - 1 : 0;
+            const bool some = left != 0u;
+            left &= left - 1u;
+            uint2 v[2];
+            values_at(v, at, 2, false);
+            uint32_t a[4];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+              const bool mine = some && ((f[nt] >> ks) & 1u);
+              a[nt] = mine ? v[nt].x : 0u; a[2 + nt] = mine ? v[nt].y : 0u;
+              at[nt] += mine ? 1u : 0u;
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              mma16816(s2[nb], a[0], a[1], a[2], a[3], pick_of<NKS>(qb[nb], 0, ks), pick_of<NKS>(qb[nb], 1, ks));
+          } while (__any_sync(0xffffffffu, left != 0u));
+        }
+      }
 
       // ---- scale, cap, mask -----------------------------------------------------------------------------------------------------
 #pragma unroll
@@ -376,18 +380,6 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       }
 
       // ---- O^T += V^T P^T ---------------------------------------------------------------------------------------------------------
-      uint32_t fv[4] = {0u, 0u, 0u, 0u}, pv[4] = {0u, 0u, 0u, 0u};
-      if constexpr (OUTL) {
-        if (vstep) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int t = 2 * j + ((x & 1) ^ vswz) + (x >> 1) * 8;
-            const uint32_t f = __shfl_sync(0xffffffffu, fl, 16 + t);
-            fv[x] = f >> (r * NVG);
-            pv[x] = at_v + 8u * (__shfl_sync(0xffffffffu, before, 16 + t) + __popc(f & ((1u << (r * NVG)) - 1u)));
-          }
-        }
-      }
       static_for<0, NVG>([&](auto g_) {
         constexpr int g = decltype(g_)::value;
         uint32_t lo[4], hi[4];
@@ -404,18 +396,6 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
           lo[x] = hmul2_u32(cw.x, rr);
           hi[x] = hmul2_u32(cw.y, rr);
         });
-        if constexpr (OUTL) {
-          if (vstep & (1u << g)) {
-            uint2 v[4];
-            values_at(v, pv, 4);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const bool f = (fv[x] & (1u << g)) != 0u;
-              lo[x] = f ? v[x].x : lo[x]; hi[x] = f ? v[x].y : hi[x];
-              pv[x] += f ? 8u : 0u;
-            }
-          }
-        }
         const uint32_t a0 = __byte_perm(lo[0], lo[1], 0x5410), a1 = __byte_perm(lo[0], lo[1], 0x7632);
         const uint32_t a2 = __byte_perm(lo[2], lo[3], 0x5410), a3 = __byte_perm(lo[2], lo[3], 0x7632);
         const uint32_t e0 = __byte_perm(hi[0], hi[1], 0x5410), e1 = __byte_perm(hi[0], hi[1], 0x7632);
@@ -426,6 +406,41 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
           mma16816(o[nb][2 * g + 1], e0, e1, e2, e3, pb[nb][0], pb[nb][1]);
         }
       });
+      // ... of V: two more products for every g that has some
+      if constexpr (OUTL) {
+        if (vcols) {
+          uint32_t f[4], at[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int t = 2 * j + ((x & 1) ^ vswz) + (x >> 1) * 8;
+            const uint32_t w_ = __shfl_sync(0xffffffffu, fl, 16 + t);
+            f[x] = w_ >> (r * NVG);
+            at[x] = __shfl_sync(0xffffffffu, before, 16 + t) + __popc(w_ & ((1u << (r * NVG)) - 1u));
+          }
+          static_for<0, NVG>([&](auto g_) {
+            constexpr int g = decltype(g_)::value;
+            if (vcols & ((NVG == 4 ? 0x11111111u : 0x55555555u) << g)) {
+              uint2 v[4];
+              values_at(v, at, 4, true);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const bool mine = (f[x] & (1u << g)) != 0u;
+                if (!mine) v[x] = make_uint2(0u, 0u);
+                at[x] += mine ? 1u : 0u;
+              }
+              const uint32_t a0 = __byte_perm(v[0].x, v[1].x, 0x5410), a1 = __byte_perm(v[0].x, v[1].x, 0x7632);
+              const uint32_t a2 = __byte_perm(v[2].x, v[3].x, 0x5410), a3 = __byte_perm(v[2].x, v[3].x, 0x7632);
+              const uint32_t e0 = __byte_perm(v[0].y, v[1].y, 0x5410), e1 = __byte_perm(v[0].y, v[1].y, 0x7632);
+              const uint32_t e2 = __byte_perm(v[2].y, v[3].y, 0x5410), e3 = __byte_perm(v[2].y, v[3].y, 0x7632);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                mma16816(o[nb][2 * g], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
+                mma16816(o[nb][2 * g + 1], e0, e1, e2, e3, pb[nb][0], pb[nb][1]);
+              }
+            }
+          });
+        }
+      }
     }
 
     // ---- the unit's result, or a part of it --------------------------------------------------------------------------------------

@@ -66,13 +66,13 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
   if (n > 0) {
     it.u = __ldg(p.wunit + w);
     it.unit(p.units, p.seqs, f0 - __ldg(p.base + it.u));
+    it.find_page(p.tabs, p.pool.page_bits);
   }
   Stager<false, OUTL> sg;
   sg.init(p.pool, L, lane);
   auto stage = [&](uint32_t at) {
-    const int page = __ldg(p.tabs + it.tab + ((it.tile * kTile) >> p.pool.page_bits));
-    sg.template tile<IB ? row_bytes_of<N, IB, RB>() : 0>(p.pool, L, ROW, ring32 + at, ring + at, h, page, it.tile, lane);
-    it.next(p.units, p.seqs);
+    sg.template tile<IB ? row_bytes_of<N, IB, RB>() : 0>(p.pool, L, ROW, ring32 + at, ring + at, h, it.page, it.tile, lane);
+    it.next(p.units, p.seqs, p.tabs, p.pool.page_bits);
   };
   uint32_t at0 = 0u, at1 = L.bytes, at2 = 2 * L.bytes;
   if (n > 0) stage(at0);
@@ -134,18 +134,17 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
         if constexpr (IB != 0) ld.template load_span<FL::KW, FL::LK>(kw[nt], sp + t * ROW, j, true);
         rs[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt);
       }
-      uint32_t kstep = 0u, fk[2] = {0u, 0u}, pk[2] = {0u, 0u};
+      uint32_t kcols = 0u, fk_t = 0u, before = 0u;
       bool wide = false;
       if constexpr (OUTL) {
-        uint32_t fk_t = 0u;
         if (lane < kTile && t0 + lane < s.kv) fk_t = reinterpret_cast<const uint32_t*>(sp + L.flk)[lane];
-        kstep = __reduce_or_sync(0xffffffffu, fk_t);
-        if (kstep) {
-          // Every lane its token's values times qmax / rs in two halves (see paged_decode.cuh).  An entry takes 16 bytes then, so a stage
-          // holds half as many, and they are read before any is written.
-          const uint32_t own = __popc(fk_t), before = counts_before(own, lane);
-          const Entries en = entries_of<false>(p.pool, L, sp);
-          wide = __any_sync(0xffffffffu, own != 0u && before + own > min(en.nk, (uint32_t)kPay / 2)) || __reduce_max_sync(0xffffffffu, own) > 4u;
+        kcols = __reduce_or_sync(0xffffffffu, fk_t);
+        if (kcols) {
+          // Every lane its token's values times qmax / rs in two halves (see paged_decode.cuh).  An entry takes 16 bytes then: all are read
+          // before any is written.
+          const uint32_t own = __popc(fk_t);
+          before = counts_before(own, lane);
+          wide = __any_sync(0xffffffffu, before + own > (lane < 16 ? kPayK : 0xffffu) || own > 4u);
           const float rs_t = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[lane & 15], p.sdt);
           const float inv = rs_t != 0.f ? __fdiv_rn(p.qmaxf, rs_t) : 0.f;
           auto operand = [&](uint2 v) {
@@ -168,20 +167,12 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
             for (int x = 0; x < 4; ++x) if (x < (int)own) d[x] = operand(v[x]);
           } else {
             const int64_t ph = *reinterpret_cast<const int*>(sp + L.off + 16);
-            uint32_t from = en.k0 + before;
+            uint32_t from = *reinterpret_cast<const uint32_t*>(sp + L.off) + before;
             for (uint32_t x = 0; x < own; ++x, ++from)
               my_wide()[before + x] = operand(from < (uint32_t)p.pool.K.out_cap ? __ldg(reinterpret_cast<const uint2*>(p.pool.K.out_vals) + ph * p.pool.K.out_cap + from) : make_uint2(0u, 0u));
           }
           __syncwarp();
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const uint32_t f = __shfl_sync(0xffffffffu, fk_t, nt * 8 + r);
-            fk[nt] = f >> (j * NKS);
-            pk[nt] = 16u * (__shfl_sync(0xffffffffu, before, nt * 8 + r) + __popc(f & ((1u << (j * NKS)) - 1u)));
-          }
         }
-        if constexpr (NKS == 8) { kstep |= kstep >> 16; kstep |= kstep >> 8; kstep &= 0xffu; }
-        else { kstep |= kstep >> 8; kstep |= kstep >> 4; kstep &= 0xfu; }
       }
       // two chains of the high halves' products and one of the low ones': the tensor cores cut a sum's bits with every step
       float sc[NB][4], s2[NB][4], s3[NB][4];
@@ -206,32 +197,44 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
           split(cw.x, a[nt], b[nt]);
           split(cw.y, a[2 + nt], b[2 + nt]);
         });
-        if constexpr (OUTL) {
-          if (kstep & (1u << ks)) {
-            uint4 v[2];
-            if (!wide) {
-#pragma unroll
-              for (int nt = 0; nt < 2; ++nt) v[nt] = *reinterpret_cast<const uint4*>(sp + L.pay + pk[nt]);
-            } else {
-              const unsigned char* far = reinterpret_cast<const unsigned char*>(my_wide());
-#pragma unroll
-              for (int nt = 0; nt < 2; ++nt) v[nt] = __ldcg(reinterpret_cast<const uint4*>(far + pk[nt]));
-            }
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-              const bool f = (fk[nt] & (1u << ks)) != 0u;
-              a[nt] = f ? v[nt].x : a[nt]; a[2 + nt] = f ? v[nt].y : a[2 + nt];
-              b[nt] = f ? v[nt].z : b[nt]; b[2 + nt] = f ? v[nt].w : b[2 + nt];
-              pk[nt] += f ? 16u : 0u;
-            }
-          }
-        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           mma16816((ks & 1) ? s2[nb] : sc[nb], a[0], a[1], a[2], a[3], qb[nb][ks][0], qb[nb][ks][1]);
           mma16816(s3[nb], b[0], b[1], b[2], b[3], qb[nb][ks][0], qb[nb][ks][1]);
         }
       });
+      // flagged chunks: products of their own (see paged_decode.cuh)
+      if constexpr (OUTL) {
+        if (kcols) {
+          uint32_t left = (kcols >> (j * NKS)) & ((1u << NKS) - 1u), f[2], at[2];
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            const uint32_t w_ = __shfl_sync(0xffffffffu, fk_t, nt * 8 + r);
+            f[nt] = w_ >> (j * NKS);
+            at[nt] = __shfl_sync(0xffffffffu, before, nt * 8 + r) + __popc(w_ & ((1u << (j * NKS)) - 1u));
+          }
+          do {
+            const int ks = left ? __ffs(left) - 1 : 0;
+            const bool some = left != 0u;
+            left &= left - 1u;
+            uint32_t a[4], b[4];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+              const bool mine = some && ((f[nt] >> ks) & 1u);
+              const uint4 v = wide ? __ldcg(my_wide() + at[nt]) : reinterpret_cast<const uint4*>(sp + L.pay)[at[nt]];
+              a[nt] = mine ? v.x : 0u; a[2 + nt] = mine ? v.y : 0u;
+              b[nt] = mine ? v.z : 0u; b[2 + nt] = mine ? v.w : 0u;
+              at[nt] += mine ? 1u : 0u;
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              const uint32_t q0 = pick_of<NKS>(qb[nb], 0, ks), q1 = pick_of<NKS>(qb[nb], 1, ks);
+              mma16816(s2[nb], a[0], a[1], a[2], a[3], q0, q1);
+              mma16816(s3[nb], b[0], b[1], b[2], b[3], q0, q1);
+            }
+          } while (__any_sync(0xffffffffu, left != 0u));
+        }
+      }
       float* dst = p.scores + ((int64_t)h * total + f0 + i) * (kTile * R) + r * R + 2 * j;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {

@@ -10,14 +10,14 @@
 namespace hqmq {
 namespace paged {
 
-constexpr int kPay = 96;       // values of flagged chunks staged per tile, of both tensors (of a tile with more, all go through global memory)
+constexpr int kPayK = 64, kPayV = 32;      // values of flagged chunks staged per tile (those of a tile with more go through global memory)
 constexpr int kTileStages = 3;
 
 // Rows of IB + RB bits per chunk; IB = 0: any width, at run time.
 template <int N, int IB, int RB>
 __host__ __device__ constexpr int row_bytes_of() { return (N * (IB + RB) + 31) / 32 * 4; }
 
-// Where the parts of a stage lie.  Values of flagged chunks: K's, then V's (each 8 bytes, or 16 where a value is kept in two halves).
+// Where the parts of a stage lie.  Values of flagged chunks, 8 bytes each: K's, then V's; K's alone have 16, where a value is kept in two halves.
 struct TileLayout { int v, rsk, rsv, flk, flv, off, pay, bytes; };
 __host__ __device__ constexpr TileLayout tile_layout(int row, bool hasv, bool outl) {
   TileLayout l{};
@@ -28,7 +28,7 @@ __host__ __device__ constexpr TileLayout tile_layout(int row, bool hasv, bool ou
   l.flk = at; at += outl ? kTile * 4 : 0;
   l.flv = at; at += outl && hasv ? kTile * 4 : 0;
   l.off = at; at += outl ? 32 : 0;          // K's entries before the tile and behind it; V's; page
-  l.pay = at; at += outl ? kPay * 8 : 0;
+  l.pay = at; at += outl ? (hasv ? kPayK * 8 + kPayV * 8 : kPayK * 16) : 0;
   l.bytes = (at + 15) & ~15;
   return l;
 }
@@ -39,17 +39,19 @@ struct PoolView {
   int Hkv, page_bits;
 };
 
-// The tiles of a warp's stretch, in order.
+// The tiles of a warp's stretch, in order.  The page of a tile is loaded a tile ahead: it is what the copies' addresses wait for.
 struct TileIter {
-  int u, tile, hi, tab, left;
+  int u, tile, hi, tab, left, page;
   __device__ __forceinline__ void unit(const int4* units, const int4* seqs, int skip) {
     const int4 un = __ldg(units + u);
     tile = un.z + skip; hi = un.w;
     tab = __ldg(&seqs[un.x].w);
   }
-  __device__ __forceinline__ void next(const int4* units, const int4* seqs) {
+  __device__ __forceinline__ void find_page(const int* tabs, int page_bits) { page = __ldg(tabs + tab + ((tile * kTile) >> page_bits)); }
+  __device__ __forceinline__ void next(const int4* units, const int4* seqs, const int* tabs, int page_bits) {
     if (--left <= 0) return;
     if (++tile == hi) { ++u; unit(units, seqs, 0); }
+    find_page(tabs, page_bits);
   }
 };
 
@@ -104,30 +106,22 @@ struct Stager {
   }
 };
 
-// The values of a staged tile's flagged chunks, 8 bytes each: K's first, then V's, as many as there is room for (an entry the side
-// buffer had no room for reads as 0).  Ranges: entries before the tile and behind it.
-struct Entries { uint32_t k0, nk, v0, nv; };
-template <bool HASV>
-__device__ __forceinline__ Entries entries_of(const PoolView& p, const TileLayout& l, const unsigned char* sp) {
-  const uint4 o = *reinterpret_cast<const uint4*>(sp + l.off);
-  Entries e;
-  e.k0 = o.x; e.v0 = o.z;
-  e.nk = p.K.flags ? min(o.y - o.x, (uint32_t)kPay) : 0u;
-  e.nv = HASV && p.V.flags ? min(o.w - o.z, (uint32_t)kPay - e.nk) : 0u;
-  return e;
-}
+// The values of a staged tile's flagged chunks, as many as there is room for (an entry the side buffer had no room for reads as 0).  A
+// lane copies up to two of K's and one of V's: no loop.
 template <bool HASV>
 __device__ __forceinline__ void stage_values(const PoolView& p, const TileLayout& l, uint32_t sb, unsigned char* sp, int lane) {
-  const Entries e = entries_of<HASV>(p, l, sp);
-  if (e.nk + e.nv == 0u) return;
+  const uint4 o = *reinterpret_cast<const uint4*>(sp + l.off);       // entries before the tile and behind it: K's, V's
   const int64_t ph = *reinterpret_cast<const int*>(sp + l.off + 16);
-  for (uint32_t i = lane; i < e.nk + e.nv; i += 32) {
-    const bool is_v = HASV && i >= e.nk;
-    const uint32_t at = is_v ? e.v0 + (i - e.nk) : e.k0 + i, cap = is_v ? (uint32_t)p.V.out_cap : (uint32_t)p.K.out_cap;
-    const unsigned char* v = reinterpret_cast<const unsigned char*>(is_v ? p.V.out_vals : p.K.out_vals);
-    if (at < cap) cp_async8(sb + l.pay + 8 * i, v + (ph * cap + at) * 8);
-    else *reinterpret_cast<uint2*>(sp + l.pay + 8 * i) = make_uint2(0u, 0u);
+  auto copy = [&](const hqmq_packed& x, uint32_t at, uint32_t end, int to) {
+    if (at >= end) return;
+    if (at < (uint32_t)x.out_cap) cp_async8(sb + l.pay + to, reinterpret_cast<const unsigned char*>(x.out_vals) + (ph * x.out_cap + at) * 8);
+    else *reinterpret_cast<uint2*>(sp + l.pay + to) = make_uint2(0u, 0u);
+  };
+  if (p.K.flags && o.y != o.x) {
+    copy(p.K, o.x + lane, o.y, 8 * lane);
+    copy(p.K, o.x + 32 + lane, o.y, 256 + 8 * lane);
   }
+  if (HASV && p.V.flags && o.w != o.z) copy(p.V, o.z + lane, o.w, kPayK * 8 + 8 * lane);
 }
 
 __device__ __forceinline__ float4 values_of(uint2 v, int dtype) {
@@ -225,6 +219,19 @@ __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& 
     qb[ks][1] = pack_half2(f[4 * ks + 2] * div, f[4 * ks + 3] * div);
   }
   return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+// Element `k` of an array in registers.
+template <int N>
+__device__ __forceinline__ uint32_t pick_of(const uint32_t (*a)[2], int which, int k) {
+  uint32_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = a[i][which];
+#pragma unroll
+  for (int s = N / 2; s > 0; s >>= 1)
+#pragma unroll
+    for (int i = 0; i < s; ++i) v[i] = k & s ? v[i + s] : v[i];
+  return v[0];
 }
 
 // softcap * tanh(x / softcap) in the exp2 domain, from x * 2 log2(e) / softcap: 1 - 2 / (2^y + 1)
