@@ -55,13 +55,19 @@ PoolView pool_view(const hqmq_paged_attn_args* a) {
   return v;
 }
 
-cudaError_t launch(const void* k, dim3 grid, int threads, void** args, size_t smem, cudaStream_t st, bool dependent) {
+cudaError_t launch(const void* k, dim3 grid, int threads, void** args, size_t smem, cudaStream_t st, bool dependent, int cluster = 1) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
+  if (cluster > 1) {
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cluster; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    dependent = true;
+  } else {
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
-  if (dependent) { cfg.attrs = &at; cfg.numAttrs = 1; }
+  if (dependent) { cfg.attrs = &at; cfg.numAttrs = 1; }          // (never both)
   return cudaLaunchKernelExC(&cfg, k, args);
 }
 
@@ -94,7 +100,7 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   const int4* d = reinterpret_cast<const int4*>(a->plan_data);
   p.hdr = a->plan_data;
   p.seqs = d + pl.seqs / 4; p.units = d + pl.dec_unit / 4; p.cuts = d + pl.dec_cut / 4;
-  p.base = a->plan_data + pl.dec_base; p.wunit = a->plan_data + pl.dec_warp; p.tabs = a->plan_data + pl.tabs;
+  p.base = a->plan_data + pl.dec_base; p.warps = a->plan_data + pl.dec_warp; p.tabs = a->plan_data + pl.tabs;
   p.ctas = pl.dec_ctas;
   p.parts = reinterpret_cast<float*>(ws);
   p.wide = reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(ws) + decode_parts(pl));
@@ -116,8 +122,9 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   const DecodeKernels k = pl.d == 128 ? decode_kernels_128(p.ib, a->K.radius_bits, nb, outl) : decode_kernels_64(p.ib, a->K.radius_bits, nb, outl);
   HQMQ_CHECK_CUDA(raise_smem_limit(k.decode, smem));
   void* args[] = {&p};
-  HQMQ_CHECK_CUDA(launch(k.decode, dim3(p.ctas * pl.H_kv), warps * 32, args, smem, st, false));
-  if (p.ctas > 1) HQMQ_CHECK_CUDA(launch(k.merge, dim3(p.ctas - 1, pl.H_kv, nb * pl.d / 16 * 32 / 64), 64, args, 0, st, true));
+  p.fused = p.ctas > 1 && as_cluster(p.ctas, pl.H_kv);
+  HQMQ_CHECK_CUDA(launch(k.decode, dim3(p.ctas * pl.H_kv), warps * 32, args, smem, st, false, p.fused ? p.ctas : 1));
+  if (p.ctas > 1 && !p.fused) HQMQ_CHECK_CUDA(launch(k.merge, dim3(p.ctas - 1, pl.H_kv, nb * pl.d / 16 * 32 / 64), 64, args, 0, st, true));
   return HQMQ_OK;
 }
 
@@ -187,7 +194,7 @@ extern "C" int hqmq_paged_mass(const hqmq_paged_attn_args* a, void* workspace, s
   const int4* d = reinterpret_cast<const int4*>(a->plan_data);
   p.hdr = a->plan_data;
   p.seqs = d + pl.seqs / 4; p.units = d + pl.ms_unit / 4; p.groups = d + pl.ms_group / 4;
-  p.base = a->plan_data + pl.ms_base; p.wunit = a->plan_data + pl.ms_warp; p.tabs = a->plan_data + pl.tabs;
+  p.base = a->plan_data + pl.ms_base; p.warps = a->plan_data + pl.ms_warp; p.tabs = a->plan_data + pl.tabs;
   p.ctas = pl.ms_ctas;
   p.parts = reinterpret_cast<float2*>(ws + m.parts); p.cta_parts = reinterpret_cast<float2*>(ws + m.cta);
   p.stats = reinterpret_cast<float2*>(ws + m.stats); p.scores = reinterpret_cast<float*>(ws + m.scores);

@@ -52,6 +52,11 @@ constexpr int kMassRowsWide = 32;                    // rows of a unit of the we
 constexpr int kMassGroup = 512;                      // tokens of a CTA of the weights' second kernel
 constexpr int kMaxCodewords = 6144;                   // two tables and the rings of 16 warps in shared memory, whatever the radius bits
 constexpr int kMaxPage = 1024;                       // tokens of a page
+constexpr int kWarpRecord = 8;                       // words of a warp's record: its stretch, first unit and tile, the unit's end, the
+                                                     // sequence's place among the tables, the first tile's page: one load, then the copies
+// CTAs of a head that run as one cluster (148 SMs hold fifteen clusters of eight of these CTAs).
+constexpr int kClusterMax = 8;
+inline bool as_cluster(int ctas, int heads) { return ctas <= kClusterMax && (int64_t)ctas * heads <= 112; }
 inline int dec_warps(int rows) { return rows > 8 ? kDecWarpsWide : kDecWarps; }
 
 int check_plan(const hqmq_paged_plan& p);

@@ -24,8 +24,8 @@ struct DecodeParams {
   float kfac, cap_log2;          // kfac: what a product is multiplied by beside rs (softmax scale * log2 e / qmax, or with a cap 2 log2 e / cap times that)
   float qmaxf, vfac;             // 1 / qmax
   int sdt;
-  const int4* seqs; const int4* units; const int* base; const int* wunit; const int4* cuts; const int* tabs; const int* hdr;
-  int ctas;
+  const int4* seqs; const int4* units; const int* base; const int* warps; const int4* cuts; const int* tabs; const int* hdr;
+  int ctas, fused;               // fused: the CTAs of a head are a cluster
   float* parts;                  // [CTA][warps][2][part], then [CTA][2][part]
   uint2* wide;                   // [CTA][warps][K, V][16 N]: values of a tile with more flagged chunks than a stage holds
 };
@@ -107,19 +107,12 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   const int h = (int)blockIdx.x / p.ctas, k = (int)blockIdx.x - h * p.ctas;
   const int n_units = p.hdr[0], total = p.hdr[1], n_warps = p.ctas * NW;
   const int w = k * NW + warp;
-  const int f0 = stretch_begin(w, total, n_warps), f1 = stretch_begin(w + 1, total, n_warps);
+  TileIter it;                       // the tile to be staged next
+  const int2 range = it.init(p.warps + w * kWarpRecord);
+  const int f0 = range.x, f1 = range.y, n = f1 - f0, u_first = __ldg(p.warps + k * NW * kWarpRecord + 2);
   const int c0 = stretch_begin(k * NW, total, n_warps), c1 = stretch_begin((k + 1) * NW, total, n_warps);
-  if (c0 >= c1) return;
 
   // ---- the first tiles on their way, then the tables -----------------------------------------------------------------------
-  TileIter it;                       // the tile to be staged next
-  int n = f1 - f0;
-  it.left = n;
-  if (n > 0) {
-    it.u = __ldg(p.wunit + w);
-    it.unit(p.units, p.seqs, f0 - __ldg(p.base + it.u));
-    it.find_page(p.tabs, p.pool.page_bits);
-  }
   Stager<true, OUTL> sg;
   sg.init(p.pool, L, lane);
   auto stage = [&](uint32_t at) {    // the tile that `it` is at, to the stage at `at`
@@ -150,7 +143,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   auto my_wide = [&] { return p.wide + ((size_t)blockIdx.x * NW + (threadIdx.x >> 5)) * (32 * N); };     // (hardly ever asked for: not held)
   float* my_parts = p.parts + ((size_t)blockIdx.x * NW + warp) * 2 * PART;
 
-  int u = n > 0 ? __ldg(p.wunit + w) : 0, i = 0;
+  int u = __ldg(p.warps + w * kWarpRecord + 2), i = 0;
   bool first_seg = true;
   while (i < n) {
     // ---- a unit, or what the stretch has of it ------------------------------------------------------------------------------
@@ -482,7 +475,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   // (every warp's first segment left its part in slot 0, a later one that is cut, the stretch's last, in slot 1)
   const float* cta_parts = p.parts + (size_t)blockIdx.x * NW * 2 * PART;
   float* out_parts = p.parts + ((size_t)gridDim.x * NW + blockIdx.x) * 2 * PART;
-  for (int v = __ldg(p.wunit + k * NW); v < n_units; ++v) {
+  for (int v = u_first; c0 < c1 && v < n_units; ++v) {
     const int b0 = __ldg(p.base + v), b1 = __ldg(p.base + v + 1);
     if (b0 >= c1) break;
     const int wa = warp_of(b0, total, n_warps), wb = warp_of(b1 - 1, total, n_warps);
@@ -506,9 +499,24 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       }
     }
   }
+  // ---- units cut between CTAs: where those are a cluster, its CTAs share them out -------------------------------------------------
+  if (p.fused) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    constexpr int PER = NB * NOT * 32;
+    const int n_cuts = p.hdr[5];
+    const float* all = p.parts + ((size_t)gridDim.x * NW + (size_t)h * p.ctas) * 2 * PART;
+    for (int y = k * THREADS + threadIdx.x; y < n_cuts * PER; y += p.ctas * THREADS) {
+      const int4 c = __ldg(p.cuts + y / PER);
+      const int idx = y % PER;
+      auto part_of = [&](int x) { return all + ((size_t)(c.y + x) * 2 + (x == 0 ? c.w : 0)) * PART; };
+      float4 x; float2 m, l;
+      merge_parts<N, NB>(idx, c.z - c.y + 1, part_of, x, m, l);
+      emit_merged<N, NB>(p, seq_of(p, c.x), h, idx, x, m, l);
+    }
+  }
 }
 
-// Units cut between CTAs: blockIdx.x = the cut, blockIdx.y = KV head, blockIdx.z = 64 of the part's quadruples.
+// Units cut between CTAs, where those are no cluster: blockIdx.x = the cut, blockIdx.y = KV head, blockIdx.z = 64 of the part's quadruples.
 template <int N, int NB>
 __global__ void __launch_bounds__(64) paged_merge_kernel(const DecodeParams p) {
   constexpr int NW = NB == 1 ? kDecWarps : kDecWarpsWide, PART = part_floats<N, NB>();

@@ -25,7 +25,7 @@ struct MassParams {
   float kfac, cap, cap_in;       // cap (exp2 domain) * tanh(x * cap_in)
   float qmaxf;
   int sdt;
-  const int4* seqs; const int4* units; const int* base; const int* wunit; const int4* groups; const int* tabs; const int* hdr;
+  const int4* seqs; const int4* units; const int* base; const int* warps; const int4* groups; const int* tabs; const int* hdr;
   int ctas;
   float* scores;                 // [head][tile of the flat sequence][16][rows of a unit]
   float2* parts;                 // [CTA][warps][2][rows]
@@ -56,18 +56,13 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
   const int h = (int)blockIdx.x / p.ctas, k = (int)blockIdx.x - h * p.ctas;
   const int n_units = p.hdr[2], total = p.hdr[3], n_warps = p.ctas * NW;
   const int w = k * NW + warp;
-  const int f0 = stretch_begin(w, total, n_warps), f1 = stretch_begin(w + 1, total, n_warps);
+  TileIter it;                       // the tile to be staged next
+  const int2 range = it.init(p.warps + w * kWarpRecord);
+  const int f0 = range.x, f1 = range.y, n = f1 - f0, u_first = __ldg(p.warps + k * NW * kWarpRecord + 2);
   const int c0 = stretch_begin(k * NW, total, n_warps), c1 = stretch_begin((k + 1) * NW, total, n_warps);
   if (c0 >= c1) return;
 
-  TileIter it;
-  int n = f1 - f0;
-  it.left = n;
-  if (n > 0) {
-    it.u = __ldg(p.wunit + w);
-    it.unit(p.units, p.seqs, f0 - __ldg(p.base + it.u));
-    it.find_page(p.tabs, p.pool.page_bits);
-  }
+  // ---- the first tiles on their way, then the tables -----------------------------------------------------------------------
   Stager<false, OUTL> sg;
   sg.init(p.pool, L, lane);
   auto stage = [&](uint32_t at) {
@@ -92,7 +87,7 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
   auto my_wide = [&] { return p.wide + ((size_t)blockIdx.x * NW + (threadIdx.x >> 5)) * (16 * N); };
   float2* my_parts = p.parts + ((size_t)blockIdx.x * NW + warp) * 2 * R;
 
-  int u = n > 0 ? __ldg(p.wunit + w) : 0, i = 0;
+  int u = __ldg(p.warps + w * kWarpRecord + 2), i = 0;
   bool first_seg = true;
   while (i < n) {
     const int4 un = __ldg(p.units + u), sq4 = __ldg(p.seqs + un.x);
@@ -277,7 +272,7 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
   __syncthreads();
   // units cut between the CTA's warps
   const float2* cta = p.parts + (size_t)blockIdx.x * NW * 2 * R;
-  for (int v = __ldg(p.wunit + k * NW); v < n_units; ++v) {
+  for (int v = u_first; v < n_units; ++v) {
     const int b0 = __ldg(p.base + v), b1 = __ldg(p.base + v + 1);
     if (b0 >= c1) break;
     const int wa = warp_of(b0, total, n_warps), wb = warp_of(b1 - 1, total, n_warps);

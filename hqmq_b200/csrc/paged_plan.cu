@@ -81,10 +81,14 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
   if (total_q > (1 << 30) || n_tab > (1 << 28) || dec_tiles > (1 << 29)) return HQMQ_ERR_SHAPE;
   p.total_q = (int)total_q; p.most_q = all_q; p.n_tab = (int)n_tab;
   p.dec_units = dec_units; p.dec_rows = dec_rows > 8 ? 16 : 8; p.dec_tiles = (int)dec_tiles;
-  // CTAs per head: one per SM in all, no more than leave every warp two tiles
+  // CTAs per head: one per SM in all, no more than leave every warp two tiles; or one, while the CTAs of all heads fit as clusters (whose
+  // parts need no second kernel)
   const int most = std::max(1, HQMQ_PAGED_MAX_CTAS / p.H_kv);
   auto ctas = [&](int64_t tiles, int warps) { return (int)std::max<int64_t>(1, std::min<int64_t>(most, (tiles + 2 * warps - 1) / (2 * warps))); };
-  p.dec_ctas = ctas(dec_tiles, dec_warps(p.dec_rows));
+  const int W_ = dec_warps(p.dec_rows);
+  p.dec_ctas = ctas(dec_tiles, W_);
+  const int single = (int)std::min<int64_t>(1 << 20, (dec_tiles + W_ - 1) / W_);
+  if (single >= 1 && as_cluster(single, p.H_kv)) p.dec_ctas = single;
   // chunks
   p.ch_seqs = ch_seqs;
   const int P = 128 / G;
@@ -159,7 +163,7 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
   take(p.seqs, 4 * (int64_t)p.n_seqs);
   take(p.dec_unit, 4 * (int64_t)p.dec_units);
   take(p.dec_base, (int64_t)p.dec_units + 1);
-  take(p.dec_warp, (int64_t)p.dec_ctas * dec_warps(p.dec_rows) + 1);
+  take(p.dec_warp, kWarpRecord * (int64_t)p.dec_ctas * dec_warps(p.dec_rows));
   take(p.dec_cut, 4 * (int64_t)p.dec_ctas);
   take(p.ch_unit, 8 * ch_units);
   take(p.ch_order, p.ch_whole ? ch_units : 0);
@@ -167,7 +171,7 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
   take(p.ch_img, 4 * (int64_t)ch_seqs);
   take(p.ms_unit, 4 * ms_units);
   take(p.ms_base, ms_units + 1);
-  take(p.ms_warp, (int64_t)p.ms_ctas * kMassWarps + 1);
+  take(p.ms_warp, kWarpRecord * (int64_t)p.ms_ctas * kMassWarps);
   take(p.ms_group, 4 * (int64_t)p.ms_group_room);
   take(p.tabs, p.tab_room ? p.tab_room : n_tab);
   if (at > (1 << 30)) return HQMQ_ERR_SHAPE;
@@ -236,20 +240,25 @@ extern "C" int hqmq_paged_plan_fill(const hqmq_paged_plan* plan, const int32_t* 
       }
     q_off += q; tab += pages;
   }
-  // flat sequences: the unit in which every warp's stretch begins; units cut between CTAs
-  auto stretches = [&](int units, int total, int ctas, int warps, int base_at, int warp_at) {
+  // flat sequences: what every warp's stretch begins with; units cut between CTAs
+  auto stretches = [&](int units, int total, int ctas, int warps, int unit_at, int base_at, int warp_at) {
     const int n = ctas * warps;
     out[base_at + units] = total;
     int u = 0;
-    for (int w = 0; w <= n; ++w) {
-      const int f = stretch_begin(w, total, n);
-      while (u + 1 < units && out[base_at + u + 1] <= f) ++u;
-      out[warp_at + w] = u;
+    for (int w = 0; w < n; ++w) {
+      const int f0 = stretch_begin(w, total, n), f1 = stretch_begin(w + 1, total, n);
+      while (u + 1 < units && out[base_at + u + 1] <= f0) ++u;
+      const int32_t* un = out + unit_at + 4 * u;
+      const int32_t* sq = out + p.seqs + 4 * un[0];
+      const int tile = f0 < total ? un[2] + f0 - out[base_at + u] : un[2];
+      int32_t* r = out + warp_at + kWarpRecord * w;
+      r[0] = f0; r[1] = f1; r[2] = u; r[3] = tile;
+      r[4] = un[3]; r[5] = sq[3]; r[6] = out[p.tabs + sq[3] + tile * 16 / p.page_tokens];
     }
   };
   if (p.dec_units) {
     const int W = dec_warps(p.dec_rows), n = p.dec_ctas * W;
-    stretches(p.dec_units, p.dec_tiles, p.dec_ctas, W, p.dec_base, p.dec_warp);
+    stretches(p.dec_units, p.dec_tiles, p.dec_ctas, W, p.dec_unit, p.dec_base, p.dec_warp);
     int cuts = 0;
     for (int u = 0; u < p.dec_units; ++u) {
       const int b0 = out[p.dec_base + u], b1 = out[p.dec_base + u + 1];
@@ -260,7 +269,7 @@ extern "C" int hqmq_paged_plan_fill(const hqmq_paged_plan* plan, const int32_t* 
     }
     out[5] = cuts;
   }
-  if (p.ms_units) stretches(p.ms_units, p.ms_tiles, p.ms_ctas, kMassWarps, p.ms_base, p.ms_warp);
+  if (p.ms_units) stretches(p.ms_units, p.ms_tiles, p.ms_ctas, kMassWarps, p.ms_unit, p.ms_base, p.ms_warp);
   if (p.ch_units) {
     const int32_t* un = out + p.ch_unit;
     if (p.ch_whole) {

@@ -42,6 +42,12 @@ struct PoolView {
 // The tiles of a warp's stretch, in order.  The page of a tile is loaded a tile ahead: it is what the copies' addresses wait for.
 struct TileIter {
   int u, tile, hi, tab, left, page;
+  // from a warp's record; returns the stretch
+  __device__ __forceinline__ int2 init(const int* record) {
+    const int4 a = __ldg(reinterpret_cast<const int4*>(record)), b = __ldg(reinterpret_cast<const int4*>(record) + 1);
+    u = a.z; tile = a.w; hi = b.x; tab = b.y; page = b.z; left = a.y - a.x;
+    return make_int2(a.x, a.y);
+  }
   __device__ __forceinline__ void unit(const int4* units, const int4* seqs, int skip) {
     const int4 un = __ldg(units + u);
     tile = un.z + skip; hi = un.w;

@@ -16,6 +16,7 @@ All arithmetic runs in the kernels of csrc/paged_*; CPU tensors raise.
 from __future__ import annotations
 
 import ctypes as C
+from threading import get_ident
 from typing import Optional, Sequence
 
 import numpy as np
@@ -34,6 +35,15 @@ class PagePlanes(PackedKV):
         t = getattr(self, name)
         if t is None:
             raise _lib.HqmqError(f"hqmq_b200: these pages have no plane {name!r} (no outliers)")
+        views = self.__dict__.setdefault("_views", {})
+        if name not in views or views[name][0] is not t:
+            views[name] = (t, self._as_pages(t, name))
+        return views[name][1]
+
+    def __getstate__(self):
+        return {k: v for k, v in super().__getstate__().items() if k != "_views"}
+
+    def _as_pages(self, t, name):
         rows = self.B * self.H * self.T_cap
         if name == "codes":
             return t[:rows * self.row_bytes].view(self.B, self.H, self.T_cap, self.row_bytes)
@@ -78,6 +88,9 @@ class PagedKV:
         PackedKV.place(torch.device(device), self.K, self.V)
         self.device = self.K.device
         self.K.T = self.V.T = page_tokens
+        # what the arguments of a call depend on, besides addresses
+        self.kind = (n_pages, page_tokens, n_kv_heads, d_head, S, radius_bits, dtype, self.device, bool(outliers_K), bool(outliers_V),
+                     self.K.out_cap, self.V.out_cap)
 
     def new_mass(self) -> torch.Tensor:
         """Zeroed weights, one per token, page and KV head (see ``paged_attention_mass``)."""
@@ -172,9 +185,16 @@ class PagedBatch:
                    "hqmq_paged_plan_fill")
         return host, kv, q, (table, need, pages)
 
+    def _keep(self, key, call):
+        if len(self._calls) >= 64:
+            self._calls.clear()
+        self._calls[key] = call
+        return call
+
     def _take(self, kv, q, pages):
+        self._calls: dict = {}                   # argument structs of repeated calls
         self.kv_lens, self.q_lens = kv, q
-        self.total_q, self.longest = int(q.sum()), int(kv.max())
+        self.total_q, self.longest, self.shortest = int(q.sum()), int(kv.max()), int(kv.min())
         self._table, self._need, flat = pages
         self.pages = frozenset(flat.tolist())
         self._unshared = len(self.pages) == flat.size
@@ -221,14 +241,14 @@ def _belongs(pool: PagedKV, batch: PagedBatch, what: str):
         raise ValueError(f"{what}: the batch was made for another pool's geometry or device")
 
 
-def _codebook(t: torch.Tensor, pool: PagedKV, what: str) -> torch.Tensor:
+def _codebook(t: torch.Tensor, pool: PagedKV, what: str) -> None:
     if t.shape != (pool.H_kv, 24 * pool.S, 4) or t.dtype != torch.float16 or t.device != pool.device:
         raise ValueError(f"{what}: an fp16 table of shape {(pool.H_kv, 24 * pool.S, 4)} on {pool.device} "
                          f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
-    return t.contiguous()
 
 
 def _attn_args(Q, pool, batch, table_K, softmax_scale, softcap, sinks, what):
+    """Checks, and the argument struct of a call without its addresses."""
     _lib.require_cuda(Q, what)
     _belongs(pool, batch, what)
     if batch.n_heads is None:
@@ -239,38 +259,32 @@ def _attn_args(Q, pool, batch, table_K, softmax_scale, softcap, sinks, what):
         raise ValueError(f"{what}: Q on {Q.device}, the pool on {pool.device}")
     if Q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"{what}: Q is fp32, fp16 or bf16, not {Q.dtype}")
-    if Q.stride(-1) != 1:
-        Q = Q.contiguous()
     if softcap is not None and not 1e-3 <= softcap <= 1e30:
         raise ValueError(f"softcap={softcap}: a positive number (None: no cap)")
-    if sinks is not None:
-        if sinks.shape != (batch.n_heads,) or sinks.device != pool.device:
-            raise ValueError(f"{what}: sinks are one number per query head on {pool.device}")
-        sinks = sinks.to(torch.float32).contiguous()
-    table_K = _codebook(table_K, pool, what)
+    if sinks is not None and (sinks.shape != (batch.n_heads,) or sinks.device != pool.device):
+        raise ValueError(f"{what}: sinks are one number per query head on {pool.device}")
+    _codebook(table_K, pool, what)
     a = _lib.PagedAttnArgs()
     a.struct_size = C.sizeof(_lib.PagedAttnArgs)
-    a.q_dtype, a.Q = _lib.dtype_enum(Q.dtype), Q.data_ptr()
+    a.q_dtype = _lib.dtype_enum(Q.dtype)
     a.q_stride[0], a.q_stride[1] = Q.stride(0), Q.stride(1)
     a.r_qmax = pool.K.qmax
     a.softmax_scale = pool.d_head ** -0.5 if softmax_scale is None else float(softmax_scale)
     a.softcap = 0.0 if softcap is None else float(softcap)
-    if sinks is not None:
-        a.sinks = sinks.data_ptr()
-    a.K, a.V = pool.K.c_struct(), pool.V.c_struct()
-    a.table_K = table_K.data_ptr()
-    a.plan, a.plan_data = batch.plan, batch.data.data_ptr()
-    return a, (Q, sinks, table_K)
+    return a
 
 
-def _call(a, size_fn, fn, device, what):
-    with _lib.device_guard(device):
+def _sized(a, pool, batch, size_fn, fn, Q, tables, sinks, what):
+    """The workspace of a call with these arguments (addresses as they are: some are checked)."""
+    a.K, a.V, a.plan, a.plan_data = pool.K.c_struct(), pool.V.c_struct(), batch.plan, batch.data.data_ptr()
+    a.Q, a.table_K = Q.data_ptr(), tables[0].data_ptr()
+    if len(tables) > 1:
+        a.table_V = tables[1].data_ptr()
+    with _lib.device_guard(pool.device):
         nbytes = size_fn(C.byref(a))
-        # (0: the arguments are refused; the call says why)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        rc = fn(C.byref(a), ws.data_ptr() if nbytes else None, nbytes, _lib.stream_ptr())
-        if rc:
-            _lib.check(rc, what)
+        if not nbytes:                           # the arguments are refused: the call says why
+            _lib.check(fn(C.byref(a), None, 0, _lib.stream_ptr()), what)
+    return nbytes
 
 
 def paged_attention(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, table_K: torch.Tensor, table_V: torch.Tensor,
@@ -283,19 +297,40 @@ def paged_attention(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, table_K: 
 
     Sequences with few rows (new tokens times heads per KV head up to 16) are read in place; the pages of prompt chunks are decoded
     once per call into operand tiles for the tensor cores, half a gigabyte at a time."""
-    a, keep = _attn_args(Q, pool, batch, table_K, softmax_scale, softcap, sinks, "paged_attention")
-    table_V = _codebook(table_V, pool, "paged_attention")
+    if Q.stride(-1) != 1:
+        Q = Q.contiguous()
+    if sinks is not None:
+        sinks = sinks.to(torch.float32).contiguous()
+    table_K, table_V = table_K.contiguous(), table_V.contiguous()
     O = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device) if out is None else out
-    if O.shape != Q.shape or O.device != Q.device:
-        raise ValueError(f"paged_attention: out is {tuple(Q.shape)} on {Q.device}")
-    if batch.total_q == 0:
-        return O
-    if O.stride(-1) != 1:
-        raise _lib.HqmqError("hqmq_b200: the output tensor needs unit stride on the last dim")
-    a.o_dtype, a.O, a.table_V = _lib.dtype_enum(O.dtype), O.data_ptr(), table_V.data_ptr()
-    a.o_stride[0], a.o_stride[1] = O.stride(0), O.stride(1)
+    # (a batch serves call after call, layer after layer: the struct of a call that differs in addresses only is kept with it, per thread)
+    key = ("attn", get_ident(), pool.kind, Q.shape, Q.stride(), Q.dtype, Q.device, O.shape, O.stride(), O.dtype, O.device, table_K.shape,
+           table_K.dtype, table_K.device, table_V.shape, table_V.dtype, table_V.device, softmax_scale, softcap,
+           None if sinks is None else (sinks.shape, sinks.device))
     L = _lib.lib()
-    _call(a, L.hqmq_paged_attn_workspace_bytes, L.hqmq_paged_attn, pool.device, "hqmq_paged_attn")
+    hit = batch._calls.get(key)
+    if hit is None:
+        a = _attn_args(Q, pool, batch, table_K, softmax_scale, softcap, sinks, "paged_attention")
+        _codebook(table_V, pool, "paged_attention")
+        if O.shape != Q.shape or O.device != Q.device:
+            raise ValueError(f"paged_attention: out is {tuple(Q.shape)} on {Q.device}")
+        if batch.total_q == 0:
+            return O
+        if O.stride(-1) != 1:
+            raise _lib.HqmqError("hqmq_b200: the output tensor needs unit stride on the last dim")
+        a.o_dtype, a.O = _lib.dtype_enum(O.dtype), O.data_ptr()
+        a.o_stride[0], a.o_stride[1] = O.stride(0), O.stride(1)
+        nbytes = _sized(a, pool, batch, L.hqmq_paged_attn_workspace_bytes, L.hqmq_paged_attn, Q, (table_K, table_V), sinks, "hqmq_paged_attn")
+        hit = batch._keep(key, (a, C.byref(a), nbytes))
+    a, ref, nbytes = hit
+    a.K, a.V = pool.K.c_struct(), pool.V.c_struct()
+    a.Q, a.O, a.table_K, a.table_V = Q.data_ptr(), O.data_ptr(), table_K.data_ptr(), table_V.data_ptr()
+    a.sinks = None if sinks is None else sinks.data_ptr()
+    with _lib.device_guard(pool.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=pool.device)
+        rc = L.hqmq_paged_attn(ref, ws.data_ptr(), nbytes, _lib.stream_ptr())
+        if rc:
+            _lib.check(rc, "hqmq_paged_attn")
     return O
 
 
@@ -313,21 +348,41 @@ def paged_attention_mass(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, tabl
     new zeroed tensor or ``out`` (which may be ``prior``).  Only the batch's tokens are written.  Products are kept to 22 bits and sums
     in fp32, so weights may be compared and accumulated over many steps.  Q is fp16 or bf16; the scores of all queries are held
     in the workspace, so this is for decode steps and for the last tokens of a prompt."""
-    a, keep = _attn_args(Q, pool, batch, table_K, softmax_scale, softcap, sinks, "paged_attention_mass")
-    if Q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"paged_attention_mass: Q is fp16 or bf16, not {Q.dtype}")
-    if batch._unshared is False:
-        raise ValueError("paged_attention_mass: a page of the batch belongs to two sequences, whose weights would be one")
+    if Q.stride(-1) != 1:
+        Q = Q.contiguous()
+    if sinks is not None:
+        sinks = sinks.to(torch.float32).contiguous()
+    table_K = table_K.contiguous()
     for t, what in ((prior, "prior"), (out, "out")):
         if t is not None:
             _check_mass(t, pool, f"paged_attention_mass: {what}")
-    if not -float("inf") < decay < float("inf"):
-        raise ValueError(f"decay={decay}")
+    key = ("mass", get_ident(), pool.kind, Q.shape, Q.stride(), Q.dtype, Q.device, table_K.shape, table_K.dtype, table_K.device, softmax_scale,
+           softcap, decay, None if sinks is None else (sinks.shape, sinks.device))
+    L = _lib.lib()
+    hit = batch._calls.get(key)
+    if hit is None:
+        a = _attn_args(Q, pool, batch, table_K, softmax_scale, softcap, sinks, "paged_attention_mass")
+        if Q.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"paged_attention_mass: Q is fp16 or bf16, not {Q.dtype}")
+        if not -float("inf") < decay < float("inf"):
+            raise ValueError(f"decay={decay}")
+        a.decay, a.mass = float(decay), pool.K.c_struct().rs         # (any address: it is set below)
+        nbytes = _sized(a, pool, batch, L.hqmq_paged_mass_workspace_bytes, L.hqmq_paged_mass, Q, (table_K,), sinks, "hqmq_paged_mass")
+        hit = batch._keep(key, (a, C.byref(a), nbytes))
+    if batch._unshared is False:
+        raise ValueError("paged_attention_mass: a page of the batch belongs to two sequences, whose weights would be one")
     if out is None:
         out = pool.new_mass()
-    a.prior, a.mass, a.decay = (None if prior is None else prior.data_ptr()), out.data_ptr(), float(decay)
-    L = _lib.lib()
-    _call(a, L.hqmq_paged_mass_workspace_bytes, L.hqmq_paged_mass, pool.device, "hqmq_paged_mass")
+    a, ref, nbytes = hit
+    a.K, a.V = pool.K.c_struct(), pool.V.c_struct()
+    a.Q, a.table_K, a.mass = Q.data_ptr(), table_K.data_ptr(), out.data_ptr()
+    a.prior = None if prior is None else prior.data_ptr()
+    a.sinks = None if sinks is None else sinks.data_ptr()
+    with _lib.device_guard(pool.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=pool.device)
+        rc = L.hqmq_paged_mass(ref, ws.data_ptr(), nbytes, _lib.stream_ptr())
+        if rc:
+            _lib.check(rc, "hqmq_paged_mass")
     return out
 
 
@@ -366,11 +421,12 @@ def paged_evict(pool: PagedKV, batch: PagedBatch, target: PagedBatch, mass: torc
         raise ValueError(f"paged_evict: {len(batch.kv_lens)} sequences, and {len(target.kv_lens)} in the target")
     if first < 0 or last < 0:
         raise ValueError("paged_evict: first and last are counts")
-    more = target.kv_lens > batch.kv_lens
-    if more.any():
+    gone = batch.kv_lens - target.kv_lens
+    if gone.min() < 0:
+        more = gone < 0
         raise ValueError(f"paged_evict: sequence {int(more.argmax())} would grow from {int(batch.kv_lens[more][0])} to {int(target.kv_lens[more][0])} tokens")
-    short = (target.kv_lens < batch.kv_lens) & (target.kv_lens < first + last)
-    if short.any():
+    if target.shortest < first + last and ((gone > 0) & (target.kv_lens < first + last)).any():
+        short = (gone > 0) & (target.kv_lens < first + last)
         raise ValueError(f"paged_evict: sequence {int(short.argmax())} keeps {int(target.kv_lens[short][0])} tokens, fewer than the {first} first and {last} last")
     if not target._unshared or not target.pages.isdisjoint(batch.pages):
         raise ValueError("paged_evict: target's pages belong to one sequence each and are none of the batch's")
@@ -382,13 +438,21 @@ def paged_evict(pool: PagedKV, batch: PagedBatch, target: PagedBatch, mass: torc
     kept = torch.empty(n, pool.H_kv, target.longest, dtype=torch.int32, device=pool.device)
     if target.longest == 0:
         return kept
-    a = _lib.PagedEvictArgs()
-    a.struct_size = C.sizeof(_lib.PagedEvictArgs)
-    a.first, a.last, a.kept_stride = int(first), int(last), target.longest
-    a.K, a.V = pool.K.c_struct(), pool.V.c_struct()
+    key = ("evict", get_ident(), pool.kind, first, last, target.longest)
+    hit = batch._calls.get(key)
+    if hit is None:
+        a = _lib.PagedEvictArgs()
+        a.struct_size = C.sizeof(_lib.PagedEvictArgs)
+        a.first, a.last, a.kept_stride = int(first), int(last), target.longest
+        a.longest, a.most_kept = batch.longest, target.longest
+        a.src = batch.plan
+        hit = batch._keep(key, (a, C.byref(a)))
+    a, ref = hit
+    a.K, a.V, a.dst = pool.K.c_struct(), pool.V.c_struct(), target.plan
     a.mass, a.new_mass, a.kept = mass.data_ptr(), out_mass.data_ptr(), kept.data_ptr()
-    a.src, a.dst, a.src_data, a.dst_data = batch.plan, target.plan, batch.data.data_ptr(), target.data.data_ptr()
-    a.longest, a.most_kept = batch.longest, target.longest
+    a.src_data, a.dst_data = batch.data.data_ptr(), target.data.data_ptr()
     with _lib.device_guard(pool.device):
-        _lib.check(_lib.lib().hqmq_paged_evict(C.byref(a), _lib.stream_ptr()), "hqmq_paged_evict")
+        rc = _lib.lib().hqmq_paged_evict(ref, _lib.stream_ptr())
+        if rc:
+            _lib.check(rc, "hqmq_paged_evict")
     return kept

@@ -37,7 +37,7 @@ def stretch(w, total, n):
     return w * total // n if w < n else total
 
 
-def check_flat(words, units, bases, warps, total, ctas, per_cta, want):
+def check_flat(words, units, bases, warps, total, ctas, per_cta, want, tables, page):
     """Units in order with their tile ranges, prefix sums, and the unit that every warp's stretch begins in."""
     got = [tuple(words[units + 4 * i:units + 4 * i + 4].tolist()) for i in range(len(want))]
     assert got == want
@@ -46,9 +46,13 @@ def check_flat(words, units, bases, warps, total, ctas, per_cta, want):
     n = ctas * per_cta
     for w in range(n):
         f = stretch(w, total, n)
+        rec = words[warps + 8 * w:warps + 8 * w + 7].tolist()
+        assert rec[:2] == [f, stretch(w + 1, total, n)]
         if f < total:
-            u = words[warps + w]
-            assert base[u] <= f < base[u + 1]
+            u = rec[2]
+            assert base[u] <= f < base[u + 1] and rec[3:5] == [want[u][2] + f - base[u], want[u][3]]
+            s = want[u][0]
+            assert rec[5] == sum(len(t) for t in tables[:s]) and rec[6] == tables[s][rec[3] * 16 // page]
 
 
 @pytest.mark.parametrize("seed", range(12))
@@ -78,7 +82,7 @@ def test_plan_covers_every_tile_once(seed):
     assert p.dec_units == len(dec) and p.dec_rows == (16 if any(q[s] * G > 8 for s in few) else 8)
     if dec:
         per = DEC_WARPS_WIDE if p.dec_rows > 8 else DEC_WARPS
-        check_flat(w, p.dec_unit, p.dec_base, p.dec_warp, p.dec_tiles, p.dec_ctas, per, dec)
+        check_flat(w, p.dec_unit, p.dec_base, p.dec_warp, p.dec_tiles, p.dec_ctas, per, dec, tables, page)
         # units between CTAs: every cut names its first and last CTA
         base = w[p.dec_base:p.dec_base + len(dec) + 1]
         n = p.dec_ctas * per
@@ -92,7 +96,7 @@ def test_plan_covers_every_tile_once(seed):
     ms = [(s, r, *tiles(*keys_of(kv[s], q[s], G, window, r, min(q[s] * G, r + rows)))) for s in range(B) for r in range(0, q[s] * G, rows)]
     assert p.ms_units == len(ms)
     if ms:
-        check_flat(w, p.ms_unit, p.ms_base, p.ms_warp, p.ms_tiles, p.ms_ctas, MASS_WARPS, ms)
+        check_flat(w, p.ms_unit, p.ms_base, p.ms_warp, p.ms_tiles, p.ms_ctas, MASS_WARPS, ms, tables, page)
     groups = [w[p.ms_group + 4 * i:p.ms_group + 4 * i + 4].tolist() for i in range(p.ms_groups)]
     assert [g[:2] for g in groups] == [[s, t] for s in range(B) for t in range(0, kv[s], GROUP)]
     for s, t, u0, u1 in groups:
