@@ -81,15 +81,16 @@ __global__ void __launch_bounds__(128) paged_store_kernel(const StoreParams p) {
 // A cluster of C CTAs per (sequence, KV head), each with a stretch of the tokens, their weights as ordered integers in shared memory.
 // Radix select of the smallest weight that stays in three steps (11, 11 and 10 bits): a histogram per CTA, summed over the cluster through
 // distributed shared memory by every CTA for itself.  Then every warp counts and writes its own stretch, 32 tokens at a time.
-// Bound: one read of the weights; a few cluster barriers.
-constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
+// Bound: latencies, of the one read of the weights (16 bytes a thread, four in flight: a float at a time, behind its page's number, took
+// 73 us for 8 heads of 131072 tokens) and of four cluster barriers.
+constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
 constexpr int kSelCached = 40960;               // tokens of a CTA whose keys are kept in shared memory (160 KB)
 
 struct EvictParams {
   hqmq_packed K, V;
   const float* mass; float* new_mass; int* kept;
   const int4* src_seqs; const int* src_tabs; const int4* dst_seqs; const int* dst_tabs;
-  int first, last, kept_stride, Hkv, page_bits, per_page, cached;
+  int first, last, kept_stride, Hkv, page_bits, per_page, cached, n_seqs;
 };
 
 __device__ __forceinline__ uint32_t order_key(float f) {      // larger is heavier; no number: 0, below every number
@@ -110,6 +111,14 @@ __device__ __forceinline__ uint32_t peer_u32(const void* at, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ uint2 peer_u64(const void* at, uint32_t rank) {
+  uint32_t a;
+  uint2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(at)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
 __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const EvictParams p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   uint32_t* hist = reinterpret_cast<uint32_t*>(smem_raw);         // [3][2048]
@@ -126,13 +135,20 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
   const int per = ((n + C - 1) / C + 31) & ~31, t0 = min(n, rank * per), t1 = min(n, t0 + per);
   const int mine = t1 - t0;
   for (int i = tid; i < 3 * 2048; i += kSelThreads) hist[i] = 0u;
-  auto key_of = [&](int t) {
+  const float* mass_h = p.mass + ((int64_t)h << p.page_bits);
+  auto quad_of = [&](int t) {                  // the weights of tokens t .. t + 3 (t a multiple of four, so they lie in one page)
     const int page = __ldg(p.src_tabs + tab + (t >> p.page_bits));
-    return order_key(__ldg(p.mass + ((((int64_t)page * p.Hkv + h) << p.page_bits) + (t & ((1 << p.page_bits) - 1)))));
+    return __ldg(reinterpret_cast<const float4*>(mass_h + (((int64_t)page * p.Hkv) << p.page_bits) + (t & ((1 << p.page_bits) - 1))));
   };
-  auto key_at = [&](int i) { return p.cached ? keys[i] : key_of(t0 + i); };
+  auto key_at = [&](int i) {
+    if (p.cached) return keys[i];
+    const float4 v = quad_of((t0 + i) & ~3);
+    const int x = (t0 + i) & 3;
+    return order_key(x == 0 ? v.x : x == 1 ? v.y : x == 2 ? v.z : v.w);
+  };
   auto free_at = [&](int t) { return t >= first && t < n - last; };       // neither a first nor a last token
   __syncthreads();
+  grid_dep_launch();
   const bool all = keep >= n;
   const uint32_t want = (uint32_t)(keep - first - last);                  // of the free ones
   uint32_t prefix = 0u, left = want;
@@ -140,20 +156,34 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
       uint32_t* hp = hist + pass * 2048;
-      for (int i = tid; i < mine; i += kSelThreads) {
-        uint32_t k;
-        if (pass == 0) { k = key_of(t0 + i); if (p.cached) keys[i] = k; }
-        else k = key_at(i);
-        if (free_at(t0 + i) && (pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix)) atomicAdd(hp + ((k >> shift) & (bins - 1)), 1u);
+      auto count = [&](int i, uint32_t k) {
+        if (i < mine && free_at(t0 + i) && (pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix)) atomicAdd(hp + ((k >> shift) & (bins - 1)), 1u);
+      };
+      if (pass == 0 || !p.cached) {
+#pragma unroll 4
+        for (int i = 4 * tid; i < mine; i += 4 * kSelThreads) {
+          const float4 v = quad_of(t0 + i);
+          const uint4 k = make_uint4(order_key(v.x), order_key(v.y), order_key(v.z), order_key(v.w));
+          if (p.cached) *reinterpret_cast<uint4*>(keys + i) = k;
+          count(i, k.x); count(i + 1, k.y); count(i + 2, k.z); count(i + 3, k.w);
+        }
+      } else {
+        for (int i = 4 * tid; i < mine; i += 4 * kSelThreads) {
+          const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+          count(i, k.x); count(i + 1, k.y); count(i + 2, k.z); count(i + 3, k.w);
+        }
       }
       cluster_sync();
-      // bins 4 tid .. 4 tid + 3, summed over the cluster; then how many lie in higher bins
-      uint32_t c[4] = {0u, 0u, 0u, 0u};
-      if (4 * tid < bins)
-        for (int x = 0; x < C; ++x)
+      // bins 2 tid and 2 tid + 1, summed over the cluster; then how many lie in higher bins
+      uint32_t c[2] = {0u, 0u};
+      if (2 * tid < bins) {
+        uint2 v[8];                              // (all on their way before any is added)
 #pragma unroll
-          for (int b = 0; b < 4; ++b) c[b] += peer_u32(hp + 4 * tid + b, x);
-      const uint32_t sum = c[0] + c[1] + c[2] + c[3];
+        for (int x = 0; x < 8; ++x) { v[x] = make_uint2(0u, 0u); if (x < C) v[x] = peer_u64(hp + 2 * tid, x); }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) { c[0] += v[x].x; c[1] += v[x].y; }
+      }
+      const uint32_t sum = c[0] + c[1];
       const uint32_t wt = __reduce_add_sync(0xffffffffu, sum), below = warp_before(sum, lane);
       if (lane == 0) wsum[warp] = wt;
       __syncthreads();
@@ -161,8 +191,8 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
       for (int x = warp + 1; x < kSelWarps; ++x) above += wsum[x];
       // (left is at least 1 where there is a choice; with nothing wanted the highest bin is taken, of which none stays)
 #pragma unroll
-      for (int b = 3; b >= 0; --b) {
-        if (left > 0 ? above < left && above + c[b] >= left : false) { pick[0] = 4 * tid + b; pick[1] = left - above; }
+      for (int b = 1; b >= 0; --b) {
+        if (left > 0 ? above < left && above + c[b] >= left : false) { pick[0] = 2 * tid + b; pick[1] = left - above; }
         above += c[b];
       }
       __syncthreads();
@@ -213,89 +243,133 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
 }
 
 // ---- evict: their rows go to the new pages ----------------------------------------------------------------------------------------------
-// blockIdx.x = (sequence, new page), y = KV head, z = tensor (the keys' CTAs move the weights, too).
-__global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
-  __shared__ int s_page[kMaxPage];
-  __shared__ uint16_t s_row[kMaxPage];
-  __shared__ uint32_t s_at[kMaxPage], s_flag[kMaxPage], s_warp[8];
-  const int sq = blockIdx.x / p.per_page, pi = blockIdx.x - sq * p.per_page, h = blockIdx.y;
+// A warp per 64 tokens of a new page, two per lane; page, KV head and tensor by (blockIdx.x, warp), y, z.  The warps of a page meet once, to
+// know the entries before theirs.  (A CTA of 256 threads per page, with its scans by block, took 4200 instructions a warp for 64 tokens:
+// 67 us for 16 x 2048 tokens of 8 heads.)  Bound: the chain position - page - row - entries, five loads deep, with 32 to 64 warps an SM in it.
+constexpr int kMoveWarps = 8;
+__global__ void __launch_bounds__(512) evict_move_kernel(const EvictParams p) {
+  __shared__ uint32_t s_count[16];
+  __shared__ int64_t s_row[16][64];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pt = 1 << p.page_bits, wpp = pt >> 6, slots = (int)(blockDim.x >> 5) / wpp, slot = warp / wpp, part = warp - slot * wpp;
+  const int item = blockIdx.x * slots + slot, sq = item / p.per_page, pi = item - sq * p.per_page, h = blockIdx.y;
   const hqmq_packed& X = blockIdx.z ? p.V : p.K;
-  const int4 src = __ldg(p.src_seqs + sq), dst = __ldg(p.dst_seqs + sq);
-  const int pt = 1 << p.page_bits, keep = min(dst.x, src.x), n = min(pt, keep - pi * pt);
-  if (n <= 0) return;
-  const int64_t ph = (int64_t)__ldg(p.dst_tabs + dst.w + pi) * p.Hkv + h, drow = ph << p.page_bits;
-  const int* kept = p.kept + ((int64_t)sq * p.Hkv + h) * p.kept_stride + (int64_t)pi * pt;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  auto row_of = [&](int i) { return (((int64_t)s_page[i] * p.Hkv + h) << p.page_bits) + s_row[i]; };
-  for (int i = tid; i < n; i += 256) {
-    const int t = min(max(__ldg(kept + i), 0), src.x - 1);
-    s_page[i] = __ldg(p.src_tabs + src.w + (t >> p.page_bits));
-    s_row[i] = (uint16_t)(t & (pt - 1));
-    const int64_t r = row_of(i);
-    reinterpret_cast<uint16_t*>(X.rs)[drow + i] = __ldg(reinterpret_cast<const uint16_t*>(X.rs) + r);
-    if (blockIdx.z == 0) p.new_mass[drow + i] = p.mass[r];
-    if (X.flags) s_flag[i] = X.flags[r];
+  int keep = 0, n = 0;
+  int4 src = make_int4(0, 0, 0, 0);
+  int64_t ph = 0;
+  if (sq < p.n_seqs) {
+    src = __ldg(p.src_seqs + sq);
+    const int4 dst = __ldg(p.dst_seqs + sq);
+    keep = min(dst.x, src.x);
+    n = max(0, min(64, keep - (pi * pt + part * 64)));
+    if (n > 0) ph = (int64_t)__ldg(p.dst_tabs + dst.w + pi) * p.Hkv + h;
   }
-  __syncthreads();
-  // code rows: 16, 8 or 4 bytes a thread, whole rows side by side
-  auto rows = [&](auto zero) {
+  grid_dep_wait();
+  const int64_t drow = (ph << p.page_bits) + part * 64;
+  const int* kept = p.kept + ((int64_t)sq * p.Hkv + h) * p.kept_stride + (int64_t)pi * pt + part * 64;
+  int t[2];
+  int64_t row[2];
+  uint32_t fl[2] = {0u, 0u};
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int i = lane + 32 * x;
+    t[x] = i < n ? min(max(__ldg(kept + i), 0), src.x - 1) : 0;
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int i = lane + 32 * x;
+    const int page = i < n ? __ldg(p.src_tabs + src.w + (t[x] >> p.page_bits)) : 0;
+    t[x] &= pt - 1;
+    row[x] = (((int64_t)page * p.Hkv + h) << p.page_bits) + t[x];
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int i = lane + 32 * x;
+    if (i < n) {
+      if (X.flags) fl[x] = X.flags[row[x]];
+      reinterpret_cast<uint16_t*>(X.rs)[drow + i] = reinterpret_cast<const uint16_t*>(X.rs)[row[x]];
+      if (blockIdx.z == 0) p.new_mass[drow + i] = p.mass[row[x]];
+    }
+  }
+  // Code rows: the new ones are one stretch of pieces of 16 or 4 bytes, dealt out to the lanes; a piece's row says where it comes from.
+  if (n > 0) { s_row[warp][lane] = row[0]; s_row[warp][lane + 32] = row[1]; }
+  __syncwarp();
+  auto rows = [&](auto zero, int pieces) {
     using T = decltype(zero);
-    const int w = X.row_bytes / (int)sizeof(T);
-    T* d = reinterpret_cast<T*>(X.codes) + drow * w;
+    T* d = reinterpret_cast<T*>(X.codes) + drow * pieces;
     const T* s = reinterpret_cast<const T*>(X.codes);
-    for (int i = tid; i < n * w; i += 256) {
-      const int k = i / w;
-      d[i] = s[row_of(k) * w + (i - k * w)];
+    const uint32_t inv = 65536u / (uint32_t)pieces + 1u;      // i / pieces = i * inv >> 16 for i < 64 * pieces (pieces <= 32)
+    const int all = n * pieces;
+    constexpr int U = 8;                                      // pieces of a lane on their way at a time
+#pragma unroll 1
+    for (int i0 = lane; i0 < all; i0 += 32 * U) {
+      T v[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + 32 * k, q = (int)((uint32_t)i * inv >> 16);
+        if (i < all) v[k] = s[s_row[warp][q] * pieces + (i - q * pieces)];
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (i0 + 32 * k < all) d[i0 + 32 * k] = v[k];
     }
   };
-  if (X.row_bytes % 16 == 0) rows(make_uint4(0u, 0u, 0u, 0u));
-  else rows(0u);
-  if (!X.flags) return;
-  // side buffer: entries before every token
-  uint32_t run = 0u;
-  for (int i0 = 0; i0 < n; i0 += 256) {
-    const int i = i0 + tid;
-    const uint32_t c = i < n ? __popc(s_flag[i]) : 0u, before = warp_before(c, lane);
-    if (lane == 31) s_warp[warp] = before + c;
+  if (X.row_bytes % 16 == 0) rows(make_uint4(0u, 0u, 0u, 0u), X.row_bytes / 16);
+  else rows(0u, X.row_bytes / 4);
+  if (!X.flags) return;                        // (the same for the whole block)
+  // side buffer: entries before every token, of this warp's, then of the page's warps before it
+  const uint32_t c0 = __popc(fl[0]), c1 = __popc(fl[1]), b0 = warp_before(c0, lane), n0 = __shfl_sync(0xffffffffu, b0 + c0, 31);
+  const uint32_t b1 = n0 + warp_before(c1, lane), all = __shfl_sync(0xffffffffu, b1 + c1, 31);
+  uint32_t before = 0u, total = all;
+  if (wpp > 1) {
+    if (lane == 0) s_count[warp] = all;
     __syncthreads();
-    uint32_t base = run, all = 0u;
-    for (int x = 0; x < 8; ++x) { if (x < warp) base += s_warp[x]; all += s_warp[x]; }
-    if (i < n) {
-      s_at[i] = base + before;
-      X.flags[drow + i] = s_flag[i];
-      const uint32_t end = base + before + c;
-      uint32_t* off = X.out_off + ph * (pt / HQMQ_OUT_BLOCK + 1);
-      if (i == 0) off[0] = 0u;
-      if (((i + 1) & (HQMQ_OUT_BLOCK - 1)) == 0 || i == n - 1) off[i / HQMQ_OUT_BLOCK + 1] = end;
-    }
-    run += all;
-    __syncthreads();
+    total = 0u;
+    for (int x = 0; x < wpp; ++x) { const uint32_t y = s_count[slot * wpp + x]; before += x < part ? y : 0u; total += y; }
   }
-  // (blocks behind the last token hold nothing)
-  for (int b = (n + HQMQ_OUT_BLOCK - 1) / HQMQ_OUT_BLOCK + 1 + tid; b <= pt / HQMQ_OUT_BLOCK; b += 256)
-    X.out_off[ph * (pt / HQMQ_OUT_BLOCK + 1) + b] = run;
-  if (tid == 0) X.out_count[ph] = run;
-  // eight lanes per token: its entries' place is the block's offset and the counts of the tokens before it in the block
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const int i = i0 + tid / 8, q = tid & 7;
-    const uint32_t c = i < n ? __popc(s_flag[i]) : 0u;
-    uint32_t prior = 0u;
-    if (c) {
-      const int64_t r = row_of(i);
-      const int in_blk = s_row[i] & (HQMQ_OUT_BLOCK - 1);
-      for (int x = q; x < in_blk; x += 8) prior += __popc(X.flags[r - in_blk + x]);
+  if (sq >= p.n_seqs || pi * pt >= keep) return;
+  if (n == 0 && !(part * 64 > 0)) return;
+  if (n == 0) {                                // blocks of the page behind its last token hold nothing
+    uint32_t* off = reinterpret_cast<uint32_t*>(X.out_off);
+    const int4 dst = __ldg(p.dst_seqs + sq);
+    const int64_t o = ((int64_t)__ldg(p.dst_tabs + dst.w + pi) * p.Hkv + h) * (pt / HQMQ_OUT_BLOCK + 1) + part * 4;
+    if (lane >= 1 && lane <= 4) off[o + lane] = total;
+    return;
+  }
+  uint32_t* off = X.out_off + ph * (pt / HQMQ_OUT_BLOCK + 1) + part * 4;
+  if (part == 0 && lane == 0) { off[0] = 0u; X.out_count[ph] = total; }
+  const uint32_t at[2] = {before + b0, before + b1}, cnt[2] = {c0, c1};
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int i = lane + 32 * x;
+    if (i < n) X.flags[drow + i] = fl[x];
+    // (the counts of lanes behind the last token are zero: whole blocks end where they would)
+    if ((lane & 15) == 15) off[(i >> 4) + 1] = at[x] + cnt[x];
+  }
+  // a token's entries: the block's offset and the counts of the tokens before it in the block say where they are
+  uint32_t from[2] = {0u, 0u};
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (cnt[x]) {
+      const int in_blk = t[x] & (HQMQ_OUT_BLOCK - 1);
+      const uint4* f4 = reinterpret_cast<const uint4*>(X.flags + (row[x] - in_blk));
+      uint32_t c = X.out_off[(row[x] >> p.page_bits) * (pt / HQMQ_OUT_BLOCK + 1) + t[x] / HQMQ_OUT_BLOCK];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint4 f = f4[q];
+        c += (4 * q < in_blk ? __popc(f.x) : 0) + (4 * q + 1 < in_blk ? __popc(f.y) : 0) + (4 * q + 2 < in_blk ? __popc(f.z) : 0) +
+             (4 * q + 3 < in_blk ? __popc(f.w) : 0);
+      }
+      from[x] = c;
     }
-    prior += __shfl_xor_sync(0xffffffffu, prior, 1);
-    prior += __shfl_xor_sync(0xffffffffu, prior, 2);
-    prior += __shfl_xor_sync(0xffffffffu, prior, 4);
-    if (c) {
-      const int64_t sph = (int64_t)s_page[i] * p.Hkv + h;
-      const uint32_t from = X.out_off[sph * (pt / HQMQ_OUT_BLOCK + 1) + s_row[i] / HQMQ_OUT_BLOCK] + prior, to = s_at[i];
-      const uint2* sv = reinterpret_cast<const uint2*>(X.out_vals) + sph * X.out_cap;
-      uint2* dv = reinterpret_cast<uint2*>(X.out_vals) + ph * X.out_cap;
-      for (uint32_t x = q; x < c; x += 8)
-        if (to + x < (uint32_t)X.out_cap) dv[to + x] = from + x < (uint32_t)X.out_cap ? sv[from + x] : make_uint2(0u, 0u);
-    }
+  }
+  const uint2* sv = reinterpret_cast<const uint2*>(X.out_vals);
+  uint2* dv = reinterpret_cast<uint2*>(X.out_vals) + ph * X.out_cap;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int64_t s0 = (row[x] >> p.page_bits) * X.out_cap;
+    for (uint32_t e = 0; e < cnt[x]; ++e)
+      if (at[x] + e < (uint32_t)X.out_cap) dv[at[x] + e] = from[x] + e < (uint32_t)X.out_cap ? sv[s0 + from[x] + e] : make_uint2(0u, 0u);
   }
 }
 
@@ -342,7 +416,7 @@ extern "C" int hqmq_paged_evict(const hqmq_paged_evict_args* a, void* stream) {
   if (s.n_seqs != d.n_seqs || s.n_pages != d.n_pages || s.page_tokens != d.page_tokens || s.H_kv != d.H_kv || s.d != d.d) return HQMQ_ERR_SHAPE;
   if ((rc = check_pool(a->K, s)) != 0 || (rc = check_pool(a->V, s)) != 0) return rc;
   if (!a->mass || !a->new_mass || !a->kept || !a->src_data || !a->dst_data || a->first < 0 || a->last < 0) return HQMQ_ERR_ARG;
-  if (((uintptr_t)a->src_data | (uintptr_t)a->dst_data) & 15) return HQMQ_ERR_ALIGN;
+  if (((uintptr_t)a->src_data | (uintptr_t)a->dst_data | (uintptr_t)a->mass) & 15) return HQMQ_ERR_ALIGN;
   if (a->most_kept < 0 || a->longest < a->most_kept || a->kept_stride < a->most_kept || (int64_t)s.n_seqs * s.H_kv * 8 > 0x7fffffff) return HQMQ_ERR_SHAPE;
   if (a->longest == 0 || a->kept_stride == 0) return HQMQ_OK;
   EvictParams p;
@@ -369,9 +443,13 @@ extern "C" int hqmq_paged_evict(const hqmq_paged_evict_args* a, void* stream) {
   void* args[] = {&p};
   HQMQ_CHECK_CUDA(cudaLaunchKernelExC(&cfg, (const void*)&evict_select_kernel, args));
   if (a->most_kept == 0) return HQMQ_OK;
-  p.per_page = (a->most_kept + s.page_tokens - 1) / s.page_tokens;
-  if ((int64_t)p.per_page * s.n_seqs > 0x7fffffff) return HQMQ_ERR_SHAPE;
-  evict_move_kernel<<<dim3(p.per_page * s.n_seqs, s.H_kv, 2), 256, 0, st>>>(p);
-  HQMQ_LAUNCH_CHECK();
+  p.per_page = (a->most_kept + s.page_tokens - 1) / s.page_tokens; p.n_seqs = s.n_seqs;
+  const int wpp = s.page_tokens / 64, warps = wpp > kMoveWarps ? wpp : kMoveWarps;
+  const int64_t items = (int64_t)p.per_page * s.n_seqs;
+  if (items > 0x7ffffff0) return HQMQ_ERR_SHAPE;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)((items * wpp + warps - 1) / warps), s.H_kv, 2); cfg.blockDim = dim3(warps * 32); cfg.dynamicSmemBytes = 0;
+  HQMQ_CHECK_CUDA(cudaLaunchKernelExC(&cfg, (const void*)&evict_move_kernel, args));
   return HQMQ_OK;
 }

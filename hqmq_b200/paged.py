@@ -335,7 +335,7 @@ def paged_attention(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, table_K: 
 
 
 def _check_mass(t: torch.Tensor, pool: PagedKV, what: str):
-    if t.shape != (pool.n_pages, pool.H_kv, pool.page_tokens) or t.dtype != torch.float32 or t.device != pool.device or not t.is_contiguous():
+    if t.shape != (pool.n_pages, pool.H_kv, pool.page_tokens) or t.dtype != torch.float32 or t.device != pool.device or not t.is_contiguous() or t.data_ptr() & 15:
         raise ValueError(f"{what}: weights are contiguous fp32 {(pool.n_pages, pool.H_kv, pool.page_tokens)} on {pool.device}, "
                          f"as PagedKV.new_mass gives them")
 
