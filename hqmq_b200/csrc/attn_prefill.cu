@@ -208,15 +208,16 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-// tanh for |x| <= 1/2, its series up to x^11 (the next term is under 4.4e-7), and anywhere: 1 - 2 / (e^2x + 1)
+// tanh(x) for |x| <= 1 as x times a polynomial in x^2 through its values at the six Chebyshev nodes of [0, 1]: within 4.5e-7.  Anywhere:
+// 1 - 2 / (e^2x + 1).
 __device__ __forceinline__ float2 cap_near(float2 x) {
-  const float2 q = mul2(x, x);
   auto c = [](float v) { return make_float2(v, v); };
-  float2 y = fma2(q, c(-1382.f / 155925.f), c(62.f / 2835.f));
-  y = fma2(q, y, c(-17.f / 315.f));
-  y = fma2(q, y, c(2.f / 15.f));
-  y = fma2(q, y, c(-1.f / 3.f));
-  return fma2(mul2(q, y), x, x);
+  const float2 q = mul2(x, x);
+  float2 y = fma2(q, c(-0.00305822911f), c(0.0167208556f));
+  y = fma2(q, y, c(-0.0515859872f));
+  y = fma2(q, y, c(0.13280721f));
+  y = fma2(q, y, c(-0.333289504f));
+  return mul2(x, fma2(q, y, c(0.999999404f)));
 }
 __device__ __forceinline__ float cap_exp(float x) { return 1.f - __fdividef(2.f, fast_exp2(2.885390081777927f * x) + 1.f); }
 // A row's sum with its head's sink (m: the row's maximum, exp2 domain); infinite where the sink is beyond all scores.
@@ -608,16 +609,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
               mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1])));
           float mc = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kmul;
           if constexpr (MODE == 2) {
-            // The scores become tanh(score / cap), in place.  The series holds up to half the cap; a tile of a warp with a larger score, or a
-            // masked one, goes through exp2.  (Either way the exponentials that follow take them as they took scores: with the cap inside that
-            // code, twice over, 1 x 16k, 2048 queries took 2108 us.)
+            // The scores become tanh(score / cap), in place.  The polynomial holds up to the cap; a tile of a warp with a larger score, or a
+            // masked one, goes through exp2 (1322 us for all tiles of the case below, 782 with a polynomial up to half the cap for all).  (Either way the exponentials that follow take them as they took scores: with the cap inside that
+            // code, twice over, 1 x 16k, 2048 queries took 2108 us; the polynomial alone inside it spills, 4200.)
             float mn[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
 #pragma unroll
             for (int c = 0; c < 128; c += 8)
 #pragma unroll
               for (int e = 0; e < 4; ++e) mn[e] = fminf(mn[e], fminf(__uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1])));
             const float lo = fminf(fminf(mn[0], mn[1]), fminf(mn[2], mn[3])) * kmul;
-            if (__all_sync(0xffffffffu, fmaxf(mc, -lo) * p.cap_in <= 0.5f)) {
+            if (__all_sync(0xffffffffu, fmaxf(mc, -lo) * p.cap_in <= 1.f)) {
 #pragma unroll
               for (int c = 0; c < 128; c += 2) {
                 const float2 y = cap_near(mul2(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), cap2));
