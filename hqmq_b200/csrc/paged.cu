@@ -12,7 +12,6 @@ namespace paged {
 namespace {
 
 constexpr size_t kSmemMax = 232448;          // 227 KB
-constexpr size_t kPastPay = 16;              // (a lane without a flagged chunk reads the place behind a stage's last value)
 constexpr float kLog2e = 1.4426950408889634f;
 
 int log2_of(int x) { int b = 0; while ((1 << b) < x) ++b; return b; }
@@ -72,7 +71,7 @@ cudaError_t launch(const void* k, dim3 grid, int threads, void** args, size_t sm
 }
 
 size_t part_bytes(const hqmq_paged_plan& p) {
-  const int nb = p.dec_rows > 8 ? 2 : 1;
+  const int nb = p.dec_rows / 8;
   return (size_t)nb * (p.d / 16 * 128 + 16) * 4;
 }
 size_t decode_parts(const hqmq_paged_plan& p) { return up256((size_t)p.dec_ctas * p.H_kv * (dec_warps(p.dec_rows) + 1) * 2 * part_bytes(p)); }
@@ -105,8 +104,8 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   p.parts = reinterpret_cast<float*>(ws);
   p.wide = reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(ws) + decode_parts(pl));
   const bool outl = a->K.flags || a->V.flags;
-  const int nb = pl.dec_rows > 8 ? 2 : 1, warps = dec_warps(pl.dec_rows);
-  const size_t rings = (size_t)warps * kTileStages * tile_layout(p.row_bytes, true, outl).bytes + kPastPay, table = (size_t)(p.table_rows >> 1) * 8;
+  const int nb = pl.dec_rows / 8, warps = dec_warps(pl.dec_rows);
+  const size_t rings = (size_t)warps * kTileStages * tile_layout(p.row_bytes, true, outl).bytes + kPastPay + (nb > 2 ? (size_t)warps * nb * pl.d * 16 : 0), table = (size_t)(p.table_rows >> 1) * 8;
   // (a field that no encoder writes may index up to 2^ib / 2 entries: what that reaches lies in the block's shared memory, too)
   const size_t any = (size_t)4 << p.ib;
   auto need = [&](int rk, int rv) { return std::max(rings + (table << rk) + (table << rv), std::max(any << rk, (table << rk) + (any << rv))); };
@@ -205,7 +204,7 @@ extern "C" int hqmq_paged_mass(const hqmq_paged_attn_args* a, void* workspace, s
   const int nb = pl.ms_rows / 8;
   void* args[] = {&p};
   if (pl.ms_units) {
-    const size_t rings = (size_t)kMassWarps * kTileStages * tile_layout(p.row_bytes, false, outl).bytes + kPastPay, table = (size_t)(p.table_rows >> 1) * 8;
+    const size_t rings = (size_t)kMassWarps * kTileStages * tile_layout(p.row_bytes, false, outl).bytes + kPastPay + (nb > 1 ? (size_t)kMassWarps * nb * pl.d * 16 : 0), table = (size_t)(p.table_rows >> 1) * 8;
     auto need = [&](int rk) { return std::max(rings + (table << rk), ((size_t)4 << p.ib) << rk); };
     if (need(0) > kSmemMax) return HQMQ_ERR_UNSUPPORTED;
     while (p.repk < 4 && need(p.repk + 1) <= kSmemMax) ++p.repk;

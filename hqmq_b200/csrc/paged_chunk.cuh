@@ -22,7 +22,8 @@ struct PagedExpandParams {
 
 // grid (stretches of the image tiles, heads of the group, 2), as prefill_expand_kernel: eight warps, a warp the 16 tokens of a block of
 // a tile.  A 128-token tile lies in one page or two neighbouring entries of the table; a block lies in one.
-template <int N>
+// IB, RB: index and radius bits of a field (0: any, at run time).
+template <int N, int IB, int RB>
 __global__ void __launch_bounds__(256, 4) paged_expand_kernel(const PagedExpandParams e) {
   constexpr uint32_t TB = (uint32_t)pf_tile_bytes(4 * N);
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -50,8 +51,9 @@ __global__ void __launch_bounds__(256, 4) paged_expand_kernel(const PagedExpandP
   const bool outl = pk.flags != nullptr;
   constexpr int TPW = 32 / N, NF = 16 / TPW;
   const int half = N == 32 ? 0 : lane >> 4, c = N == 32 ? lane : lane & 15;
-  const int cb = e.ib + pk.radius_bits, bit = c * cb, row_words = pk.row_bytes >> 2, sh = bit & 31, w0 = bit >> 5, w1 = sh + cb > 32 ? 1 : 0;
-  const uint32_t imask = (1u << e.ib) - 1u, fmask = (1u << cb) - 1u;
+  const int ib = IB ? IB : e.ib, cb = IB ? IB + RB : e.ib + pk.radius_bits, row_words = IB ? (N * (IB + RB) + 31) / 32 : pk.row_bytes >> 2;
+  const int bit = c * cb, sh = bit & 31, w0 = bit >> 5, w1 = sh + cb > 32 ? 1 : 0;
+  const uint32_t imask = (1u << ib) - 1u, fmask = (1u << cb) - 1u;
   const uint32_t* codes = reinterpret_cast<const uint32_t*>(pk.codes) + w0;
   const uint32_t last_row = (uint32_t)e.table_rows - 1u;      // (a field that no encoder writes reads the last codeword)
   const int pt_mask = (1 << e.page_bits) - 1;
@@ -73,13 +75,13 @@ __global__ void __launch_bounds__(256, 4) paged_expand_kernel(const PagedExpandP
       if (outl) myflag = __ldg(pk.flags + row + lane);
     }
     if (outl) run = __ldg(pk.out_off + ph * ((pt_mask + 1) / HQMQ_OUT_BLOCK + 1) + (tb & pt_mask) / HQMQ_OUT_BLOCK);
+    const uint32_t* r0 = codes + (row + half) * row_words;
 #pragma unroll
     for (int k = 0; k < NF; ++k) {
-      const int t = k * TPW + half;
-      if (tb + t < kv) {
-        const uint32_t* r = codes + (row + t) * row_words;
-        const uint32_t raw = __funnelshift_r(__ldg(r), __ldg(r + w1), sh) & fmask;
-        f[k] = (raw & imask) | ((raw >> e.ib) << 16);
+      if (tb + k * TPW + half < kv) {
+        const uint32_t* r = r0 + k * TPW * row_words;
+        if constexpr (IB + RB == 16) f[k] = __ldg(r) >> sh;          // (two fields a word: none straddles)
+        else f[k] = __funnelshift_r(__ldg(r), __ldg(r + w1), sh);
       }
     }
   };
@@ -95,6 +97,7 @@ __global__ void __launch_bounds__(256, 4) paged_expand_kernel(const PagedExpandP
       fetch(first + i - img0);
       float big = 0.f;
       const int t_first = first * kPfTok, t_end = min(kv, (first + tiles) * kPfTok);
+#pragma unroll 4
       for (int t = t_first + threadIdx.x * 8; t < t_end; t += 256 * 8) {
         const int64_t row = (((int64_t)__ldg(e.tabs + tab + (t >> e.page_bits)) * e.Hkv + h) << e.page_bits) + (t & pt_mask);
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(pk.rs) + row));
@@ -148,8 +151,8 @@ __global__ void __launch_bounds__(256, 4) paged_expand_kernel(const PagedExpandP
 #pragma unroll
     for (int k = 0; k < NF; ++k) {
       const int tl = warp * 16 + k * TPW + half;
-      const float fac = __shfl_sync(0xffffffffu, myfac, k * TPW + half) * (float)(f[k] >> 16);
-      const uint2 cw = tbl[min(f[k] & 0xffffu, last_row)];
+      const float fac = __shfl_sync(0xffffffffu, myfac, k * TPW + half) * (float)((f[k] & fmask) >> ib);
+      const uint2 cw = tbl[min(f[k] & imask, last_row)];
       const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&cw.x)), d = __half22float2(*reinterpret_cast<const __half2*>(&cw.y));
       *reinterpret_cast<uint2*>(kd + tl * 128 + ((((c & 15) >> 1) ^ (tl & 7)) << 4)) = make_uint2(pack_half2(a.x * fac, a.y * fac), pack_half2(d.x * fac, d.y * fac));
     }
@@ -167,6 +170,14 @@ __global__ void __launch_bounds__(256, 4) paged_expand_kernel(const PagedExpandP
       __syncwarp();
     }
   }
+}
+
+template <int N>
+const void* pick_expand(int ib, int rb) {
+  if (ib == 10 && rb == 3) return (const void*)&paged_expand_kernel<N, 10, 3>;
+  if (ib == 12 && rb == 4) return (const void*)&paged_expand_kernel<N, 12, 4>;
+  if (ib == 13 && rb == 6) return (const void*)&paged_expand_kernel<N, 13, 6>;
+  return (const void*)&paged_expand_kernel<N, 0, 0>;
 }
 
 struct ChunkPlaces { size_t mul, img, part, bytes; };
@@ -226,7 +237,7 @@ int chunk_launch(const hqmq_paged_attn_args* a, void* workspace, cudaStream_t st
   e.kimg = ws + at.img; e.vimg = e.kimg + (size_t)pl.ch_heads * pl.ch_img_tiles * pf_tile_bytes(pl.d);
   p.kimg = e.kimg; p.vimg = e.vimg;
   const bool cap = a->softcap > 0.f, wide = pl.d == 128;
-  const void* ek = wide ? (const void*)&paged_expand_kernel<32> : (const void*)&paged_expand_kernel<16>;
+  const void* ek = wide ? pick_expand<32>(e.ib, a->K.radius_bits) : pick_expand<16>(e.ib, a->K.radius_bits);
   const void* ak = wide ? (cap ? (const void*)&prefill_attn_kernel<128, 2> : (const void*)&prefill_attn_kernel<128, 1>)
                         : (cap ? (const void*)&prefill_attn_kernel<64, 2> : (const void*)&prefill_attn_kernel<64, 1>);
   const void* mk = wide ? (const void*)&prefill_merge_kernel<128, 1> : (const void*)&prefill_merge_kernel<64, 1>;

@@ -103,6 +103,9 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 3, r = lane >> 2;
   unsigned char* ring = tblV + (size_t)(p.table_rows >> 1) * strideV + (size_t)warp * kTileStages * L.bytes;
   const uint32_t ring32 = smem_u32(ring);
+  // (of 32 rows, a warp's queries are 8 KB in shared memory, as the fragments that a lane reads: registers hold the accumulators)
+  constexpr bool QREG = NB <= 2;
+  uint2* q_s = reinterpret_cast<uint2*>(tblV + (size_t)(p.table_rows >> 1) * strideV + (size_t)NW * kTileStages * L.bytes + kPastPay) + warp * (NKS * NB * 32);
   grid_dep_launch();
   const int h = (int)blockIdx.x / p.ctas, k = (int)blockIdx.x - h * p.ctas;
   const int n_units = p.hdr[0], total = p.hdr[1], n_warps = p.ctas * NW;
@@ -151,10 +154,16 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
     const Seq s{sq4.x, sq4.y, sq4.z, sq4.w};
     const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
     const int rows = s.q * p.q.G;
-    uint32_t qb[NB][NKS][2];
+    uint32_t qb[QREG ? NB : 1][NKS][2];
     float qmul[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) qmul[nb] = load_query<NKS, true>(qb[nb], p.q, s.q_off, h, nb * 8 + r, rows, j) * kfac;
+    for (int nb = 0; nb < NB; ++nb) {
+      qmul[nb] = load_query<NKS, true>(qb[QREG ? nb : 0], p.q, s.q_off, h, nb * 8 + r, rows, j) * kfac;
+      if constexpr (!QREG) {
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) q_s[(ks * NB + nb) * 32 + lane] = make_uint2(qb[0][ks][0], qb[0][ks][1]);
+      }
+    }
     const int p_first = s.kv - s.q, edge_lo = p.window > 0 ? s.kv - p.window : 0;    // (the last query sees nothing before edge_lo)
     float m_run[NB][2], l_run[NB][2], o[NB][NOT][4];
 #pragma unroll
@@ -259,7 +268,12 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
           a[2 + nt] = hmul2_u32(cw.y, rr);
         });
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma16816((ks & 1) ? s2[nb] : sc[nb], a[0], a[1], a[2], a[3], qb[nb][ks][0], qb[nb][ks][1]);
+        for (int nb = 0; nb < NB; ++nb) {
+          uint2 q;
+          if constexpr (QREG) q = make_uint2(qb[nb][ks][0], qb[nb][ks][1]);
+          else q = q_s[(ks * NB + nb) * 32 + lane];
+          mma16816((ks & 1) ? s2[nb] : sc[nb], a[0], a[1], a[2], a[3], q.x, q.y);
+        }
       });
 
       // Flagged chunks of K: the four groups of lanes that share a j take a column of theirs each, one more product.  (Put into the
@@ -288,8 +302,12 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
               at[nt] += mine ? 1u : 0u;
             }
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-              mma16816(s2[nb], a[0], a[1], a[2], a[3], pick_of<NKS>(qb[nb], 0, ks), pick_of<NKS>(qb[nb], 1, ks));
+            for (int nb = 0; nb < NB; ++nb) {
+              uint2 q;
+              if constexpr (QREG) q = make_uint2(pick_of<NKS>(qb[nb], 0, ks), pick_of<NKS>(qb[nb], 1, ks));
+              else q = q_s[(ks * NB + nb) * 32 + lane];
+              mma16816(s2[nb], a[0], a[1], a[2], a[3], q.x, q.y);
+            }
           } while (__any_sync(0xffffffffu, left != 0u));
         }
       }
@@ -549,6 +567,7 @@ const void* pick_decode(int ib, int rb) {
 template <int N>
 DecodeKernels pick_kernels(int ib, int rb, int nb, bool outl) {
   if (nb == 1) return {outl ? pick_decode<N, 1, true>(ib, rb) : pick_decode<N, 1, false>(ib, rb), (const void*)&paged_merge_kernel<N, 1>};
+  if (nb == 4) return {outl ? pick_decode<N, 4, true>(ib, rb) : pick_decode<N, 4, false>(ib, rb), (const void*)&paged_merge_kernel<N, 4>};
   return {outl ? pick_decode<N, 2, true>(ib, rb) : pick_decode<N, 2, false>(ib, rb), (const void*)&paged_merge_kernel<N, 2>};
 }
 

@@ -52,6 +52,8 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 3, r = lane >> 2;
   unsigned char* ring = tblK + (size_t)(p.table_rows >> 1) * strideK + (size_t)warp * kTileStages * L.bytes;
   const uint32_t ring32 = smem_u32(ring);
+  constexpr bool QREG = NB == 1;               // (queries in registers, or in shared memory as in paged_decode.cuh)
+  uint2* q_s = reinterpret_cast<uint2*>(tblK + (size_t)(p.table_rows >> 1) * strideK + (size_t)NW * kTileStages * L.bytes + kPastPay) + warp * (NKS * NB * 32);
   grid_dep_launch();
   const int h = (int)blockIdx.x / p.ctas, k = (int)blockIdx.x - h * p.ctas;
   const int n_units = p.hdr[2], total = p.hdr[3], n_warps = p.ctas * NW;
@@ -94,11 +96,15 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
     const Seq s{sq4.x, sq4.y, sq4.z, sq4.w};
     const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
     const int rows = s.q * p.q.G, row0 = un.y;
-    uint32_t qb[NB][NKS][2];
+    uint32_t qb[1][NKS][2];
     float qmul[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float mul = load_query<NKS, false>(qb[nb], p.q, s.q_off, h, row0 + nb * 8 + r, rows, j);
+      const float mul = load_query<NKS, false>(qb[0], p.q, s.q_off, h, row0 + nb * 8 + r, rows, j);
+      if constexpr (!QREG) {
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) q_s[(ks * NB + nb) * 32 + lane] = make_uint2(qb[0][ks][0], qb[0][ks][1]);
+      }
       qmul[nb][0] = __shfl_sync(0xffffffffu, mul, 8 * j);
       qmul[nb][1] = __shfl_sync(0xffffffffu, mul, 8 * j + 4);
     }
@@ -194,8 +200,11 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
         });
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          mma16816((ks & 1) ? s2[nb] : sc[nb], a[0], a[1], a[2], a[3], qb[nb][ks][0], qb[nb][ks][1]);
-          mma16816(s3[nb], b[0], b[1], b[2], b[3], qb[nb][ks][0], qb[nb][ks][1]);
+          uint2 q;
+          if constexpr (QREG) q = make_uint2(qb[0][ks][0], qb[0][ks][1]);
+          else q = q_s[(ks * NB + nb) * 32 + lane];
+          mma16816((ks & 1) ? s2[nb] : sc[nb], a[0], a[1], a[2], a[3], q.x, q.y);
+          mma16816(s3[nb], b[0], b[1], b[2], b[3], q.x, q.y);
         }
       });
       // flagged chunks: products of their own (see paged_decode.cuh)
@@ -223,9 +232,11 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-              const uint32_t q0 = pick_of<NKS>(qb[nb], 0, ks), q1 = pick_of<NKS>(qb[nb], 1, ks);
-              mma16816(s2[nb], a[0], a[1], a[2], a[3], q0, q1);
-              mma16816(s3[nb], b[0], b[1], b[2], b[3], q0, q1);
+              uint2 q;
+              if constexpr (QREG) q = make_uint2(pick_of<NKS>(qb[0], 0, ks), pick_of<NKS>(qb[0], 1, ks));
+              else q = q_s[(ks * NB + nb) * 32 + lane];
+              mma16816(s2[nb], a[0], a[1], a[2], a[3], q.x, q.y);
+              mma16816(s3[nb], b[0], b[1], b[2], b[3], q.x, q.y);
             }
           } while (__any_sync(0xffffffffu, left != 0u));
         }

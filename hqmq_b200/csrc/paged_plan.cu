@@ -6,8 +6,8 @@
 namespace hqmq {
 namespace paged {
 
-// Sequences of up to 16 rows take the decode kernel, the others decode their cache once into operand tiles (attn_prefill.cu).
-bool chunked(int q, int G) { return q * G > 16; }
+// Sequences of up to 32 rows take the decode kernel, the others decode their cache once into operand tiles (attn_prefill.cu).
+bool chunked(int q, int G) { return q * G > 32; }
 
 int check_plan(const hqmq_paged_plan& p) {
   if (p.struct_size != sizeof(hqmq_paged_plan)) return HQMQ_ERR_ARG;
@@ -80,7 +80,7 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
   }
   if (total_q > (1 << 30) || n_tab > (1 << 28) || dec_tiles > (1 << 29)) return HQMQ_ERR_SHAPE;
   p.total_q = (int)total_q; p.most_q = all_q; p.n_tab = (int)n_tab;
-  p.dec_units = dec_units; p.dec_rows = dec_rows > 8 ? 16 : 8; p.dec_tiles = (int)dec_tiles;
+  p.dec_units = dec_units; p.dec_rows = dec_rows > 16 ? 32 : dec_rows > 8 ? 16 : 8; p.dec_tiles = (int)dec_tiles;
   // CTAs per head: one per SM in all, no more than leave every warp two tiles; or one, while the CTAs of all heads fit as clusters (whose
   // parts need no second kernel)
   const int most = std::max(1, HQMQ_PAGED_MAX_CTAS / p.H_kv);

@@ -12,6 +12,7 @@ namespace paged {
 
 constexpr int kPayK = 64, kPayV = 32;      // values of flagged chunks staged per tile (those of a tile with more go through global memory)
 constexpr int kTileStages = 3;
+constexpr size_t kPastPay = 16;            // (a lane without a flagged chunk reads the place behind a stage's last value)
 
 // Rows of IB + RB bits per chunk; IB = 0: any width, at run time.
 template <int N, int IB, int RB>

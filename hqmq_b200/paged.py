@@ -295,7 +295,7 @@ def paged_attention(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, table_K: 
     the last ones).  ``softcap``: scores become softcap * tanh(score / softcap).  ``sinks`` (H_q): a logit per head that takes part in the
     softmax and has no value.  ``table_K`` / ``table_V``: the quantizer's fp16 tables, as in ``fused_attention_packed``.
 
-    Sequences with few rows (new tokens times heads per KV head up to 16) are read in place; the pages of prompt chunks are decoded
+    Sequences with few rows (new tokens times heads per KV head up to 32) are read in place; the pages of prompt chunks are decoded
     once per call into operand tiles for the tensor cores, half a gigabyte at a time."""
     if Q.stride(-1) != 1:
         Q = Q.contiguous()

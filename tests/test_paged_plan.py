@@ -77,9 +77,9 @@ def test_plan_covers_every_tile_once(seed):
         assert w[p.tabs + tab:p.tabs + tab + len(tables[s])].tolist() == tables[s]
         at += q[s]
     tiles = lambda lo, hi: (lo // 16, -(-hi // 16))
-    few = [s for s in range(B) if 0 < q[s] * G <= 16]
+    few = [s for s in range(B) if 0 < q[s] * G <= 32]
     dec = [(s, 0, *tiles(*keys_of(kv[s], q[s], G, window, 0, q[s] * G))) for s in few]
-    assert p.dec_units == len(dec) and p.dec_rows == (16 if any(q[s] * G > 8 for s in few) else 8)
+    assert p.dec_units == len(dec) and p.dec_rows == next(r for r in (8, 16, 32) if all(q[s] * G <= r for s in few))
     if dec:
         per = DEC_WARPS_WIDE if p.dec_rows > 8 else DEC_WARPS
         check_flat(w, p.dec_unit, p.dec_base, p.dec_warp, p.dec_tiles, p.dec_ctas, per, dec, tables, page)
@@ -103,7 +103,7 @@ def test_plan_covers_every_tile_once(seed):
         assert [u for u in range(len(ms)) if ms[u][0] == s] == list(range(u0, u1))
     # prompt chunks: units of a sequence in order, images of the tiles that any of them sees, pieces of equal size
     P, units = 128 // G, []
-    chunks = [s for s in range(B) if q[s] * G > 16]
+    chunks = [s for s in range(B) if q[s] * G > 32]
     per = p.ch_streams * P
     img = 0
     for i, s in enumerate(chunks):
