@@ -35,7 +35,8 @@ int check_args(const hqmq_paged_attn_args* a, bool mass) {
     return a->mass ? HQMQ_OK : HQMQ_ERR_ARG;
   }
   if ((rc = check_pool(a->V, p)) != 0) return rc;
-  if (a->V.S != a->K.S || a->V.radius_bits != a->K.radius_bits || a->V.scale_dtype != a->K.scale_dtype) return HQMQ_ERR_UNSUPPORTED;
+  if (a->V.S != a->K.S || a->V.radius_bits != a->K.radius_bits || a->V.scale_dtype != a->K.scale_dtype ||
+      (a->K.flags && a->V.flags && a->K.out_dtype != a->V.out_dtype)) return HQMQ_ERR_UNSUPPORTED;
   if (!a->table_V || (p.total_q > 0 && !a->O)) return HQMQ_ERR_ARG;
   if (!is_float_dtype(a->o_dtype)) return HQMQ_ERR_DTYPE;
   if ((uintptr_t)a->table_V & 7) return HQMQ_ERR_ALIGN;
@@ -92,7 +93,7 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   p.o_vec = is_half_dtype(a->o_dtype) && ((uintptr_t)a->O & 3) == 0 && a->o_stride[0] % 2 == 0 && a->o_stride[1] % 2 == 0;
   p.tblK = a->table_K; p.tblV = a->table_V; p.sinks = a->sinks;
   p.table_rows = 24 * a->K.S; p.ib = idx_bits_for(a->K.S); p.row_bytes = a->K.row_bytes;
-  p.window = pl.window; p.sdt = a->K.scale_dtype;
+  p.window = pl.window; p.sdt = a->K.scale_dtype; p.pay_bf16 = (a->K.flags ? a->K : a->V).out_dtype == HQMQ_BF16;
   p.qmaxf = (float)a->r_qmax; p.vfac = 1.f / (float)a->r_qmax;
   p.kfac = a->softmax_scale * kLog2e / (float)a->r_qmax;
   if (a->softcap > 0.f) { p.cap_log2 = a->softcap * kLog2e; p.kfac *= 2.f / a->softcap; }

@@ -23,7 +23,7 @@ struct DecodeParams {
   int table_rows, ib, row_bytes, repk, repv, window;
   float kfac, cap_log2;          // kfac: what a product is multiplied by beside rs (softmax scale * log2 e / qmax, or with a cap 2 log2 e / cap times that)
   float qmaxf, vfac;             // 1 / qmax
-  int sdt;
+  int sdt, pay_bf16;             // type of the scales; whether the flagged chunks' values are bf16 (else fp16)
   const int4* seqs; const int4* units; const int* base; const int* warps; const int4* cuts; const int* tabs; const int* hdr;
   int ctas, fused;               // fused: the CTAs of a head are a cluster
   float* parts;                  // [CTA][warps][2][part], then [CTA][2][part]
@@ -218,11 +218,8 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
           // every lane its token's values, in place
           const float rs = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[lane], p.sdt);
           const float inv = rs != 0.f ? __fdividef(p.qmaxf, rs) : 0.f;
-          const int dt = lane < 16 ? p.pool.K.out_dtype : p.pool.V.out_dtype;
-          auto operand = [&](uint2 v) {
-            const float4 x = values_of(v, dt);
-            return make_uint2(pack_half2(x.x * inv, x.y * inv), pack_half2(x.z * inv, x.w * inv));
-          };
+          const bool bf = p.pay_bf16 != 0;
+          auto operand = [&](uint2 v) { return make_uint2(scaled_pair(v.x, inv, bf), scaled_pair(v.y, inv, bf)); };
           if (!wide) {
             uint2* e = reinterpret_cast<uint2*>(sp + L.pay + (lane < 16 ? 0 : kPayK * 8)) + before;
             for (uint32_t x = 0; x < own; ++x, ++e) *e = operand(*e);
@@ -276,22 +273,20 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         }
       });
 
-      // Flagged chunks of K: the four groups of lanes that share a j take a column of theirs each, one more product.  (Put into the
-      // fragments above instead, the branches of every step kept the look-ups from being issued ahead: 381 us against 170 without
-      // outliers for 16 x 32k, 287 with that part left out.)
+      // Flagged chunks of K: one more product for every step of the others' that has some.  (Put into the fragments above instead, the
+      // branches of every step kept the look-ups from being issued ahead: 381 us against 170 without outliers for 16 x 32k, 287 with that part
+      // left out.  A column per group of lanes at a time, which takes fewer products, pays where the queries are in shared memory: picked from
+      // registers by selects it took 145 instructions a tile, 339 us against 317; of 32 rows it takes 88 us against 102 for 8 x 8111.)
       if constexpr (OUTL) {
         if (kcols) {
-          uint32_t left = (kcols >> (j * NKS)) & ((1u << NKS) - 1u), f[2], at[2];
+          uint32_t f[2], at[2];
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) {
             const uint32_t w_ = __shfl_sync(0xffffffffu, fl, nt * 8 + r);
             f[nt] = w_ >> (j * NKS);
             at[nt] = __shfl_sync(0xffffffffu, before, nt * 8 + r) + __popc(w_ & ((1u << (j * NKS)) - 1u));
           }
-          do {
-            const int ks = left ? __ffs(left) - 1 : 0;
-            const bool some = left != 0u;
-            left &= left - 1u;
+          auto step = [&](int ks, bool some, auto query) {
             uint2 v[2];
             values_at(v, at, 2, false);
             uint32_t a[4];
@@ -302,13 +297,24 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
               at[nt] += mine ? 1u : 0u;
             }
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              uint2 q;
-              if constexpr (QREG) q = make_uint2(pick_of<NKS>(qb[nb], 0, ks), pick_of<NKS>(qb[nb], 1, ks));
-              else q = q_s[(ks * NB + nb) * 32 + lane];
-              mma16816(s2[nb], a[0], a[1], a[2], a[3], q.x, q.y);
-            }
-          } while (__any_sync(0xffffffffu, left != 0u));
+            for (int nb = 0; nb < NB; ++nb) { const uint2 q = query(nb); mma16816(s2[nb], a[0], a[1], a[2], a[3], q.x, q.y); }
+          };
+          if constexpr (QREG) {
+            uint32_t steps = kcols;
+            if constexpr (NKS == 8) { steps |= steps >> 16; steps |= steps >> 8; } else { steps |= steps >> 8; steps |= steps >> 4; }
+            static_for<0, NKS>([&](auto ks_) {
+              constexpr int ks = decltype(ks_)::value;
+              if (steps & (1u << ks)) step(ks, true, [&](int nb) { return make_uint2(qb[nb][ks][0], qb[nb][ks][1]); });
+            });
+          } else {
+            uint32_t left = (kcols >> (j * NKS)) & ((1u << NKS) - 1u);
+            do {
+              const int ks = left ? __ffs(left) - 1 : 0;
+              const bool some = left != 0u;
+              left &= left - 1u;
+              step(ks, some, [&](int nb) { return q_s[(ks * NB + nb) * 32 + lane]; });
+            } while (__any_sync(0xffffffffu, left != 0u));
+          }
         }
       }
 

@@ -210,17 +210,14 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
       // flagged chunks: products of their own (see paged_decode.cuh)
       if constexpr (OUTL) {
         if (kcols) {
-          uint32_t left = (kcols >> (j * NKS)) & ((1u << NKS) - 1u), f[2], at[2];
+          uint32_t f[2], at[2];
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) {
             const uint32_t w_ = __shfl_sync(0xffffffffu, fk_t, nt * 8 + r);
             f[nt] = w_ >> (j * NKS);
             at[nt] = __shfl_sync(0xffffffffu, before, nt * 8 + r) + __popc(w_ & ((1u << (j * NKS)) - 1u));
           }
-          do {
-            const int ks = left ? __ffs(left) - 1 : 0;
-            const bool some = left != 0u;
-            left &= left - 1u;
+          auto step = [&](int ks, bool some, auto query) {
             uint32_t a[4], b[4];
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
@@ -232,13 +229,27 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-              uint2 q;
-              if constexpr (QREG) q = make_uint2(pick_of<NKS>(qb[0], 0, ks), pick_of<NKS>(qb[0], 1, ks));
-              else q = q_s[(ks * NB + nb) * 32 + lane];
+              const uint2 q = query(nb);
               mma16816(s2[nb], a[0], a[1], a[2], a[3], q.x, q.y);
               mma16816(s3[nb], b[0], b[1], b[2], b[3], q.x, q.y);
             }
-          } while (__any_sync(0xffffffffu, left != 0u));
+          };
+          if constexpr (QREG) {
+            uint32_t steps = kcols;
+            if constexpr (NKS == 8) { steps |= steps >> 16; steps |= steps >> 8; } else { steps |= steps >> 8; steps |= steps >> 4; }
+            static_for<0, NKS>([&](auto ks_) {
+              constexpr int ks = decltype(ks_)::value;
+              if (steps & (1u << ks)) step(ks, true, [&](int) { return make_uint2(qb[0][ks][0], qb[0][ks][1]); });
+            });
+          } else {
+            uint32_t left = (kcols >> (j * NKS)) & ((1u << NKS) - 1u);
+            do {
+              const int ks = left ? __ffs(left) - 1 : 0;
+              const bool some = left != 0u;
+              left &= left - 1u;
+              step(ks, some, [&](int nb) { return q_s[(ks * NB + nb) * 32 + lane]; });
+            } while (__any_sync(0xffffffffu, left != 0u));
+          }
         }
       }
       float* dst = p.scores + ((int64_t)h * total + f0 + i) * (kTile * R) + r * R + 2 * j;

@@ -118,19 +118,28 @@ struct Stager {
 template <bool HASV>
 __device__ __forceinline__ void stage_values(const PoolView& p, const TileLayout& l, uint32_t sb, unsigned char* sp, int lane) {
   const uint4 o = *reinterpret_cast<const uint4*>(sp + l.off);       // entries before the tile and behind it: K's, V's
-  const int64_t ph = *reinterpret_cast<const int*>(sp + l.off + 16);
-  auto copy = [&](const hqmq_packed& x, uint32_t at, uint32_t end, int to) {
-    if (at >= end) return;
-    if (at < (uint32_t)x.out_cap) cp_async8(sb + l.pay + to, reinterpret_cast<const unsigned char*>(x.out_vals) + (ph * x.out_cap + at) * 8);
-    else *reinterpret_cast<uint2*>(sp + l.pay + to) = make_uint2(0u, 0u);
+  const int ph = *reinterpret_cast<const int*>(sp + l.off + 16);
+  auto copy = [&](const hqmq_packed& x, uint32_t from, uint32_t end, int to, bool twice) {
+    const uint32_t at = from + lane, room = min(end, (uint32_t)x.out_cap);
+    const unsigned char* v = reinterpret_cast<const unsigned char*>(x.out_vals) + ((int64_t)ph * x.out_cap + at) * 8;
+    if (at < room) cp_async8(sb + l.pay + to + 8 * lane, v);
+    if (twice && at + 32 < room) cp_async8(sb + l.pay + to + 256 + 8 * lane, v + 256);
+    if (end > (uint32_t)x.out_cap) {           // (hardly ever: a side buffer that overflowed)
+      if (at >= room) *reinterpret_cast<uint2*>(sp + l.pay + to + 8 * lane) = make_uint2(0u, 0u);
+      if (twice && at + 32 >= room) *reinterpret_cast<uint2*>(sp + l.pay + to + 256 + 8 * lane) = make_uint2(0u, 0u);
+    }
   };
-  if (p.K.flags && o.y != o.x) {
-    copy(p.K, o.x + lane, o.y, 8 * lane);
-    copy(p.K, o.x + 32 + lane, o.y, 256 + 8 * lane);
-  }
-  if (HASV && p.V.flags && o.w != o.z) copy(p.V, o.z + lane, o.w, kPayK * 8 + 8 * lane);
+  if (p.K.flags && o.y != o.x) copy(p.K, o.x, o.y, 0, true);
+  if (HASV && p.V.flags && o.w != o.z) copy(p.V, o.z, o.w, kPayK * 8, false);
 }
 
+// Two 16-bit values times f as two fp16 ones.
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t v, float f, bool bf16) {
+  float2 x;
+  if (bf16) x = make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  else x = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return pack_half2(x.x * f, x.y * f);
+}
 __device__ __forceinline__ float4 values_of(uint2 v, int dtype) {
   float2 a, b;
   if (dtype == HQMQ_BF16) {
@@ -226,19 +235,6 @@ __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& 
     qb[ks][1] = pack_half2(f[4 * ks + 2] * div, f[4 * ks + 3] * div);
   }
   return __uint_as_float((uint32_t)(127 + e) << 23);
-}
-
-// Element `k` of an array in registers.
-template <int N>
-__device__ __forceinline__ uint32_t pick_of(const uint32_t (*a)[2], int which, int k) {
-  uint32_t v[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = a[i][which];
-#pragma unroll
-  for (int s = N / 2; s > 0; s >>= 1)
-#pragma unroll
-    for (int i = 0; i < s; ++i) v[i] = k & s ? v[i + s] : v[i];
-  return v[0];
 }
 
 // softcap * tanh(x / softcap) in the exp2 domain, from x * 2 log2(e) / softcap: 1 - 2 / (2^y + 1)
