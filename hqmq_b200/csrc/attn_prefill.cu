@@ -219,7 +219,7 @@ __device__ __forceinline__ float2 cap_near(float2 x) {
   y = fma2(q, y, c(-0.333289504f));
   return mul2(x, fma2(q, y, c(0.999999404f)));
 }
-__device__ __forceinline__ float cap_exp(float x) { return 1.f - __fdividef(2.f, fast_exp2(2.885390081777927f * x) + 1.f); }
+__device__ __forceinline__ float cap_far(float x) { return 1.f - __fdividef(2.f, fast_exp2(2.885390081777927f * x) + 1.f); }
 // A row's sum with its head's sink (m: the row's maximum, exp2 domain); infinite where the sink is beyond all scores.
 __device__ __forceinline__ float with_sink(const PrefillParams& p, int head, float m, float l) {
   if (m == -INFINITY) return l;
@@ -407,6 +407,88 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
     constexpr int QL = D / 8, QR = 32 / QL;      // lanes per row, rows per warp-wide load
     const int c_q = lane % QL;
     const uint32_t g_inv = 65536u / (uint32_t)p.G + 1u;                   // rw / G = rw * g_inv >> 16 for rw < 128
+    // Ragged batches: queries of any size, relative to a power of two per warp (which owns the rows it loads); returns that power.  Two
+    // passes, the largest and then the values, the second out of the L1 cache.
+    auto load_q_scaled = [&](const PfPiece& w) {
+      const PfRows u = pf_rows<MODE>(p, w.bh, w.m);
+      const int tq0 = (u.m * p.streams + s) * p.P, n_pos = min(p.P, u.Tq - tq0), rw0 = (warp & 3) * 32 + lane / QL;
+      const int64_t qb = u.q0 + (int64_t)(u.h * p.G) * p.qs_h + (int64_t)tq0 * p.qs_t + 8 * c_q;
+      const bool bf = p.q_dtype == HQMQ_BF16;
+      const uint4* qp = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.Q) + qb);
+      const int st_h = (int)(p.qs_h >> 3), st_t = (int)(p.qs_t >> 3);
+      auto fetch = [&](uint4* v, int k0) {         // eight pieces of 16 bytes on their way
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int rw = rw0 + (k0 + k) * QR, pw = (int)((uint32_t)rw * g_inv >> 16), gw = rw - pw * p.G;
+          v[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (pw < n_pos) v[k] = __ldg(qp + (gw * st_h + pw * st_t));
+        }
+      };
+      auto slow = [&](int k, float* f) {           // any strides, any type
+        const int rw = rw0 + k * QR, pw = (int)((uint32_t)rw * g_inv >> 16), gw = rw - pw * p.G;
+        const int64_t o = qb + (int64_t)gw * p.qs_h + (int64_t)pw * p.qs_t;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = pw < n_pos ? load_float(p.Q, o + e, p.q_dtype) : 0.f;
+      };
+      auto put = [&](int k, uint4 v) {
+        const int rw = rw0 + k * QR;
+        const uint32_t dst = sQ + s * TB + rw * 128 + (c_q >> 3) * 16384 + (((c_q & 7) ^ (rw & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+      };
+      float big = 0.f;
+      if (p.q_vec) {
+        uint32_t mx = 0u;                          // (the bits of 16-bit sizes order like their values)
+#pragma unroll 1
+        for (int k0 = 0; k0 < QL; k0 += 8) {
+          uint4 v[8];
+          fetch(v, k0);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu), __vmaxu2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu)));
+        }
+        big = fmaxf(bits16_to_float((uint16_t)mx, p.q_dtype), bits16_to_float((uint16_t)(mx >> 16), p.q_dtype));
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < QL; ++k) {
+          float f[8];
+          slow(k, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(f[e]));
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      const int e2 = min(100, max(-100, (int)(__float_as_uint(big) >> 23) - 127));
+      const float mul = __uint_as_float((uint32_t)(127 - e2) << 23);
+      if (p.q_vec) {
+#pragma unroll 1
+        for (int k0 = 0; k0 < QL; k0 += 8) {
+          uint4 v[8];
+          fetch(v, k0);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            uint32_t* w4 = reinterpret_cast<uint32_t*>(&v[k]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 h2 = __half22float2(*reinterpret_cast<const __half2*>(&w4[e]));
+              w4[e] = pack_half2((bf ? __uint_as_float(w4[e] << 16) : h2.x) * mul, (bf ? __uint_as_float(w4[e] & 0xffff0000u) : h2.y) * mul);
+            }
+            put(k0 + k, v[k]);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < QL; ++k) {
+          float f[8];
+          slow(k, f);
+          put(k, make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul), pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul)));
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(qfull + 8 * s);
+      return __uint_as_float((uint32_t)(127 + e2) << 23);
+    };
     auto load_q = [&](const PfPiece& w) {
       const PfRows rw_ = pf_rows<MODE>(p, w.bh, w.m);
       const int64_t qb = rw_.q0 + (int64_t)(rw_.h * p.G) * p.qs_h + 8 * c_q;
@@ -473,7 +555,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
     float2 l2 = make_float2(0.f, 0.f);
     for (bool first = true;; first = false) {
       // the last Q K^T of the unit is complete (or there is no unit yet): the next unit's queries may take their place
-      if (more) load_q(nq);
+      float q_next = 1.f;
+      if (more) {
+        if constexpr (MODE == 0) load_q(nq); else q_next = load_q_scaled(nq);
+      }
       if (!first) {
         ok = wait(odone + 8 * s, u & 1u);
         ok = __all_sync(0xffffffffu, ok);
@@ -567,7 +652,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
       const int beg_lo = __reduce_min_sync(0xffffffffu, live ? beg : 0x7fffffff), beg_hi = __reduce_max_sync(0xffffffffu, live ? beg : 0);
       const int end_lo = __reduce_min_sync(0xffffffffu, live ? end : 0x7fffffff), end_hi = __reduce_max_sync(0xffffffffu, live ? end : 0);
       if (!live) { beg = beg_lo; end = end_hi; }
-      const float kmul = p.kmul[w.scale];
+      const float kmul = MODE == 0 ? p.kmul[w.scale] : p.kmul[w.scale] * q_next;
       vmul = lost ? NAN : p.vmul[w.scale];
       const float2 kmul2 = make_float2(kmul, kmul);
       float2 cap2 = kmul2, smul2 = kmul2;        // what a score is multiplied by under the tanh, and before its exponential
@@ -610,8 +695,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
           float mc = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kmul;
           if constexpr (MODE == 2) {
             // The scores become tanh(score / cap), in place.  The polynomial holds up to the cap; a tile of a warp with a larger score, or a
-            // masked one, goes through exp2 (1322 us for all tiles of the case below, 782 with a polynomial up to half the cap for all).  (Either way the exponentials that follow take them as they took scores: with the cap inside that
-            // code, twice over, 1 x 16k, 2048 queries took 2108 us; the polynomial alone inside it spills, 4200.)
+            // masked one, goes through exp2 (1322 us for all tiles of the case below, 782 with a polynomial up to half the cap for all), which
+            // loses 2^-23 of the cap: 0.002 of a log2 at the largest that is taken.  (The exponentials that follow take them as they took scores:
+            // with the cap inside that code, twice over, 1 x 16k, 2048 queries took 2108 us; the polynomial alone inside it spills, 4200; ahead of the
+            // masks it spills, too, 898.)
             float mn[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
 #pragma unroll
             for (int c = 0; c < 128; c += 8)
@@ -624,14 +711,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
                 const float2 y = cap_near(mul2(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), cap2));
                 r[c] = __float_as_uint(y.x); r[c + 1] = __float_as_uint(y.y);
               }
+              mc = cap_near(make_float2(mc * p.cap_in, 0.f)).x * p.cap_log2;
             } else {
 #pragma unroll
               for (int c = 0; c < 128; ++c) {
                 const float x = __uint_as_float(r[c]);
-                r[c] = x == -INFINITY ? 0xff800000u : __float_as_uint(cap_exp(x * cap2.x));
+                r[c] = x == -INFINITY ? 0xff800000u : __float_as_uint(cap_far(x * cap2.x));
               }
+              if (mc != -INFINITY) mc = cap_far(mc * p.cap_in) * p.cap_log2;
             }
-            if (mc != -INFINITY) mc = cap_exp(mc * p.cap_in) * p.cap_log2;
           }
           if (__any_sync(0xffffffffu, mc > m_run + kPfSlack)) {
             const float m_new = fmaxf(m_run, mc);

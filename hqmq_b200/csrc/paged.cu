@@ -28,8 +28,8 @@ int check_args(const hqmq_paged_attn_args* a, bool mass) {
   if (!is_float_dtype(a->q_dtype)) return HQMQ_ERR_DTYPE;
   if (((uintptr_t)a->plan_data & 15) || ((uintptr_t)a->table_K & 7)) return HQMQ_ERR_ALIGN;
   if (a->r_qmax != (1 << a->K.radius_bits) - 1) return HQMQ_ERR_SHAPE;
-  if (!(a->softcap >= 0.f) || a->softcap > 1e30f || (a->softcap > 0.f && a->softcap < 1e-3f)) return HQMQ_ERR_ARG;
-  if (!(a->softmax_scale > -INFINITY && a->softmax_scale < INFINITY)) return HQMQ_ERR_ARG;
+  if (!(a->softcap >= 0.f) || a->softcap > 1e4f || (a->softcap > 0.f && a->softcap < 1e-3f)) return HQMQ_ERR_ARG;
+  if (!(a->softmax_scale > 0.f && a->softmax_scale < INFINITY)) return HQMQ_ERR_ARG;
   if (mass) {
     if (!is_half_dtype(a->q_dtype)) return HQMQ_ERR_UNSUPPORTED;
     return a->mass ? HQMQ_OK : HQMQ_ERR_ARG;
@@ -96,7 +96,7 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   p.window = pl.window; p.sdt = a->K.scale_dtype; p.pay_bf16 = (a->K.flags ? a->K : a->V).out_dtype == HQMQ_BF16;
   p.qmaxf = (float)a->r_qmax; p.vfac = 1.f / (float)a->r_qmax;
   p.kfac = a->softmax_scale * kLog2e / (float)a->r_qmax;
-  if (a->softcap > 0.f) { p.cap_log2 = a->softcap * kLog2e; p.kfac *= 2.f / a->softcap; }
+  if (a->softcap > 0.f) { p.cap_log2 = a->softcap * kLog2e; p.kfac *= 1.f / p.cap_log2; }
   const int4* d = reinterpret_cast<const int4*>(a->plan_data);
   p.hdr = a->plan_data;
   p.seqs = d + pl.seqs / 4; p.units = d + pl.dec_unit / 4; p.cuts = d + pl.dec_cut / 4;

@@ -21,7 +21,7 @@ struct DecodeParams {
   const uint16_t* tblK; const uint16_t* tblV;
   const float* sinks;
   int table_rows, ib, row_bytes, repk, repv, window;
-  float kfac, cap_log2;          // kfac: what a product is multiplied by beside rs (softmax scale * log2 e / qmax, or with a cap 2 log2 e / cap times that)
+  float kfac, cap_log2;          // kfac: what a product is multiplied by beside rs (softmax scale * log2 e / qmax; with a cap over cap_log2)
   float qmaxf, vfac;             // 1 / qmax
   int sdt, pay_bf16;             // type of the scales; whether the flagged chunks' values are bf16 (else fp16)
   const int4* seqs; const int4* units; const int* base; const int* warps; const int4* cuts; const int* tabs; const int* hdr;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) sc[nb][x] = capped(sc[nb][x], p.cap_log2);
+          for (int x = 0; x < 4; ++x) sc[nb][x] = p.cap_log2 * tanh_of(sc[nb][x]);
       }
       if (edge) {
 #pragma unroll

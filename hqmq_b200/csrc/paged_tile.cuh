@@ -237,8 +237,14 @@ __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& 
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// softcap * tanh(x / softcap) in the exp2 domain, from x * 2 log2(e) / softcap: 1 - 2 / (2^y + 1)
-__device__ __forceinline__ float capped(float y, float cap_log2) { return cap_log2 - __fdividef(2.f * cap_log2, fast_exp2(y) + 1.f); }
+// tanh(x): for |x| <= 1/2 as x times a cubic in x^2 through its values at the Chebyshev nodes of [0, 1/4] (within 5e-7 of the value,
+// however small: a cap far above the scores leaves them as they are), beyond as 1 - 2 / (e^2x + 1).
+__device__ __forceinline__ float tanh_of(float x) {
+  const float q = x * x;
+  const float near = x * fmaf(q, fmaf(q, fmaf(q, -0.0443927385f, 0.131899402f), -0.333262831f), 0.999999464f);
+  const float far = 1.f - __fdividef(2.f, fast_exp2(2.885390081777927f * x) + 1.f);
+  return q <= 0.25f ? near : far;
+}
 
 }  // namespace paged
 }  // namespace hqmq

@@ -259,8 +259,10 @@ def _attn_args(Q, pool, batch, table_K, softmax_scale, softcap, sinks, what):
         raise ValueError(f"{what}: Q on {Q.device}, the pool on {pool.device}")
     if Q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"{what}: Q is fp32, fp16 or bf16, not {Q.dtype}")
-    if softcap is not None and not 1e-3 <= softcap <= 1e30:
-        raise ValueError(f"softcap={softcap}: a positive number (None: no cap)")
+    if softcap is not None and not 1e-3 <= softcap <= 1e4:
+        raise ValueError(f"softcap={softcap}: a number from 0.001 to 10000 (None: no cap)")
+    if softmax_scale is not None and not 0.0 < softmax_scale < float("inf"):
+        raise ValueError(f"softmax_scale={softmax_scale}: a positive number (None: 1 / sqrt(d_head))")
     if sinks is not None and (sinks.shape != (batch.n_heads,) or sinks.device != pool.device):
         raise ValueError(f"{what}: sinks are one number per query head on {pool.device}")
     _codebook(table_K, pool, what)

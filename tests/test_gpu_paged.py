@@ -256,20 +256,30 @@ def test_attention_types_strides_and_scale(q_dtype, o_dtype):
     check_attend(w, again, q, q_lens, 4, scale=0.03)
 
 
-def test_attention_of_values_far_from_one():
+@pytest.mark.parametrize("n_q", [1, 8, 40])
+@pytest.mark.parametrize("q_pow,k_pow,v_pow", [(60, -60, -40), (-30, 30, 40), (20, -20, 0)])
+def test_attention_of_values_far_from_one(n_q, q_pow, k_pow, v_pow):
     """Keys, values and queries whose sizes fp16 does not hold: operands are relative to powers of two."""
-    for n_q in (1, 40):
-        w = World(1, 128, 96, 4, [200, 90], outliers="both")
-        for pk, f in ((w.pool.K, 2.0 ** -60), (w.pool.V, 2.0 ** -40)):
-            for name in ("rs", "out_vals"):
-                pk.pages(name).mul_(f)
-        q = queries(w, [n_q, n_q], 4, torch.bfloat16) * 2.0 ** 60
-        out = hqmq.paged_attention(q.to(DEV), w.pool, w.batch([n_q, n_q], 4), *w.tab) if n_q == 1 else None
-        if out is not None:
-            K, V = w.dense()
-            for s in range(2):
-                o, _, bound, _ = attend64(q[s:s + 1], K[s], V[s], 4, None, None, None, 128 ** -0.5)
-                assert bool(((out[s:s + 1].cpu().double() - o).abs() <= bound + o.abs() * 2.0 ** -8 + 2.0 ** -50).all())
+    w = World(1, 128, 96, 4, [200, 90], outliers="both")
+    for pk, e in ((w.pool.K, k_pow), (w.pool.V, v_pow)):
+        for name in ("rs", "out_vals"):
+            pk.pages(name).mul_(2.0 ** e)
+    q = (queries(w, [n_q, n_q], 4, torch.bfloat16).float() * 2.0 ** q_pow).to(torch.bfloat16)
+    out = hqmq.paged_attention(q.to(DEV), w.pool, w.batch([n_q, n_q], 4), *w.tab).cpu()
+    K, V = w.dense()
+    for s in range(2):
+        o, _, bound, _ = attend64(q[s * n_q:(s + 1) * n_q], K[s], V[s], 4, None, None, None, 128 ** -0.5)
+        off = (out[s * n_q:(s + 1) * n_q].double() - o).abs()
+        assert bool((off <= bound + o.abs() * (2.0 ** -8 + 2.0 ** -18)).all())
+
+
+@pytest.mark.parametrize("cap", [0.01, 1.0, 30.0, 1e4])
+def test_caps_from_small_to_large(cap):
+    w = World(1, 128, 96, 4, [300, 70])
+    for q_lens in ([1, 1], [40, 20]):
+        q = queries(w, q_lens, 4, torch.bfloat16, scale=3.0)
+        out = hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab, softcap=cap)
+        check_attend(w, out, q, q_lens, 4, cap=cap)
 
 
 def test_a_shared_prefix_and_the_same_page_twice():
@@ -613,8 +623,9 @@ def test_refusals():
             ok(**kw)
     with pytest.raises(_lib.HqmqError):
         ok(out=torch.empty(2, 8, 256, device=DEV)[..., ::2])
-    with pytest.raises(_lib.HqmqError):
-        ok(softmax_scale=float("nan"))
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            ok(softmax_scale=scale)
     with pytest.raises(TypeError):
         ok(Q=q.to(torch.int32))
     with pytest.raises(TypeError):

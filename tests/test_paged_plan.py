@@ -239,7 +239,8 @@ def _args(pool, batch, G=2):
 @pytest.mark.parametrize("change,code", [
     (dict(struct_size=8), -1), (dict(Q=None), -1), (dict(O=None), -1), (dict(plan_data=None), -1), (dict(table_K=None), -1),
     (dict(q_dtype=_lib.I32), -3), (dict(o_dtype=_lib.I8), -3), (dict(plan_data=(1 << 20) + 4), -4), (dict(r_qmax=15), -2),
-    (dict(softcap=-1.0), -1), (dict(softcap=float("nan")), -1), (dict(softmax_scale=float("nan")), -1), ({}, -5),
+    (dict(softcap=-1.0), -1), (dict(softcap=float("nan")), -1), (dict(softmax_scale=float("nan")), -1), (dict(softmax_scale=0.0), -1),
+    (dict(softcap=2e4), -1), ({}, -5),
 ])
 def test_abi_refuses_arguments(built_lib, change, code):
     pool = make_pool(outliers_K=True)
