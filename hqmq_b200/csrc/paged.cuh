@@ -52,8 +52,9 @@ constexpr int kMassRowsWide = 32;                    // rows of a unit of the we
 constexpr int kMassGroup = 512;                      // tokens of a CTA of the weights' second kernel
 constexpr int kMaxCodewords = 6144;                   // two tables and the rings of 16 warps in shared memory, whatever the radius bits
 constexpr int kMaxPage = 1024;                       // tokens of a page
-constexpr int kWarpRecord = 8;                       // words of a warp's record: its stretch, first unit and tile, the unit's end, the
-                                                     // sequence's place among the tables, the first tile's page: one load, then the copies
+constexpr int kWarpRecord = 16;                      // words of a warp's record: its stretch, first unit and tile; the unit's end, the
+                                                     // sequence's place among the tables, the first tile's page, the unit's first row; its
+                                                     // stretch of the flat sequence; the sequence: one load, then the copies and queries
 // CTAs of a head that run as one cluster (148 SMs hold fifteen clusters of eight of these CTAs).
 constexpr int kClusterMax = 8;
 inline bool as_cluster(int ctas, int heads) { return ctas <= kClusterMax && (int64_t)ctas * heads <= 112; }

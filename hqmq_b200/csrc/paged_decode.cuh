@@ -150,9 +150,9 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   bool first_seg = true;
   while (i < n) {
     // ---- a unit, or what the stretch has of it ------------------------------------------------------------------------------
-    const int4 un = __ldg(p.units + u), sq4 = __ldg(p.seqs + un.x);
-    const Seq s{sq4.x, sq4.y, sq4.z, sq4.w};
-    const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
+    const Taken un = first_seg ? take_first(p.warps + w * kWarpRecord, f0) : take_unit(p.units, p.seqs, p.base, u);
+    const Seq s = un.s;
+    const int b0 = un.b0, b1 = un.b1;
     const int rows = s.q * p.q.G;
     uint32_t qb[QREG ? NB : 1][NKS][2];
     float qmul[NB];
@@ -174,8 +174,8 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       for (int x = 0; x < NOT; ++x) o[nb][x][0] = o[nb][x][1] = o[nb][x][2] = o[nb][x][3] = 0.f;
     }
     float v_pow = 0.f, v_inv = 0.f;        // the power of two that V's scales are relative to (0: none yet), and one over it
-    const int i_end = min(n, i + (un.w - (un.z + (f0 + i - b0))));
-    int tile = un.z + (f0 + i - b0);
+    const int i_end = min(n, b1 - f0);
+    int tile = un.lo + (f0 + i - b0);
     for (; i < i_end; ++i, ++tile) {
       cp_wait_all();
       __syncwarp();

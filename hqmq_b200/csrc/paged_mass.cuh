@@ -92,10 +92,10 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
   int u = __ldg(p.warps + w * kWarpRecord + 2), i = 0;
   bool first_seg = true;
   while (i < n) {
-    const int4 un = __ldg(p.units + u), sq4 = __ldg(p.seqs + un.x);
-    const Seq s{sq4.x, sq4.y, sq4.z, sq4.w};
-    const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
-    const int rows = s.q * p.q.G, row0 = un.y;
+    const Taken un = first_seg ? take_first(p.warps + w * kWarpRecord, f0) : take_unit(p.units, p.seqs, p.base, u);
+    const Seq s = un.s;
+    const int b0 = un.b0, b1 = un.b1;
+    const int rows = s.q * p.q.G, row0 = un.row0;
     uint32_t qb[1][NKS][2];
     float qmul[NB][2];
 #pragma unroll
@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
     float2 ml[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) ml[nb][0] = ml[nb][1] = make_float2(-INFINITY, 0.f);
-    const int i_end = min(n, i + (b1 - (f0 + i)));
-    int tile = un.z + (f0 + i - b0);
+    const int i_end = min(n, b1 - f0);
+    int tile = un.lo + (f0 + i - b0);
     for (; i < i_end; ++i, ++tile) {
       cp_wait_all();
       __syncwarp();
@@ -316,16 +316,28 @@ template <int NB>
 __global__ void __launch_bounds__(256) paged_mass_kernel(const MassParams p) {
   constexpr int R = 8 * NB, LPT = R / 4, PER = kMassGroup * LPT / 256;
   __shared__ float2 s_stat[R];
-  grid_dep_wait();
+  // (the plan, and what the weights were, are there before the kernel ahead of this one)
   const int n_units = p.hdr[2], total = p.hdr[3];
-  if ((int)blockIdx.x >= p.hdr[4]) return;
+  const bool mine = (int)blockIdx.x < p.hdr[4];
   const int h = blockIdx.y, n_warps = p.ctas * kMassWarps;
-  const int4 gr = __ldg(p.groups + blockIdx.x), sq4 = __ldg(p.seqs + gr.x);
+  const int4 gr = __ldg(p.groups + (mine ? blockIdx.x : 0)), sq4 = __ldg(p.seqs + gr.x);
   const Seq s{sq4.x, sq4.y, sq4.z, sq4.w};
   const int rows = s.q * p.q.G, tid = threadIdx.x;
-  float acc[PER];
+  float acc[PER], was[PER];
+  int64_t at[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+  for (int i = 0; i < PER; ++i) {
+    acc[i] = was[i] = 0.f;
+    at[i] = -1;
+    const int t = gr.y + (tid + i * 256) / LPT;
+    if (mine && tid % LPT == 0 && t < s.kv) {
+      const int page = __ldg(p.tabs + s.tab + (t >> p.pool.page_bits));
+      at[i] = (((int64_t)page * p.pool.Hkv + h) << p.pool.page_bits) + (t & ((1 << p.pool.page_bits) - 1));
+      if (p.prior) was[i] = p.prior[at[i]];
+    }
+  }
+  grid_dep_wait();
+  if (!mine) return;
   for (int u = gr.z; u < gr.w; ++u) {
     const int4 un = __ldg(p.units + u);
     if (un.w * kTile <= gr.y || un.z * kTile >= gr.y + kMassGroup) continue;      // (the same for all threads)
@@ -371,12 +383,7 @@ __global__ void __launch_bounds__(256) paged_mass_kernel(const MassParams p) {
   for (int i = 0; i < PER; ++i) {
 #pragma unroll
     for (int o = 1; o < LPT; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-    const int t = gr.y + (tid + i * 256) / LPT;
-    if (tid % LPT == 0 && t < s.kv) {
-      const int page = __ldg(p.tabs + s.tab + (t >> p.pool.page_bits));
-      const int64_t at = (((int64_t)page * p.pool.Hkv + h) << p.pool.page_bits) + (t & ((1 << p.pool.page_bits) - 1));
-      p.mass[at] = p.prior ? fmaf(p.decay, p.prior[at], acc[i]) : acc[i];
-    }
+    if (at[i] >= 0) p.mass[at[i]] = p.prior ? fmaf(p.decay, was[i], acc[i]) : acc[i];
   }
 }
 

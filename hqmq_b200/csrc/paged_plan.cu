@@ -142,7 +142,7 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
     p.ch_ctas = p.ch_whole ? grid_w : (int)((total + L - 1) / L);
   }
   p.ms_units = (int)ms_units; p.ms_tiles = (int)ms_tiles; p.ms_groups = p.H_q ? (int)ms_groups : 0;
-  p.ms_ctas = ctas(ms_tiles, kMassWarps);
+  p.ms_ctas = (int)std::max<int64_t>(1, std::min<int64_t>(most, (ms_tiles + kMassWarps - 1) / kMassWarps));
   p.ms_tile_room = p.ms_tiles; p.ms_group_room = p.ms_groups;
   if (p.tab_room) {
     if (n_tab > p.tab_room) return HQMQ_ERR_CAPACITY;
@@ -253,7 +253,9 @@ extern "C" int hqmq_paged_plan_fill(const hqmq_paged_plan* plan, const int32_t* 
       const int tile = f0 < total ? un[2] + f0 - out[base_at + u] : un[2];
       int32_t* r = out + warp_at + kWarpRecord * w;
       r[0] = f0; r[1] = f1; r[2] = u; r[3] = tile;
-      r[4] = un[3]; r[5] = sq[3]; r[6] = out[p.tabs + sq[3] + tile * 16 / p.page_tokens];
+      r[4] = un[3]; r[5] = sq[3]; r[6] = out[p.tabs + sq[3] + tile * 16 / p.page_tokens]; r[7] = un[1];
+      r[8] = out[base_at + u]; r[9] = out[base_at + u + 1];
+      for (int i = 0; i < 4; ++i) r[12 + i] = sq[i];
     }
   };
   if (p.dec_units) {

@@ -40,6 +40,19 @@ struct PoolView {
   int Hkv, page_bits;
 };
 
+// A unit as a warp takes it up: its first row, its tiles' stretch of the flat sequence, where its tiles begin, the sequence.
+struct Taken { int row0, b0, b1, lo; Seq s; };
+__device__ __forceinline__ Taken take_unit(const int4* units, const int4* seqs, const int* base, int u) {
+  const int4 un = __ldg(units + u), sq = __ldg(seqs + un.x);
+  return Taken{un.y, __ldg(base + u), __ldg(base + u + 1), un.z, Seq{sq.x, sq.y, sq.z, sq.w}};
+}
+// ... the first one, from the warp's record (f0: the stretch's begin): no load waits for another
+__device__ __forceinline__ Taken take_first(const int* record, int f0) {
+  const int4 a = __ldg(reinterpret_cast<const int4*>(record)), b = __ldg(reinterpret_cast<const int4*>(record) + 1);
+  const int4 c = __ldg(reinterpret_cast<const int4*>(record) + 2), sq = __ldg(reinterpret_cast<const int4*>(record) + 3);
+  return Taken{b.w, c.x, c.y, a.w - (f0 - c.x), Seq{sq.x, sq.y, sq.z, sq.w}};
+}
+
 // The tiles of a warp's stretch, in order.  The page of a tile is loaded a tile ahead: it is what the copies' addresses wait for.
 struct TileIter {
   int u, tile, hi, tab, left, page;

@@ -37,7 +37,7 @@ def stretch(w, total, n):
     return w * total // n if w < n else total
 
 
-def check_flat(words, units, bases, warps, total, ctas, per_cta, want, tables, page):
+def check_flat(words, units, bases, warps, total, ctas, per_cta, want, tables, page, lengths):
     """Units in order with their tile ranges, prefix sums, and the unit that every warp's stretch begins in."""
     got = [tuple(words[units + 4 * i:units + 4 * i + 4].tolist()) for i in range(len(want))]
     assert got == want
@@ -46,13 +46,15 @@ def check_flat(words, units, bases, warps, total, ctas, per_cta, want, tables, p
     n = ctas * per_cta
     for w in range(n):
         f = stretch(w, total, n)
-        rec = words[warps + 8 * w:warps + 8 * w + 7].tolist()
+        rec = words[warps + 16 * w:warps + 16 * w + 16].tolist()
         assert rec[:2] == [f, stretch(w + 1, total, n)]
         if f < total:
             u = rec[2]
             assert base[u] <= f < base[u + 1] and rec[3:5] == [want[u][2] + f - base[u], want[u][3]]
             s = want[u][0]
-            assert rec[5] == sum(len(t) for t in tables[:s]) and rec[6] == tables[s][rec[3] * 16 // page]
+            tab = sum(len(t) for t in tables[:s])
+            assert rec[5:8] == [tab, tables[s][rec[3] * 16 // page], want[u][1]] and rec[8:10] == base[u:u + 2].tolist()
+            assert rec[12:14] == lengths[s] and rec[15] == tab
 
 
 @pytest.mark.parametrize("seed", range(12))
@@ -82,7 +84,7 @@ def test_plan_covers_every_tile_once(seed):
     assert p.dec_units == len(dec) and p.dec_rows == next(r for r in (8, 16, 32) if all(q[s] * G <= r for s in few))
     if dec:
         per = DEC_WARPS_WIDE if p.dec_rows > 8 else DEC_WARPS
-        check_flat(w, p.dec_unit, p.dec_base, p.dec_warp, p.dec_tiles, p.dec_ctas, per, dec, tables, page)
+        check_flat(w, p.dec_unit, p.dec_base, p.dec_warp, p.dec_tiles, p.dec_ctas, per, dec, tables, page, [list(x) for x in zip(kv, q)])
         # units between CTAs: every cut names its first and last CTA
         base = w[p.dec_base:p.dec_base + len(dec) + 1]
         n = p.dec_ctas * per
@@ -96,7 +98,7 @@ def test_plan_covers_every_tile_once(seed):
     ms = [(s, r, *tiles(*keys_of(kv[s], q[s], G, window, r, min(q[s] * G, r + rows)))) for s in range(B) for r in range(0, q[s] * G, rows)]
     assert p.ms_units == len(ms)
     if ms:
-        check_flat(w, p.ms_unit, p.ms_base, p.ms_warp, p.ms_tiles, p.ms_ctas, MASS_WARPS, ms, tables, page)
+        check_flat(w, p.ms_unit, p.ms_base, p.ms_warp, p.ms_tiles, p.ms_ctas, MASS_WARPS, ms, tables, page, [list(x) for x in zip(kv, q)])
     groups = [w[p.ms_group + 4 * i:p.ms_group + 4 * i + 4].tolist() for i in range(p.ms_groups)]
     assert [g[:2] for g in groups] == [[s, t] for s in range(B) for t in range(0, kv[s], GROUP)]
     for s, t, u0, u1 in groups:
