@@ -49,7 +49,9 @@ __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_grou
 constexpr int kDecWarps = 16, kDecWarpsWide = 8;     // warps of a decode CTA, for up to 8 and up to 16 rows
 constexpr int kMassWarps = 12;
 constexpr int kMassRowsWide = 32;                    // rows of a unit of the weights where a sequence has more than 8
-constexpr int kMassGroup = 512;                      // tokens of a CTA of the weights' second kernel
+// Tokens of a CTA of the weights' second kernel: of 8 rows a token has 32 bytes of scores per unit, of 32 rows 128 (512 tokens either way:
+// 46 us for the last 32 tokens of 4 x 8k, whose sequences have four units each, in 360 CTAs).
+constexpr int mass_group(int rows) { return rows > 8 ? 128 : 512; }
 constexpr int kMaxCodewords = 6144;                   // two tables and the rings of 16 warps in shared memory, whatever the radius bits
 constexpr int kMaxPage = 1024;                       // tokens of a page
 constexpr int kWarpRecord = 16;                      // words of a warp's record: its stretch, first unit and tile; the unit's end, the

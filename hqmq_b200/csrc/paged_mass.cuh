@@ -5,7 +5,7 @@
 //           products are kept whole: a codeword times its radius code has 17 bits and a flagged value times qmax / rs 24; each is the sum
 //           of two fp16 operands, hi + lo, of two products (fp16 alone: relative error of a weight 1e-3; so 1e-6).  Q is fp16 after
 //           division by a power of two: exact for fp16 and bf16, but for what is 2^-24 of the row's largest.
-//   sum     per 512 tokens of a sequence: exp2(score - m) / l over the rows, on top of decay * prior.  Every token has one owner, so
+//   sum     per 512 or 128 tokens of a sequence: exp2(score - m) / l over the rows, on top of decay * prior.  Every token has one owner, so
 //           nothing is added in an order of its own (no atomics).
 // The scores go through memory between the two (R rows x 4 bytes a token, against 50 to 80 bytes of codes): a second decoding pass
 // would cost the gathers and products again, which bound the first.
@@ -311,10 +311,10 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
   }
 }
 
-// blockIdx.x = 512 tokens of a sequence, blockIdx.y = KV head.
+// blockIdx.x = a group of tokens of a sequence, blockIdx.y = KV head.
 template <int NB>
 __global__ void __launch_bounds__(256) paged_mass_kernel(const MassParams p) {
-  constexpr int R = 8 * NB, LPT = R / 4, PER = kMassGroup * LPT / 256;
+  constexpr int R = 8 * NB, LPT = R / 4, kGroup = mass_group(R), PER = kGroup * LPT / 256;
   __shared__ float2 s_stat[R];
   // (the plan, and what the weights were, are there before the kernel ahead of this one)
   const int n_units = p.hdr[2], total = p.hdr[3];
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(256) paged_mass_kernel(const MassParams p) {
   if (!mine) return;
   for (int u = gr.z; u < gr.w; ++u) {
     const int4 un = __ldg(p.units + u);
-    if (un.w * kTile <= gr.y || un.z * kTile >= gr.y + kMassGroup) continue;      // (the same for all threads)
+    if (un.w * kTile <= gr.y || un.z * kTile >= gr.y + kGroup) continue;      // (the same for all threads)
     const int b0 = __ldg(p.base + u), b1 = __ldg(p.base + u + 1);
     __syncthreads();
     if (tid < R) {

@@ -67,7 +67,6 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
     total_q += q_lens[s];
     all_q = std::max(all_q, q_lens[s]);
     n_tab += blocks_of(kv_lens[s], p.page_tokens);
-    ms_groups += blocks_of(kv_lens[s], kMassGroup);
     if (!p.H_q || !q_lens[s]) continue;
     if (q_lens[s] > (1 << 26)) return HQMQ_ERR_SHAPE;
     most_rows = std::max(most_rows, q_lens[s] * G);
@@ -95,6 +94,7 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
   p.ch_streams = most_q > P ? 2 : 1;
   int64_t ch_units = 0, ch_tiles = 0, img = 0;
   p.ms_rows = most_rows > 8 ? kMassRowsWide : 8;
+  for (int s = 0; s < p.n_seqs; ++s) ms_groups += blocks_of(kv_lens[s], mass_group(p.ms_rows));
   for (int s = 0; s < p.n_seqs; ++s) {
     if (!p.H_q || !q_lens[s]) continue;
     const int rows = q_lens[s] * G;
@@ -150,7 +150,7 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
     const int64_t blocks = blocks_of(most_rows, p.ms_rows), tiles = blocks * p.tab_room * (p.page_tokens / 16);
     if (tiles > (1 << 29)) return HQMQ_ERR_SHAPE;
     p.ms_tile_room = (int)tiles;
-    p.ms_group_room = p.H_q ? (int)((int64_t)p.tab_room * p.page_tokens / kMassGroup + p.n_seqs) : 0;
+    p.ms_group_room = p.H_q ? (int)((int64_t)p.tab_room * p.page_tokens / mass_group(p.ms_rows) + p.n_seqs) : 0;
   }
   if (p.renew) {
     if (ch_units || had.ch_units) return HQMQ_ERR_UNSUPPORTED;
@@ -234,7 +234,7 @@ extern "C" int hqmq_paged_plan_fill(const hqmq_paged_plan* plan, const int32_t* 
       }
     }
     if (p.H_q)
-      for (int t = 0; t < kv; t += kMassGroup) {
+      for (int t = 0; t < kv; t += mass_group(p.ms_rows)) {
         int32_t* g = out + p.ms_group + 4 * mg++;
         g[0] = s; g[1] = t; g[2] = my_mu; g[3] = mu;
       }

@@ -9,7 +9,7 @@ import torch
 import hqmq_b200 as hqmq
 from hqmq_b200 import _lib
 
-DEC_WARPS, DEC_WARPS_WIDE, MASS_WARPS, GROUP = 16, 8, 12, 512
+DEC_WARPS, DEC_WARPS_WIDE, MASS_WARPS = 16, 8, 12
 
 
 def make_pool(n_pages=64, H=2, d=128, S=24, rb=3, page=64, **kw):
@@ -100,7 +100,7 @@ def test_plan_covers_every_tile_once(seed):
     if ms:
         check_flat(w, p.ms_unit, p.ms_base, p.ms_warp, p.ms_tiles, p.ms_ctas, MASS_WARPS, ms, tables, page, [list(x) for x in zip(kv, q)])
     groups = [w[p.ms_group + 4 * i:p.ms_group + 4 * i + 4].tolist() for i in range(p.ms_groups)]
-    assert [g[:2] for g in groups] == [[s, t] for s in range(B) for t in range(0, kv[s], GROUP)]
+    assert [g[:2] for g in groups] == [[s, t] for s in range(B) for t in range(0, kv[s], 512 if rows == 8 else 128)]
     for s, t, u0, u1 in groups:
         assert [u for u in range(len(ms)) if ms[u][0] == s] == list(range(u0, u1))
     # prompt chunks: units of a sequence in order, images of the tiles that any of them sees, pieces of equal size
