@@ -90,7 +90,7 @@ struct EvictParams {
   hqmq_packed K, V;
   const float* mass; float* new_mass; int* kept;
   const int4* src_seqs; const int* src_tabs; const int4* dst_seqs; const int* dst_tabs;
-  int first, last, kept_stride, Hkv, page_bits, per_page, cached, n_seqs;
+  int first, last, kept_stride, Hkv, page_bits, per_page, cached, n_seqs;      // cached: tokens of a CTA that shared memory holds
 };
 
 __device__ __forceinline__ uint32_t order_key(float f) {      // larger is heavier; no number: 0, below every number
@@ -130,10 +130,11 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
   const int sh = (int)blockIdx.x / C, sq = sh / p.Hkv, h = sh - sq * p.Hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int4 s4 = __ldg(p.src_seqs + sq);
-  const int n = s4.x, tab = s4.w, keep = min(__ldg(&p.dst_seqs[sq].x), n);
+  const int n = s4.x, tab = s4.w, keep = min(min(__ldg(&p.dst_seqs[sq].x), n), p.kept_stride);
   const int last = min(p.last, keep), first = min(p.first, keep - last);
   const int per = ((n + C - 1) / C + 31) & ~31, t0 = min(n, rank * per), t1 = min(n, t0 + per);
   const int mine = t1 - t0;
+  const bool cached = per <= p.cached;
   for (int i = tid; i < 3 * 2048; i += kSelThreads) hist[i] = 0u;
   const float* mass_h = p.mass + ((int64_t)h << p.page_bits);
   auto quad_of = [&](int t) {                  // the weights of tokens t .. t + 3 (t a multiple of four, so they lie in one page)
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     return __ldg(reinterpret_cast<const float4*>(mass_h + (((int64_t)page * p.Hkv) << p.page_bits) + (t & ((1 << p.page_bits) - 1))));
   };
   auto key_at = [&](int i) {
-    if (p.cached) return keys[i];
+    if (cached) return keys[i];
     const float4 v = quad_of((t0 + i) & ~3);
     const int x = (t0 + i) & 3;
     return order_key(x == 0 ? v.x : x == 1 ? v.y : x == 2 ? v.z : v.w);
@@ -159,12 +160,12 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
       auto count = [&](int i, uint32_t k) {
         if (i < mine && free_at(t0 + i) && (pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix)) atomicAdd(hp + ((k >> shift) & (bins - 1)), 1u);
       };
-      if (pass == 0 || !p.cached) {
+      if (pass == 0 || !cached) {
 #pragma unroll 4
         for (int i = 4 * tid; i < mine; i += 4 * kSelThreads) {
           const float4 v = quad_of(t0 + i);
           const uint4 k = make_uint4(order_key(v.x), order_key(v.y), order_key(v.z), order_key(v.w));
-          if (p.cached) *reinterpret_cast<uint4*>(keys + i) = k;
+          if (cached) *reinterpret_cast<uint4*>(keys + i) = k;
           count(i, k.x); count(i + 1, k.y); count(i + 2, k.z); count(i + 3, k.w);
         }
       } else {
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(512) evict_move_kernel(const EvictParams p) {
   if (sq < p.n_seqs) {
     src = __ldg(p.src_seqs + sq);
     const int4 dst = __ldg(p.dst_seqs + sq);
-    keep = min(dst.x, src.x);
+    keep = min(min(dst.x, src.x), p.kept_stride);
     n = max(0, min(64, keep - (pi * pt + part * 64)));
     if (n > 0) ph = (int64_t)__ldg(p.dst_tabs + dst.w + pi) * p.Hkv + h;
   }
@@ -431,8 +432,8 @@ extern "C" int hqmq_paged_evict(const hqmq_paged_evict_args* a, void* stream) {
   while (C < 8 && units * C * 2 <= 148 && a->longest >= 2 * C * 2048) C *= 2;
   while (C < 8 && (a->longest + C - 1) / C + 32 > kSelCached) C *= 2;
   const int per = ((a->longest + C - 1) / C + 31) & ~31;
-  p.cached = per <= kSelCached;
-  const size_t smem = (3 * 2048 + 4 + 2 * kSelWarps + 4 + (p.cached ? per : 0)) * 4;
+  p.cached = per <= kSelCached ? per : 0;
+  const size_t smem = (3 * 2048 + 4 + 2 * kSelWarps + 4 + (size_t)p.cached) * 4;
   cudaStream_t st = (cudaStream_t)stream;
   HQMQ_CHECK_CUDA(raise_smem_limit((const void*)&evict_select_kernel, smem));
   cudaLaunchConfig_t cfg = {};

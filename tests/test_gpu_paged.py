@@ -305,6 +305,59 @@ def test_a_scale_that_is_no_number_shows(plane):
         assert bool(out[a:b].isnan().all()) and not bool(out[:a].isnan().any()) and not bool(out[b:].isnan().any())
 
 
+def test_pages_behind_four_gigabytes():
+    """Rows, side buffers and offsets whose places pass 32 bits (K's codes are 4.6 GB)."""
+    H, n_pages, kv = 8, 140_000, [700, 90]
+    q = hqmq.HQMQ(1, H, 96, 4, device=DEV)
+    quant = hqmq.with_outlier_extraction(q, C=3.0)
+    pool = hqmq.PagedKV(n_pages, H, 128, 96, 4, DEV, outliers_K=True, outliers_V=True, out_cap=128)
+    order = list(range(n_pages - 40, n_pages))
+    random.Random(0).shuffle(order)
+    tables, at = [], 0
+    for n in kv:
+        tables.append(order[at:at + -(-n // 64)])
+        at += -(-n // 64)
+    x = [make_kv("spiky", (1, H, sum(kv), 128), i, torch.bfloat16).to(DEV) for i in (0, 1)]
+    pair = [quant.encode(x[i], 0, i) for i in (0, 1)]
+    batch = hqmq.PagedBatch(pool, tables, kv, kv)
+    hqmq.paged_store(pool, *pair, batch)
+    tab = [q.tables(0, i, DEV)["table16"] for i in (0, 1)]
+    used = [p for t in tables for p in t]
+    planes = []
+    for pk in (pool.K, pool.V):                  # (the used pages alone, as if they were a pool)
+        planes.append({**{k: v[torch.tensor(used, device=DEV)].cpu() for k, v in pk.planes().items()}, "n": 32})
+    local = [[used.index(p) for p in t] for t in tables]
+    K, V = ([dense64(x_, t, 96, 4, pages, n) for pages, n in zip(local, kv)] for x_, t in zip(planes, tab))
+    for q_lens in ([1, 1], [40, 90]):
+        qq = torch.randn(sum(q_lens), 32, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+        b = hqmq.PagedBatch(pool, tables, kv, q_lens, n_heads=32)
+        out, a = hqmq.paged_attention(qq.to(DEV), pool, b, *tab).cpu(), 0
+        for s, n in enumerate(q_lens):
+            o, _, bound, _ = attend64(qq[a:a + n], K[s], V[s], 4, None, None, None, 128 ** -0.5)
+            assert bool(((out[a:a + n].double() - o).abs() <= bound + o.abs() * (2.0 ** -8 + 2.0 ** -18) + 1e-7).all())
+            a += n
+    mass = hqmq.paged_attention_mass(qq.to(DEV), pool, b, tab[0])
+    assert abs(float(mass.sum()) - 130 * 32) < 0.1
+    dst = [order[at:at + 2], order[at + 2:at + 3]]
+    kept = hqmq.paged_evict(pool, batch, hqmq.PagedBatch(pool, dst, [100, 50]), mass).cpu()
+    for s, n in enumerate([100, 50]):
+        for h in range(H):
+            rows = [pool.K.pages("codes")[tables[s][t // 64], h, t % 64] for t in kept[s, h, :n].tolist()]
+            assert torch.equal(torch.stack(rows), torch.cat([pool.K.pages("codes")[p, h] for p in dst[s]])[:n])
+
+
+def test_sinks_of_any_type_and_size():
+    w = World(2, 128, 96, 4, [300, 90])
+    for q_lens in ([1, 1], [40, 90]):
+        q = queries(w, q_lens, 4, torch.bfloat16)
+        sinks = torch.tensor([0.0, -float("inf"), 80.0, -80.0, 3.0, 1e4, -1e4, 1.5]).to(torch.bfloat16)
+        out = hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab, sinks=sinks.to(DEV))
+        check_attend(w, out, q, q_lens, 4, sinks=sinks)
+        assert bool((out[:, 5] == 0).all())
+        off = hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab, sinks=torch.full((8,), float("inf"), device=DEV))
+        assert bool((off == 0).all())
+
+
 def test_many_sequences_and_more_heads_than_sms():
     kv = [1 + (37 * i) % 150 for i in range(300)]
     w = World(2, 64, 24, 3, kv, rounds=2)
