@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
 // know the entries before theirs.  (A CTA of 256 threads per page, with its scans by block, took 4200 instructions a warp for 64 tokens:
 // 67 us for 16 x 2048 tokens of 8 heads.)  Bound: the chain position - page - row - entries, five loads deep, with 32 to 64 warps an SM in it.
 constexpr int kMoveWarps = 8;
-__global__ void __launch_bounds__(512) evict_move_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(512, 2) evict_move_kernel(const EvictParams p) {
   __shared__ uint32_t s_count[16];
   __shared__ int64_t s_row[16][64];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(512) evict_move_kernel(const EvictParams p) {
     const T* s = reinterpret_cast<const T*>(X.codes);
     const uint32_t inv = 65536u / (uint32_t)pieces + 1u;      // i / pieces = i * inv >> 16 for i < 64 * pieces (pieces <= 32)
     const int all = n * pieces;
-    constexpr int U = 8;                                      // pieces of a lane on their way at a time
+    constexpr int U = sizeof(T) == 16 ? 4 : 8;                // pieces of a lane on their way at a time
 #pragma unroll 1
     for (int i0 = lane; i0 < all; i0 += 32 * U) {
       T v[U];
