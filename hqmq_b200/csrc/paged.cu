@@ -107,10 +107,15 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   const bool outl = a->K.flags || a->V.flags;
   const int nb = pl.dec_rows / 8, warps = dec_warps(pl.dec_rows);
   const size_t rings = (size_t)warps * kTileStages * tile_layout(p.row_bytes, true, outl).bytes + kPastPay + (nb > 2 ? (size_t)warps * nb * pl.d * 16 : 0), table = (size_t)(p.table_rows >> 1) * 8;
-  // (a field that no encoder writes may index up to 2^ib / 2 entries: what that reaches lies in the block's shared memory, too)
+  // (the tables with every warp's own entries behind the codebook, if it has some; a field that no encoder writes may index up to 2^ib / 2
+  // entries: what that reaches lies in the block's shared memory, too)
   const size_t any = (size_t)4 << p.ib;
-  auto need = [&](int rk, int rv) { return std::max(rings + (table << rk) + (table << rv), std::max(any << rk, (table << rk) + (any << rv))); };
+  size_t tk = table, tv = table;
+  p.ext = outl && has_ext(p.ib) && compiled_fields(p.ib, a->K.radius_bits) && table + (size_t)warps * kExtK * 8 <= any;
+  if (p.ext) { tk += (size_t)warps * kExtK * 8; tv += (size_t)warps * kExtV * 8; }
+  auto need = [&](int rk, int rv) { return std::max(rings + (tk << rk) + (tv << rv), std::max(any << rk, (tk << rk) + (any << rv))); };
   auto fits = [&](int rk, int rv) { return rk <= 4 && rv <= 4 && need(rk, rv) <= kSmemMax; };
+  if (p.ext && !fits(0, 0)) { p.ext = 0; tk = tv = table; }
   if (!fits(0, 0)) return HQMQ_ERR_UNSUPPORTED;
   // (replicas of the tables against bank conflicts, K first)
   for (bool more = true; more;) {

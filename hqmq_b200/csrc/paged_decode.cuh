@@ -25,10 +25,28 @@ struct DecodeParams {
   float qmaxf, vfac;             // 1 / qmax
   int sdt, pay_bf16;             // type of the scales; whether the flagged chunks' values are bf16 (else fp16)
   const int4* seqs; const int4* units; const int* base; const int* warps; const int4* cuts; const int* tabs; const int* hdr;
-  int ctas, fused;               // fused: the CTAs of a head are a cluster
+  int ctas, fused, ext;          // fused: the CTAs of a head are a cluster; ext: the tables have entries of every warp's own
   float* parts;                  // [CTA][warps][2][part], then [CTA][2][part]
   uint2* wide;                   // [CTA][warps][K, V][16 N]: values of a tile with more flagged chunks than a stage holds
 };
+
+// Values of flagged chunks as table entries: where the index bits of a field leave room behind the codebook (2^(bits - 1) sign-folded
+// entries; 896 of them at S = 96, 1792 at 192), every warp has this many entries of K's table and of V's to itself.
+constexpr int kExtK = 36, kExtV = 24;
+__host__ __device__ constexpr bool has_ext(int ib) { return ib == 12 || ib == 13; }
+// Field c of a row: IB + RB bits, the row's words the writing lane's own.
+template <int IB, int RB>
+__device__ __forceinline__ void put_field(unsigned char* row, int c, uint32_t v) {
+  constexpr int CB = IB + RB;
+  if constexpr (CB == 16) reinterpret_cast<uint16_t*>(row)[c] = (uint16_t)v;
+  else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(row) + ((c * CB) >> 5);
+    const int sh = (c * CB) & 31;
+    constexpr uint32_t mask = (1u << CB) - 1u;
+    w[0] = (w[0] & ~(mask << sh)) | (v << sh);
+    if (sh + CB > 32) w[1] = (w[1] & ~(mask >> (32 - sh))) | (v >> (32 - sh));
+  }
+}
 
 template <int N, int NB> __host__ __device__ constexpr int part_floats() { return NB * (N / 4 * 128 + 16); }
 
@@ -94,18 +112,20 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   using FL = FastLoader<N, IB ? IB : 12, IB ? RB : 4, true>;
   constexpr int NKS = Geo<N>::NKS, NVG = Geo<N>::NVG, NOT = 2 * NVG;
   constexpr int NW = NB == 1 ? kDecWarps : kDecWarpsWide, THREADS = NW * 32, PART = part_floats<N, NB>();
+  const bool ext = OUTL && has_ext(IB) && p.ext != 0;
   const int ROW = IB ? row_bytes_of<N, IB, RB>() : p.row_bytes;
   const TileLayout L = tile_layout(ROW, true, OUTL);
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const uint32_t strideK = 8u << p.repk, strideV = 8u << p.repv;
   unsigned char* tblK = smem_raw;
-  unsigned char* tblV = smem_raw + (size_t)(p.table_rows >> 1) * strideK;
+  unsigned char* tblV = smem_raw + (size_t)((p.table_rows >> 1) + (ext ? NW * kExtK : 0)) * strideK;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 3, r = lane >> 2;
-  unsigned char* ring = tblV + (size_t)(p.table_rows >> 1) * strideV + (size_t)warp * kTileStages * L.bytes;
+  unsigned char* rings = tblV + (size_t)((p.table_rows >> 1) + (ext ? NW * kExtV : 0)) * strideV;
+  unsigned char* ring = rings + (size_t)warp * kTileStages * L.bytes;
   const uint32_t ring32 = smem_u32(ring);
   // (of 32 rows, a warp's queries are 8 KB in shared memory, as the fragments that a lane reads: registers hold the accumulators)
   constexpr bool QREG = NB <= 2;
-  uint2* q_s = reinterpret_cast<uint2*>(tblV + (size_t)(p.table_rows >> 1) * strideV + (size_t)NW * kTileStages * L.bytes + kPastPay) + warp * (NKS * NB * 32);
+  uint2* q_s = reinterpret_cast<uint2*>(rings + (size_t)NW * kTileStages * L.bytes + kPastPay) + warp * (NKS * NB * 32);
   grid_dep_launch();
   const int h = (int)blockIdx.x / p.ctas, k = (int)blockIdx.x - h * p.ctas;
   const int n_units = p.hdr[0], total = p.hdr[1], n_warps = p.ctas * NW;
@@ -189,21 +209,6 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       const int t0 = tile * kTile;
       const bool edge = t0 + kTile > p_first + 1 || t0 < edge_lo;
 
-      // ---- this lane's fields, scales and flags ------------------------------------------------------------------------------
-      uint32_t kw[2][FL::KW + 1], vw[4][FL::VW + 1];
-      float ksc[2], vsc[2];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const int t = nt * 8 + r;
-        if constexpr (IB != 0) ld.template load_span<FL::KW, FL::LK>(kw[nt], sp + t * ROW, j, true);
-        ksc[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt);
-        vsc[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsv)[t], p.sdt) * p.vfac;
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int t = 2 * j + ((x & 1) ^ vswz) + (x >> 1) * 8;
-        if constexpr (IB != 0) ld.template load_span<FL::VW, FL::LV>(vw[x], sp + L.v + t * ROW, r, !edge || t0 + t < s.kv);
-      }
       uint32_t kcols = 0u, vcols = 0u;       // the columns of chunks in which some token of the tile has a flagged one
       uint32_t fl = 0u, before = 0u;         // lanes 0..15: K's tokens, 16..31: V's: flags, and entries of the tile's earlier tokens
       bool wide = false;
@@ -214,22 +219,37 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         if (kcols | vcols) {
           const uint32_t own = __popc(fl);
           before = counts_before(own, lane);
-          wide = __any_sync(0xffffffffu, before + own > (lane < 16 ? kPayK : kPayV));
+          wide = __any_sync(0xffffffffu, before + own > (uint32_t)(lane < 16 ? (ext ? kExtK : kPayK) : (ext ? kExtV : kPayV)));
           // every lane its token's values, in place
           const float rs = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[lane], p.sdt);
           const float inv = rs != 0.f ? __fdividef(p.qmaxf, rs) : 0.f;
           const bool bf = p.pay_bf16 != 0;
           auto operand = [&](uint2 v) { return make_uint2(scaled_pair(v.x, inv, bf), scaled_pair(v.y, inv, bf)); };
-          if (!wide) {
-            uint2* e = reinterpret_cast<uint2*>(sp + L.pay + (lane < 16 ? 0 : kPayK * 8)) + before;
+          uint2* e = reinterpret_cast<uint2*>(sp + L.pay + (lane < 16 ? 0 : kPayK * 8)) + before;
+          if (ext && !wide) {
+            // Entries behind the codebook are this warp's: the value goes where the lane that decodes the chunk will look, and the chunk's
+            // field in the staged row becomes that entry's, times one.
+            const bool of_v = lane >= 16;
+            const int tok = lane & 15;
+            uint32_t entry = (uint32_t)(p.table_rows >> 1) + (of_v ? warp * kExtV : warp * kExtK) + before;
+            const uint32_t stride = of_v ? strideV : strideK, mask = (stride >> 3) - 1u;
+            uint32_t dst = (of_v ? (uint32_t)(tblV - smem_raw) : 0u) + entry * stride;
+            unsigned char* row = sp + (of_v ? L.v : 0) + tok * ROW;
+            for (uint32_t m = fl; m; m &= m - 1u, ++e, ++entry, dst += stride) {
+              const int c = __ffs(m) - 1;
+              const uint32_t reader = of_v ? (uint32_t)((c / NVG) << 2 | (tok & 7) >> 1) : (uint32_t)((tok & 7) << 2 | c / NKS);
+              *reinterpret_cast<uint2*>(smem_raw + dst + ((reader & mask) << 3)) = operand(*e);
+              if constexpr (has_ext(IB)) put_field<IB, RB>(row, c, entry << 1 | 1u << IB);
+            }
+          } else if (!wide) {
             for (uint32_t x = 0; x < own; ++x, ++e) *e = operand(*e);
           } else {
             const int64_t ph = *reinterpret_cast<const int*>(sp + L.off + 16);
             const hqmq_packed& pk = lane < 16 ? p.pool.K : p.pool.V;
-            uint2* e = my_wide() + (lane < 16 ? 0 : 16 * N) + before;
+            uint2* far = my_wide() + (lane < 16 ? 0 : 16 * N) + before;
             uint32_t from = reinterpret_cast<const uint32_t*>(sp + L.off)[lane < 16 ? 0 : 2] + before;
-            for (uint32_t x = 0; x < own; ++x, ++e, ++from)
-              *e = operand(from < (uint32_t)pk.out_cap ? __ldg(reinterpret_cast<const uint2*>(pk.out_vals) + ph * pk.out_cap + from) : make_uint2(0u, 0u));
+            for (uint32_t x = 0; x < own; ++x, ++far, ++from)
+              *far = operand(from < (uint32_t)pk.out_cap ? __ldg(reinterpret_cast<const uint2*>(pk.out_vals) + ph * pk.out_cap + from) : make_uint2(0u, 0u));
           }
           __syncwarp();
         }
@@ -246,6 +266,21 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         }
       };
 
+      // ---- this lane's fields and scales ------------------------------------------------------------------------------
+      uint32_t kw[2][FL::KW + 1], vw[4][FL::VW + 1];
+      float ksc[2], vsc[2];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int t = nt * 8 + r;
+        if constexpr (IB != 0) ld.template load_span<FL::KW, FL::LK>(kw[nt], sp + t * ROW, j, true);
+        ksc[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt);
+        vsc[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsv)[t], p.sdt) * p.vfac;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = 2 * j + ((x & 1) ^ vswz) + (x >> 1) * 8;
+        if constexpr (IB != 0) ld.template load_span<FL::VW, FL::LV>(vw[x], sp + L.v + t * ROW, r, !edge || t0 + t < s.kv);
+      }
       // ---- S^T = K Q^T ---------------------------------------------------------------------------------------------------------
       float sc[NB][4], s2[NB][4];
 #pragma unroll
@@ -278,7 +313,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       // left out.  A column per group of lanes at a time, which takes fewer products, pays where the queries are in shared memory: picked from
       // registers by selects it took 145 instructions a tile, 339 us against 317; of 32 rows it takes 88 us against 102 for 8 x 8111.)
       if constexpr (OUTL) {
-        if (kcols) {
+        if (kcols && (!ext || wide)) {
           uint32_t f[2], at[2];
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) {
@@ -425,7 +460,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       });
       // ... of V: two more products for every g that has some
       if constexpr (OUTL) {
-        if (vcols) {
+        if (vcols && (!ext || wide)) {
           uint32_t f[4], at[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -563,6 +598,8 @@ struct DecodeKernels { const void* decode; const void* merge; };
 DecodeKernels decode_kernels_128(int ib, int rb, int nb, bool outl);
 DecodeKernels decode_kernels_64(int ib, int rb, int nb, bool outl);
 
+// Field widths that have kernels of their own.
+inline bool compiled_fields(int ib, int rb) { return (ib == 10 && rb == 3) || (ib == 12 && rb == 4) || (ib == 13 && rb == 6); }
 template <int N, int NB, bool OUTL>
 const void* pick_decode(int ib, int rb) {
   if (ib == 10 && rb == 3) return (const void*)&paged_decode_kernel<N, 10, 3, NB, OUTL>;

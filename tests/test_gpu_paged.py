@@ -208,7 +208,7 @@ def test_store_over_a_full_side_buffer_counts_and_drops():
 
 
 # ---- attention ------------------------------------------------------------------------------------------------------------------------
-FORMS = [(2, 4, 128, 96, 4), (1, 7, 128, 192, 6), (2, 8, 64, 96, 4), (3, 1, 128, 24, 3), (1, 16, 64, 24, 3), (2, 5, 128, 48, 5), (1, 3, 64, 192, 6)]
+FORMS = [(2, 4, 128, 96, 4), (1, 7, 128, 192, 6), (2, 8, 64, 96, 4), (3, 1, 128, 24, 3), (1, 16, 64, 24, 3), (2, 5, 128, 48, 5), (1, 3, 64, 192, 6), (1, 4, 64, 160, 4), (1, 2, 128, 256, 6)]
 
 
 @pytest.mark.parametrize("H,G,d,S,rb", FORMS)
