@@ -209,16 +209,18 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       const int t0 = tile * kTile;
       const bool edge = t0 + kTile > p_first + 1 || t0 < edge_lo;
 
-      uint32_t kcols = 0u, vcols = 0u;       // the columns of chunks in which some token of the tile has a flagged one
+      uint32_t kcols = 0u, vcols = 0u;       // the columns of chunks that have a flagged one in some token, where those are products of their own
       uint32_t fl = 0u, before = 0u;         // lanes 0..15: K's tokens, 16..31: V's: flags, and entries of the tile's earlier tokens
       bool wide = false;
       if constexpr (OUTL) {
         if (t0 + (lane & 15) < s.kv && (lane < 16 ? p.pool.K.flags : p.pool.V.flags)) fl = reinterpret_cast<const uint32_t*>(sp + L.flk)[lane];
-        kcols = __reduce_or_sync(0xffffffffu, lane < 16 ? fl : 0u);
-        vcols = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : fl);
-        if (kcols | vcols) {
+        if (__any_sync(0xffffffffu, fl != 0u)) {
           const uint32_t own = __popc(fl);
           before = counts_before(own, lane);
+          if (!ext) {
+            kcols = __reduce_or_sync(0xffffffffu, lane < 16 ? fl : 0u);
+            vcols = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : fl);
+          }
           wide = __any_sync(0xffffffffu, before + own > (uint32_t)(lane < 16 ? (ext ? kExtK : kPayK) : (ext ? kExtV : kPayV)));
           // every lane its token's values, in place
           const float rs = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[lane], p.sdt);
@@ -235,15 +237,27 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
             const uint32_t stride = of_v ? strideV : strideK, mask = (stride >> 3) - 1u;
             uint32_t dst = (of_v ? (uint32_t)(tblV - smem_raw) : 0u) + entry * stride;
             unsigned char* row = sp + (of_v ? L.v : 0) + tok * ROW;
-            for (uint32_t m = fl; m; m &= m - 1u, ++e, ++entry, dst += stride) {
-              const int c = __ffs(m) - 1;
-              const uint32_t reader = of_v ? (uint32_t)((c / NVG) << 2 | (tok & 7) >> 1) : (uint32_t)((tok & 7) << 2 | c / NKS);
-              *reinterpret_cast<uint2*>(smem_raw + dst + ((reader & mask) << 3)) = operand(*e);
-              if constexpr (has_ext(IB)) put_field<IB, RB>(row, c, entry << 1 | 1u << IB);
-            }
+            // (the lane that decodes it: K (token & 7) * 4 + chunk / NKS, V chunk / NVG * 4 + (token & 7) / 2)
+            constexpr int kLog = NKS == 8 ? 3 : 2, vLog = NVG == 4 ? 2 : 1;
+            const uint32_t rd0 = of_v ? (uint32_t)(tok & 7) >> 1 : (uint32_t)(tok & 7) << 2;
+            const int down = of_v ? vLog : kLog, up = of_v ? 2 : 0;
+            auto place = [&](auto bf_c) {
+              constexpr bool BF = decltype(bf_c)::value;
+              for (uint32_t m = fl; m; m &= m - 1u, ++e, ++entry, dst += stride) {
+                const int c = __ffs(m) - 1;
+                const uint2 v = *e;
+                *reinterpret_cast<uint2*>(smem_raw + dst + (((rd0 | (uint32_t)(c >> down) << up) & mask) << 3)) =
+                    make_uint2(scaled_pair(v.x, inv, BF), scaled_pair(v.y, inv, BF));
+                if constexpr (has_ext(IB)) put_field<IB, RB>(row, c, entry << 1 | 1u << IB);
+              }
+            };
+            if (bf) place(std::true_type{});
+            else place(std::false_type{});
           } else if (!wide) {
             for (uint32_t x = 0; x < own; ++x, ++e) *e = operand(*e);
           } else {
+            kcols = __reduce_or_sync(0xffffffffu, lane < 16 ? fl : 0u);
+            vcols = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : fl);
             const int64_t ph = *reinterpret_cast<const int*>(sp + L.off + 16);
             const hqmq_packed& pk = lane < 16 ? p.pool.K : p.pool.V;
             uint2* far = my_wide() + (lane < 16 ? 0 : 16 * N) + before;
@@ -313,7 +327,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       // left out.  A column per group of lanes at a time, which takes fewer products, pays where the queries are in shared memory: picked from
       // registers by selects it took 145 instructions a tile, 339 us against 317; of 32 rows it takes 88 us against 102 for 8 x 8111.)
       if constexpr (OUTL) {
-        if (kcols && (!ext || wide)) {
+        if (kcols) {
           uint32_t f[2], at[2];
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) {
@@ -460,7 +474,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       });
       // ... of V: two more products for every g that has some
       if constexpr (OUTL) {
-        if (vcols && (!ext || wide)) {
+        if (vcols) {
           uint32_t f[4], at[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {

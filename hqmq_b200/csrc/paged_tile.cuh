@@ -165,15 +165,15 @@ __device__ __forceinline__ float4 values_of(uint2 v, int dtype) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// Sum over the lanes before this one in its half of the warp.
+// Sum over the lanes before this one in its half of the warp, of counts up to 32: by their bits, of which two hardly ever do not do.
 __device__ __forceinline__ uint32_t counts_before(uint32_t own, int lane) {
-  uint32_t x = own;
+  const uint32_t earlier = ((1u << lane) - 1u) & (lane < 16 ? 0xffffu : 0xffff0000u);
+  uint32_t n = __popc(__ballot_sync(0xffffffffu, own & 1u) & earlier) + 2u * __popc(__ballot_sync(0xffffffffu, own & 2u) & earlier);
+  if (__any_sync(0xffffffffu, own > 3u)) {
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o, 16);
-    if ((lane & 15) >= o) x += y;
+    for (int b = 2; b < 6; ++b) n += (uint32_t)__popc(__ballot_sync(0xffffffffu, own & (1u << b)) & earlier) << b;
   }
-  return x - own;
+  return n;
 }
 
 // The codeword and radius of field `c` of a row of `cb`-bit fields (sign-folded index, the sign in the radius).
