@@ -94,7 +94,7 @@ class World:
             at += n
         self.free = order[at:]
         q = hqmq.HQMQ(1, H, S, rb, device=DEV)
-        self.inner, self.quant = q, hqmq.with_outlier_extraction(q, C=3.0) if outliers else q
+        self.inner, self.quant = q, hqmq.with_outlier_extraction(q, C=outliers if isinstance(outliers, float) else 3.0) if outliers else q
         self.pool = hqmq.PagedKV(self.n_pages, H, d, S, rb, DEV, page_tokens=page, dtype=dtype, outliers_K=bool(outliers),
                                  outliers_V=bool(outliers), out_cap=page * d // 4 if out_cap is None else out_cap)
         if garbage:        # recycled pages: rows, scales that are no number, flags, offsets and counts of an earlier life
@@ -344,6 +344,22 @@ def test_pages_behind_four_gigabytes():
         for h in range(H):
             rows = [pool.K.pages("codes")[tables[s][t // 64], h, t % 64] for t in kept[s, h, :n].tolist()]
             assert torch.equal(torch.stack(rows), torch.cat([pool.K.pages("codes")[p, h] for p in dst[s]])[:n])
+
+
+@pytest.mark.parametrize("d,S,rb", [(128, 96, 4), (64, 96, 4), (128, 192, 6), (128, 24, 3), (128, 128, 4)])
+@pytest.mark.parametrize("C", [0.7, 1.1, 1.5])
+def test_tiles_full_of_outliers(d, S, rb, C):
+    """Far more flagged chunks in a tile than are staged, or have table entries: up to all of them, in K and V."""
+    w = World(1, d, S, rb, [300, 90, 17], rounds=1, outliers=C, kind="randn")
+    for q_lens in ([1, 1, 1], [8, 3, 1], [40, 90, 17]):
+        q = queries(w, q_lens, 4, torch.bfloat16)
+        check_attend(w, hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab), q, q_lens, 4)
+    q = queries(w, [1, 5, 1], 4, torch.bfloat16)
+    mass = hqmq.paged_attention_mass(q.to(DEV), w.pool, w.batch([1, 5, 1], 4), w.tab[0])
+    K, V = w.dense()
+    _, m, _, bound = attend64(q[1:6], K[1], V[1], 4, None, None, None, d ** -0.5)
+    got = torch.cat([mass[p] for p in w.tables[1]], 1)[:, :90].cpu().double()
+    assert bool(((got - m).abs() <= bound + m * (2.0 ** -20 + 20 * 2.0 ** -24)).all())
 
 
 def test_sinks_of_any_type_and_size():
