@@ -163,19 +163,22 @@ class PagedKVCache:
 
     def evict(self, seqs: Sequence[int], keep: int, first: int = 4, last: int = 16) -> Dict[int, torch.Tensor]:
         """Cut sequences of more than ``keep`` tokens down to it, in every layer by the layer's own weights (all layers have some: see
-        ``weigh``).  Returns {layer: positions that stayed}, see ``paged_evict``; ends the step."""
+        ``weigh``).  Returns {layer: positions that stayed}, see ``paged_evict``; ends the step.  What stays is numbered anew: a layer's
+        sliding window counts tokens that are held."""
         self._known(seqs)
+        if first < 0 or last < 0:
+            raise ValueError(f"first={first}, last={last}: counts of tokens")
         if keep < first + last:
             raise ValueError(f"keep={keep}: at least the {first} first and {last} last tokens stay")
         missing = [layer for layer in self._pools if layer not in self._mass]
         if missing:
             raise _lib.HqmqError(f"hqmq_b200: no weights of layers {missing} (weigh() first)")
         cut = [int(i) for i in seqs if self._len[i] > keep]
+        per = -(-keep // self.page_tokens)
+        pages = self._take(per * len(cut)) if self._pools else []      # (raises with nothing changed)
         self._step, self._batches = None, {}
         if not cut or not self._pools:
             return {}
-        per = -(-keep // self.page_tokens)
-        pages = self._take(per * len(cut))
         tables = [pages[per * k:per * (k + 1)] for k in range(len(cut))]
         any_pool = next(iter(self._pools.values()))
         old = PagedBatch(any_pool, [self._table[i] for i in cut], [self._len[i] for i in cut])

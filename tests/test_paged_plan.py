@@ -231,6 +231,28 @@ def test_calls_refuse_host_memory():
             call()
 
 
+def test_a_cache_that_refuses_is_unchanged():
+    cache, pool = hqmq.PagedKVCache(None, 8), make_pool()
+    a, b = cache.add(2)
+    cache.begin([a, b], [200, 64])                                       # 4 pages, 1 page
+    assert cache.free_pages == 3
+    for call, error in ((lambda: cache.begin([a], [300]), _lib.HqmqError), (lambda: cache.begin([a, a], [1, 1]), ValueError),
+                        (lambda: cache.begin([7], [1]), KeyError), (lambda: cache.begin([a], [-1]), ValueError),
+                        (lambda: cache.evict([a], keep=10), ValueError), (lambda: cache.drop([a, 9]), KeyError)):
+        with pytest.raises(error):
+            call()
+    cache._pools[0], cache._mass[0] = pool, pool.new_mass()
+    for kw, error in (({"first": -1}, ValueError), ({"last": -4}, ValueError), ({"first": 40, "last": 41}, ValueError)):
+        with pytest.raises(error):
+            cache.evict([a], keep=80, **kw)
+    cache.begin([b], [128])                                              # one page left
+    with pytest.raises(_lib.HqmqError):
+        cache.evict([a], keep=80)                                        # wants two
+    assert cache.free_pages == 1 and cache.length(a) == 200 and cache.length(b) == 192 and cache._step == ([b], [128])
+    cache.drop([a, b])
+    assert cache.free_pages == 8
+
+
 def _args(pool, batch, G=2):
     a = _lib.PagedAttnArgs(struct_size=C.sizeof(_lib.PagedAttnArgs), q_dtype=_lib.BF16, o_dtype=_lib.BF16, r_qmax=7, softmax_scale=0.1)
     a.Q = a.O = a.plan_data = a.table_K = a.table_V = a.mass = 1 << 20
