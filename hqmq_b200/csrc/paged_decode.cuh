@@ -1,12 +1,20 @@
 // Attention of a few query rows per sequence over a paged cache: the kernel.
 //
 // The tile's arithmetic is that of the staged decode kernels (attn_kernel.cuh): S^T = K Q^T with the 16 tokens as rows and the query
-// rows as columns, O^T += V^T P^T, operands gathered from shared-memory tables straight into fragments.  What differs: a warp walks
-// its own stretch of tiles from unit to unit (paged.cuh); flagged chunks, which decode to zero, are products of their own behind the
-// others': a lane per token turns its values into fp16(x * qmax / rs), what the table would have given, and a lane, which owns 2 tokens
-// x N / 4 chunks of K and 4 x N / 8 of V, finds its own in the side buffer's order by counting the flags before them; V's scales enter P
-// relative to the largest one seen, a power of two that the accumulators are rescaled by like by the maximum, so that values of any size
-// keep their bits.
+// rows as columns, O^T += V^T P^T, operands gathered from shared-memory tables straight into fragments.  What differs:
+//   - a warp walks its own stretch of tiles from unit to unit (paged.cuh);
+//   - flagged chunks, whose fields decode to zero.  A lane per token turns its values into fp16(x * qmax / rs), what the table would have given.
+//     Where the index bits of a field leave room behind the codebook, the values become table entries of the warp's own and the fields of the
+//     staged row point to them, so the look-ups below find them and nothing branches on a flag.  Where they do not (13-bit fields, codebooks
+//     without room, fields of any width), or a tile has more than the warp has entries, they are products of their own behind
+//     the others': a lane, which owns 2 tokens x N / 4 chunks of K and 4 x N / 8 of V, finds its values by counting the flags before them.
+//     (16 sequences of 16 to 32 k tokens, two outlier channels a head in K: values put into the fragments by branches 381 us, products of
+//     their own 316, table entries 268; 169 without outliers.  Repeated passes of the main products for a tile with too many, in place of the
+//     products of their own, took 277 to 299; without either the kernel would take 254);
+//   - V's scales enter P relative to the largest one seen, a power of two that the accumulators are rescaled by like by the maximum, so
+//     that values of any size keep their bits.
+// What bounds it: instructions, 1013 a tile with those outliers and 680 without, at 61 to 62 % of the issue slots (chains of look-up,
+// multiply, product in 16 warps of 128 registers).
 #pragma once
 #include "attn_tma.cuh"
 #include "paged_tile.cuh"
@@ -322,7 +330,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         }
       });
 
-      // Flagged chunks of K: one more product for every step of the others' that has some.  (Put into the fragments above instead, the
+      // Flagged chunks of K that are no table entries: one more product for every step of the others' that has some.  (Put into the fragments above instead, the
       // branches of every step kept the look-ups from being issued ahead: 381 us against 170 without outliers for 16 x 32k, 287 with that part
       // left out.  A column per group of lanes at a time, which takes fewer products, pays where the queries are in shared memory: picked from
       // registers by selects it took 145 instructions a tile, 339 us against 317; of 32 rows it takes 88 us against 102 for 8 x 8111.)
