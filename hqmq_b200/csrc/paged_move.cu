@@ -20,7 +20,8 @@ __device__ __forceinline__ uint32_t warp_before(uint32_t own, int lane) {       
 
 // ---- store -----------------------------------------------------------------------------------------------------------------------
 // blockIdx.x = (sequence, page among those its new tokens touch), y = KV head, z = tensor.  The tokens are neighbours in the staging
-// planes, so their flagged values are one run there and stay one run in the page.
+// planes, so their flagged values are one run there and stay one run in the page.  Tokens from the first of them on that the page held before are
+// gone: a store may begin anywhere in what was stored.
 struct StoreParams {
   hqmq_packed src[2], dst[2];
   const int4* seqs; const int* tabs;
@@ -47,7 +48,13 @@ __global__ void __launch_bounds__(128) paged_store_kernel(const StoreParams p) {
   if (!D.flags || threadIdx.x >= 32) return;
   const int lane = threadIdx.x;
   uint32_t* off = D.out_off + ph * (pt / HQMQ_OUT_BLOCK + 1);
-  const uint32_t held = a == 0 ? 0u : D.out_count[ph];
+  // Entries of the page's tokens before the first of these: by the block's offset and its flags, not by the page's counter, which still has
+  // tokens that the sequence no longer holds (drafted ones that were taken back, a step that is stored again).
+  uint32_t held = 0u;
+  if (a > 0) {
+    const int in_blk = a & (HQMQ_OUT_BLOCK - 1);
+    held = off[a / HQMQ_OUT_BLOCK] + __reduce_add_sync(0xffffffffu, lane < in_blk ? __popc(D.flags[drow - in_blk + lane]) : 0u);
+  }
   // entries of the staging tensor before the first of these tokens
   uint32_t from = 0u;
   if (S.flags) {

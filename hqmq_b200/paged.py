@@ -390,7 +390,9 @@ def paged_attention_mass(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, tabl
 
 def paged_store(pool: PagedKV, K: PackedKV, V: PackedKV, batch: PagedBatch) -> None:
     """Encoded keys and values (``HQMQ.encode`` of (1, H_kv, total_q, d), tokens in the order of the batch's queries) become the last
-    ``q_len`` tokens of their sequences.  Pages that are written belong to one sequence."""
+    ``q_len`` tokens of their sequences.  What the pages held from the first of them on is gone: a sequence whose drafted tokens were
+    rejected goes on with a batch of its shorter length, and storing a step twice stores it once.  Pages that are written belong to one
+    sequence."""
     _belongs(pool, batch, "paged_store")
     for name, src, dst in (("K", K, pool.K), ("V", V, pool.V)):
         if src.B != 1 or src.T < batch.total_q or (src.H, src.n_chunks, src.S, src.radius_bits) != (dst.H, dst.n_chunks, dst.S, dst.radius_bits):

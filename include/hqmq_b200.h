@@ -523,8 +523,9 @@ size_t hqmq_paged_mass_workspace_bytes(const hqmq_paged_attn_args* args);
 int hqmq_paged_mass(const hqmq_paged_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Encoded tokens go to their pages: the tokens of `src` (B = 1, T_cap >= total_q), in the order of the batch's queries, become
- * the last q_len tokens of their sequences.  A page's first token resets its side buffer; the pages written must belong to one
- * sequence each.  Entries beyond out_cap are dropped and counted, as in hqmq_encode. */
+ * the last q_len tokens of their sequences.  What their pages held from the first of them on is gone, so tokens may be stored
+ * again, and a sequence that got shorter (drafted tokens that were rejected) is written on from where it ends; the pages written must belong to
+ * one sequence each.  Entries beyond out_cap are dropped and counted, as in hqmq_encode. */
 typedef struct hqmq_paged_store_args {
   uint32_t struct_size;
   int32_t reserved;

@@ -729,3 +729,59 @@ def test_nothing_to_do():
     assert float(mass.sum()) == 0.5 * 130
     empty = hqmq.PagedBatch(w.pool, [[], []], [0, 0])
     assert hqmq.paged_evict(w.pool, hqmq.PagedBatch(w.pool, w.tables, w.kv), empty, mass, first=0, last=0).shape == (2, 1, 0)
+
+
+# ---- tokens that are stored again -------------------------------------------------------------------------------------------------------------
+def _same_contents(a, b, tables, kv):
+    """Two pools hold the same tokens: rows, scales, flags, offsets, counts and the entries that those reach."""
+    page = a.page_tokens
+    for x, y in zip((host(a.K), host(a.V)), (host(b.K), host(b.V))):
+        for t, n in zip(tables, kv):
+            for k, p in enumerate(t[:-(-n // page)]):
+                m = min(page, n - k * page)
+                for name in ("codes", "rs", "flags"):
+                    assert torch.equal(x[name][p, :, :m], y[name][p, :, :m]), name
+                assert torch.equal(x["out_count"][p], y["out_count"][p])
+                assert torch.equal(x["out_off"][p, :, :-(-m // 16) + 1], y["out_off"][p, :, :-(-m // 16) + 1])
+                for h in range(x["codes"].shape[1]):
+                    e = int(x["out_count"][p, h])
+                    assert torch.equal(x["out_vals"][p, h, :e], y["out_vals"][p, h, :e])
+
+
+@pytest.mark.parametrize("H,d,S,rb,page", [(2, 128, 96, 4, 64), (1, 64, 24, 3, 128)])
+@pytest.mark.parametrize("length,drafted,taken", [(96, 4, 2), (92, 4, 4), (94, 4, 2), (62, 4, 3), (60, 70, 66), (127, 1, 1), (64, 3, 3), (20, 4, 3)])
+def test_tokens_that_were_taken_back_leave_nothing(H, d, S, rb, page, length, drafted, taken):
+    """`drafted` tokens behind `length`, of which the last `taken` are rejected; others follow: a pool that never held them holds the same."""
+    q = hqmq.HQMQ(1, H, S, rb, device=DEV)
+    quant = hqmq.with_outlier_extraction(q, C=1.5)
+    pools = [hqmq.PagedKV(8, H, d, S, rb, DEV, page_tokens=page, outliers_K=True, outliers_V=True, out_cap=page * d // 4) for _ in (0, 1)]
+    tables = [[5, 2, 7, 1][:-(-(length + 4 + drafted) // page)], [0]]
+
+    def encoded(n, seed):
+        x = [make_kv("spiky", (1, H, n, d), seed + i, torch.bfloat16).to(DEV) for i in (0, 1)]
+        pair = [q.new_cache(1, n, d, DEV, scale_dtype=torch.bfloat16, with_outliers=True, out_dtype=torch.bfloat16) for _ in (0, 1)]
+        quant.encode_pair(*x, 0, *pair)
+        return pair
+
+    def store(pool, pair, kv, new):
+        hqmq.paged_store(pool, *pair, hqmq.PagedBatch(pool, tables, kv, new))
+
+    keep = drafted - taken
+    first, draft, other, more = encoded(length + 40, 1), encoded(drafted, 3), encoded(1, 5), encoded(3, 7)
+    for i, pool in enumerate(pools):
+        store(pool, first, [length, 40], [length, 40])
+        if i == 0:
+            for _ in (0, 1):                     # (the same step twice)
+                store(pool, draft, [length + drafted, 40], [drafted, 0])
+                store(pool, other, [length + drafted, 41], [0, 1])
+        else:
+            if keep:
+                store(pool, draft, [length + keep, 40], [keep, 0])
+            store(pool, other, [length + keep, 41], [0, 1])
+        store(pool, more, [length + keep + 2, 42], [2, 1])
+    kv = [length + keep + 2, 42]
+    _same_contents(*pools, tables, kv)
+    Q = torch.randn(2, 4 * H, d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    tab = [q.tables(0, i, DEV)["table16"] for i in (0, 1)]
+    a, b = (hqmq.paged_attention(Q, p, hqmq.PagedBatch(p, tables, kv, [1, 1], n_heads=4 * H), *tab) for p in pools)
+    assert torch.equal(a, b)
