@@ -785,3 +785,27 @@ def test_tokens_that_were_taken_back_leave_nothing(H, d, S, rb, page, length, dr
     tab = [q.tables(0, i, DEV)["table16"] for i in (0, 1)]
     a, b = (hqmq.paged_attention(Q, p, hqmq.PagedBatch(p, tables, kv, [1, 1], n_heads=4 * H), *tab) for p in pools)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("power", [16, 24, 32, 40, 90])
+@pytest.mark.parametrize("q_lens", [[1, 1], [60, 33]])
+def test_scores_that_no_exponential_holds(power, q_lens):
+    """Scores up to 2^95: the largest one takes the weight."""
+    w = World(1, 128, 96, 4, [200, 90])
+    q = (queries(w, q_lens, 4, torch.bfloat16).float() * 2.0 ** power).to(torch.bfloat16)
+    out = hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab)
+    assert bool(out.isfinite().all())
+    check_attend(w, out, q, q_lens, 4)
+    # a key that is far ahead of the others: its value, alone
+    K, V = w.dense()
+    at = 0
+    for s, n in enumerate(q_lens):
+        score = torch.einsum("ihd,td->iht", q[at:at + n].double(), K[s][0])
+        score = score.masked_fill(torch.arange(w.kv[s]) > torch.arange(n).view(-1, 1, 1) + w.kv[s] - n, -math.inf)
+        size = torch.einsum("ihd,td->iht", q[at:at + n].double().abs(), K[s][0].abs()).amax(-1)
+        top = score.topk(2, -1)
+        sure = (top.values[..., 0] - top.values[..., 1] > size * 2.0 ** -9) & (top.values[..., 1] > -math.inf)
+        want = V[s][0][top.indices[..., 0]]
+        off = (out[at:at + n].cpu().double() - want).abs()
+        assert bool(sure.any()) and bool((off <= want.abs() * (2.0 ** -8 + 2.0 ** -9) + V[s].abs().amax() * 2.0 ** -24)[sure].all())
+        at += n
