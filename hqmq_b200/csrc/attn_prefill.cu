@@ -407,8 +407,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
     constexpr int QL = D / 8, QR = 32 / QL;      // lanes per row, rows per warp-wide load
     const int c_q = lane % QL;
     const uint32_t g_inv = 65536u / (uint32_t)p.G + 1u;                   // rw / G = rw * g_inv >> 16 for rw < 128
-    // Ragged batches: queries of any size, relative to a power of two per warp (which owns the rows it loads); returns that power.  Two
-    // passes, the largest and then the values, the second out of the L1 cache.
+    // Ragged batches: queries of any size, every row relative to a power of two of its own (rows are other heads and tokens, and one that is
+    // far larger, or infinite, is no reason for the others to lose their bits); returns that of this lane's row.
     auto load_q_scaled = [&](const PfPiece& w) {
       const PfRows u = pf_rows<MODE>(p, w.bh, w.m);
       const int tq0 = (u.m * p.streams + s) * p.P, n_pos = min(p.P, u.Tq - tq0), rw0 = (warp & 3) * 32 + lane / QL;
@@ -416,58 +416,39 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
       const bool bf = p.q_dtype == HQMQ_BF16;
       const uint4* qp = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.Q) + qb);
       const int st_h = (int)(p.qs_h >> 3), st_t = (int)(p.qs_t >> 3);
-      auto fetch = [&](uint4* v, int k0) {         // eight pieces of 16 bytes on their way
+      float mine = 1.f;
+      // the row's largest value, over the QL lanes that have it, as a power of two: what it is divided by (kept by the lane of the row)
+      auto divisor = [&](int k, float big) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int rw = rw0 + (k0 + k) * QR, pw = (int)((uint32_t)rw * g_inv >> 16), gw = rw - pw * p.G;
-          v[k] = make_uint4(0u, 0u, 0u, 0u);
-          if (pw < n_pos) v[k] = __ldg(qp + (gw * st_h + pw * st_t));
-        }
-      };
-      auto slow = [&](int k, float* f) {           // any strides, any type
-        const int rw = rw0 + k * QR, pw = (int)((uint32_t)rw * g_inv >> 16), gw = rw - pw * p.G;
-        const int64_t o = qb + (int64_t)gw * p.qs_h + (int64_t)pw * p.qs_t;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = pw < n_pos ? load_float(p.Q, o + e, p.q_dtype) : 0.f;
+        for (int o = 1; o < QL; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        const int e2 = min(126, max(-126, (int)(__float_as_uint(big) >> 23) - 127));
+        const float power = __uint_as_float((uint32_t)(127 + e2) << 23), of_lane = __shfl_sync(0xffffffffu, power, (lane % QR) * QL);
+        if (lane / QR == k) mine = of_lane;
+        return __uint_as_float((uint32_t)(127 - e2) << 23);
       };
       auto put = [&](int k, uint4 v) {
         const int rw = rw0 + k * QR;
         const uint32_t dst = sQ + s * TB + rw * 128 + (c_q >> 3) * 16384 + (((c_q & 7) ^ (rw & 7)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
       };
-      float big = 0.f;
-      if (p.q_vec) {
-        uint32_t mx = 0u;                          // (the bits of 16-bit sizes order like their values)
-#pragma unroll 1
-        for (int k0 = 0; k0 < QL; k0 += 8) {
-          uint4 v[8];
-          fetch(v, k0);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu), __vmaxu2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu)));
-        }
-        big = fmaxf(bits16_to_float((uint16_t)mx, p.q_dtype), bits16_to_float((uint16_t)(mx >> 16), p.q_dtype));
-      } else {
-#pragma unroll 1
-        for (int k = 0; k < QL; ++k) {
-          float f[8];
-          slow(k, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(f[e]));
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-      const int e2 = min(100, max(-100, (int)(__float_as_uint(big) >> 23) - 127));
-      const float mul = __uint_as_float((uint32_t)(127 - e2) << 23);
       if (p.q_vec) {
 #pragma unroll 1
-        for (int k0 = 0; k0 < QL; k0 += 8) {
+        for (int k0 = 0; k0 < QL; k0 += 8) {         // eight pieces of 16 bytes on their way
           uint4 v[8];
-          fetch(v, k0);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int rw = rw0 + (k0 + k) * QR, pw = (int)((uint32_t)rw * g_inv >> 16), gw = rw - pw * p.G;
+            v[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (pw < n_pos) v[k] = __ldg(qp + (gw * st_h + pw * st_t));
+          }
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             uint32_t* w4 = reinterpret_cast<uint32_t*>(&v[k]);
+            uint32_t mx = 0u;                        // (the bits of 16-bit sizes order like their values)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = __vmaxu2(mx, w4[e] & 0x7fff7fffu);
+            mx = max(mx & 0xffffu, mx >> 16);
+            const float mul = divisor(k0 + k, bits16_to_float((uint16_t)mx, p.q_dtype));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 h2 = __half22float2(*reinterpret_cast<const __half2*>(&w4[e]));
@@ -476,18 +457,25 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_kernel(const Prefi
             put(k0 + k, v[k]);
           }
         }
-      } else {
+      } else {                                       // any strides, any type
 #pragma unroll 1
         for (int k = 0; k < QL; ++k) {
-          float f[8];
-          slow(k, f);
+          const int rw = rw0 + k * QR, pw = (int)((uint32_t)rw * g_inv >> 16), gw = rw - pw * p.G;
+          const int64_t o = qb + (int64_t)gw * p.qs_h + (int64_t)pw * p.qs_t;
+          float f[8], big = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[e] = pw < n_pos ? load_float(p.Q, o + e, p.q_dtype) : 0.f;
+            big = fmaxf(big, fabsf(f[e]));
+          }
+          const float mul = divisor(k, big);
           put(k, make_uint4(pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul), pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul)));
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(qfull + 8 * s);
-      return __uint_as_float((uint32_t)(127 + e2) << 23);
+      return mine;
     };
     auto load_q = [&](const PfPiece& w) {
       const PfRows rw_ = pf_rows<MODE>(p, w.bh, w.m);

@@ -183,10 +183,12 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
     const int b0 = un.b0, b1 = un.b1;
     const int rows = s.q * p.q.G;
     uint32_t qb[QREG ? NB : 1][NKS][2];
-    float qmul[NB];
+    float qmul[NB][2];                     // of this lane's two rows
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      qmul[nb] = load_query<NKS, true>(qb[QREG ? nb : 0], p.q, s.q_off, h, nb * 8 + r, rows, j) * kfac;
+      const float mul = load_query<NKS>(qb[QREG ? nb : 0], p.q, s.q_off, h, nb * 8 + r, rows, j) * kfac;
+      qmul[nb][0] = __shfl_sync(0xffffffffu, mul, 8 * j);
+      qmul[nb][1] = __shfl_sync(0xffffffffu, mul, 8 * j + 4);
       if constexpr (!QREG) {
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) q_s[(ks * NB + nb) * 32 + lane] = make_uint2(qb[0][ks][0], qb[0][ks][1]);
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sc[nb][x] = (sc[nb][x] + s2[nb][x]) * (ksc[x >> 1] * qmul[nb]);
+        for (int x = 0; x < 4; ++x) sc[nb][x] = (sc[nb][x] + s2[nb][x]) * (ksc[x >> 1] * qmul[nb][x & 1]);
       if (p.cap_log2 > 0.f) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)

@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
     float qmul[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float mul = load_query<NKS, false>(qb[0], p.q, s.q_off, h, row0 + nb * 8 + r, rows, j);
+      const float mul = load_query<NKS>(qb[0], p.q, s.q_off, h, row0 + nb * 8 + r, rows, j);
       if constexpr (!QREG) {
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) q_s[(ks * NB + nb) * 32 + lane] = make_uint2(qb[0][ks][0], qb[0][ks][1]);

@@ -206,9 +206,9 @@ __device__ __forceinline__ void load_table(unsigned char* tbl, const uint16_t* s
 struct QueryView { const void* Q; int dtype, vec; int64_t st_t, st_h; int G; };
 
 // Row `row` (query * G + head) of a unit, this lane's dims [4 NKS j, 4 NKS (j + 1)), in fp16 after division by a power of two that
-// brings the row's largest value to [1, 2); returns that power.  (SHARED: the largest of the warp's eight rows, one power for all.)  A
-// row that is not there is zeros.
-template <int NKS, bool SHARED>
+// brings the row's largest value to [1, 2); returns that power.  A power per row: rows are other heads and tokens, and one that is far
+// larger, or infinite, is no reason for the others to lose their bits.  A row that is not there is zeros.
+template <int NKS>
 __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& q, int q_off, int h, int row, int rows, int j) {
   float f[4 * NKS];
   const int qi = row / q.G, g = row - qi * q.G;
@@ -235,10 +235,6 @@ __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& 
   for (int i = 0; i < 4 * NKS; ++i) m = fmaxf(m, fabsf(f[i]));
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  if constexpr (SHARED) {
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  }
   int e = (int)(__float_as_uint(m) >> 23) - 127;               // (subnormal: -127; infinite: 128)
   e = min(126, max(-126, e));
   const float div = __uint_as_float((uint32_t)(127 - e) << 23);

@@ -809,3 +809,40 @@ def test_scores_that_no_exponential_holds(power, q_lens):
         off = (out[at:at + n].cpu().double() - want).abs()
         assert bool(sure.any()) and bool((off <= want.abs() * (2.0 ** -8 + 2.0 ** -9) + V[s].abs().amax() * 2.0 ** -24)[sure].all())
         at += n
+
+
+# ---- rows that have nothing to do with one another ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("d,q_dtype", [(128, torch.bfloat16), (64, torch.bfloat16), (128, torch.float32)])
+@pytest.mark.parametrize("q_lens", [[1, 1], [4, 8], [60, 33]])
+def test_queries_of_sizes_far_from_one_another(d, q_dtype, q_lens):
+    """Rows from 2^-40 to 2^110 side by side: every one has the bits that it would have alone."""
+    w = World(1, d, 96, 4, [200, 90])
+    q = queries(w, q_lens, 4, torch.bfloat16)
+    powers = torch.tensor([0, 20, -40, 3, 60, 0, 110, -1, 12])[torch.arange(4 * sum(q_lens)) % 9].view(-1, 4, 1)
+    q = (q.double() * 2.0 ** powers.double()).to(q_dtype)
+    view = torch.zeros(sum(q_lens), 4, d + 1, dtype=q_dtype)
+    view[..., 1:] = q
+    for x in (q.to(DEV), view.to(DEV)[..., 1:]):             # (wide loads, and an element at a time)
+        check_attend(w, hqmq.paged_attention(x, w.pool, w.batch(q_lens, 4), *w.tab), q, q_lens, 4)
+
+
+@pytest.mark.parametrize("q_dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("q_lens", [[1, 1], [4, 8], [60, 33]])
+def test_queries_that_are_no_numbers_spoil_their_own_rows_only(q_dtype, q_lens):
+    w = World(2, 128, 96, 4, [200, 90])
+    q = queries(w, q_lens, 4, q_dtype)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool)
+    for i, (row, head, value) in enumerate(((0, 1, math.inf), (-1, 6, -math.inf), (sum(q_lens) // 2, 4, math.nan))):
+        q[row, head, 5 + 30 * i] = value
+        bad[row, head] = True
+    out = hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab).cpu()
+    K, V = w.dense()
+    at = 0
+    for s, n in enumerate(q_lens):
+        clean = torch.where(bad[at:at + n, :, None], torch.zeros((), dtype=q_dtype), q[at:at + n])
+        o, _, bound, _ = attend64(clean, K[s], V[s], 4, None, None, None, 128 ** -0.5)
+        off = (out[at:at + n].double() - o).abs()
+        fine = off <= bound + o.abs() * (HALF[q_dtype] + 2.0 ** -18) + 1e-7
+        assert bool(fine[~bad[at:at + n]].all())
+        assert bool(out[at:at + n][bad[at:at + n]].isnan().all())
+        at += n
