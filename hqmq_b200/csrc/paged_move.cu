@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(512, 2) evict_move_kernel(const EvictParams p)
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int i = lane + 32 * x;
-    t[x] = i < n ? min(max(__ldg(kept + i), 0), src.x - 1) : 0;
+    t[x] = i < n ? min(max(__ldcg(kept + i), 0), src.x - 1) : 0;        // (written by the kernel ahead: never through the read-only path)
   }
 #pragma unroll
   for (int x = 0; x < 2; ++x) {

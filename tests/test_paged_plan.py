@@ -1,6 +1,8 @@
 """Plans of calls over a paged cache (host code), their refusals, and those of the calls, without a GPU."""
 import ctypes as C
+import os
 import random
+import re
 
 import numpy as np
 import pytest
@@ -294,3 +296,14 @@ def test_abi_refuses_pools_of_another_kind(built_lib):
         for k, v in change.items():
             setattr(a.plan, k, v)
         assert L.hqmq_paged_attn(C.byref(a), None, 0, None) in (-2, -8)
+
+
+def test_what_a_call_wrote_is_not_read_through_the_read_only_path():
+    """The second kernel of a call may start while the first still runs: what that one writes (kept positions, partial results, scores,
+    image scales) is no read-only memory, and a load that says so may be moved ahead of the wait."""
+    csrc = os.path.join(os.path.dirname(hqmq.__file__), "csrc")
+    written = re.compile(r"__ldg\((?:reinterpret_cast<[^()]*>\()?&?(?:[pe]\.)?(?:kept|parts|cta_parts|stats|scores|kmul|vmul|part|kimg|vimg|new_mass)\b")
+    assert written.search("__ldg(kept + i)") and written.search("__ldg(reinterpret_cast<const float4*>(p.scores) + 1)")
+    for name in os.listdir(csrc):
+        if name.startswith(("paged", "attn_prefill")):
+            assert not written.search(open(os.path.join(csrc, name)).read()), name
