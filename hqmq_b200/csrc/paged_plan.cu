@@ -85,8 +85,15 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
   const int most = std::max(1, HQMQ_PAGED_MAX_CTAS / p.H_kv);
   auto ctas = [&](int64_t tiles, int warps) { return (int)std::max<int64_t>(1, std::min<int64_t>(most, (tiles + 2 * warps - 1) / (2 * warps))); };
   const int W_ = dec_warps(p.dec_rows);
-  p.dec_ctas = ctas(dec_tiles, W_);
-  const int single = (int)std::min<int64_t>(1 << 20, (dec_tiles + W_ - 1) / W_);
+  // Of a plan with room, by the tiles that the room holds: the lengths that it is first made with do not bound those it will serve.  (A unit's
+  // tiles are its sequence's at most, and with a window the window's, the new tokens' and one cut at either end.)
+  const auto room_of = [&](int64_t units, int queries) {
+    const int64_t held = (int64_t)p.tab_room * (p.page_tokens / 16);
+    return p.window > 0 ? std::min(held, units * (((int64_t)p.window + queries) / 16 + 2)) : held;
+  };
+  const int64_t dec_most = p.tab_room && dec_units ? std::max(dec_tiles, room_of(dec_units, (dec_rows + G - 1) / G)) : dec_tiles;
+  p.dec_ctas = ctas(dec_most, W_);
+  const int single = (int)std::min<int64_t>(1 << 20, (dec_most + W_ - 1) / W_);
   if (single >= 1 && as_cluster(single, p.H_kv)) p.dec_ctas = single;
   // chunks
   p.ch_seqs = ch_seqs;
@@ -142,7 +149,7 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
     p.ch_ctas = p.ch_whole ? grid_w : (int)((total + L - 1) / L);
   }
   p.ms_units = (int)ms_units; p.ms_tiles = (int)ms_tiles; p.ms_groups = p.H_q ? (int)ms_groups : 0;
-  p.ms_ctas = (int)std::max<int64_t>(1, std::min<int64_t>(most, (ms_tiles + kMassWarps - 1) / kMassWarps));
+  int64_t ms_most = ms_tiles;
   p.ms_tile_room = p.ms_tiles; p.ms_group_room = p.ms_groups;
   if (p.tab_room) {
     if (n_tab > p.tab_room) return HQMQ_ERR_CAPACITY;
@@ -150,8 +157,10 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
     const int64_t blocks = blocks_of(most_rows, p.ms_rows), tiles = blocks * p.tab_room * (p.page_tokens / 16);
     if (tiles > (1 << 29)) return HQMQ_ERR_SHAPE;
     p.ms_tile_room = (int)tiles;
+    if (ms_units) ms_most = std::max(ms_tiles, std::min(tiles, blocks * room_of(ms_units, (p.ms_rows + G - 1) / G)));
     p.ms_group_room = p.H_q ? (int)((int64_t)p.tab_room * p.page_tokens / mass_group(p.ms_rows) + p.n_seqs) : 0;
   }
+  p.ms_ctas = (int)std::max<int64_t>(1, std::min<int64_t>(most, (ms_most + kMassWarps - 1) / kMassWarps));
   if (p.renew) {
     if (ch_units || had.ch_units) return HQMQ_ERR_UNSUPPORTED;
     if (had.dec_units != p.dec_units || had.dec_rows != p.dec_rows || had.ms_units != p.ms_units || had.ms_rows != p.ms_rows ||

@@ -307,3 +307,30 @@ def test_what_a_call_wrote_is_not_read_through_the_read_only_path():
     for name in os.listdir(csrc):
         if name.startswith(("paged", "attn_prefill")):
             assert not written.search(open(os.path.join(csrc, name)).read()), name
+
+
+@pytest.mark.parametrize("H,G,window,q", [(8, 4, 0, 1), (2, 4, 0, 5), (8, 4, 4096, 1), (1, 1, 0, 1)])
+def test_a_plan_with_room_has_the_ctas_of_the_lengths_it_may_serve(H, G, window, q):
+    pages = 2100
+    pool, rng = make_pool(pages, H=H), random.Random(1)
+    tables = tables_for([131072, 64], 64, pages, rng)
+    full = hqmq.PagedBatch(pool, tables, [131072, 64], [q, q], n_heads=H * G, window=window or None).plan
+    short = hqmq.PagedBatch(pool, [t[:5] for t in tables], [300, 40], [q, q], n_heads=H * G, window=window or None, reserve_pages=2049)
+    assert short.plan.dec_ctas >= full.dec_ctas and short.plan.ms_ctas >= full.ms_ctas
+    none = hqmq.PagedBatch(pool, [t[:5] for t in tables], [300, 40], [q, q], n_heads=H * G, window=window or None).plan
+    assert none.dec_ctas <= 148 // H and short.plan.dec_ctas * H <= 148 and short.plan.ms_ctas * H <= 148
+    # and whatever the lengths, every tile lies in one warp's stretch
+    p = _lib.PagedPlan.from_buffer_copy(short.plan)
+    p.renew = 1
+    for kv in ([300, 40], [5, 5], [131072, 64], [70000, 17]):
+        host, *_ = short._lay_out(p, tables, kv, [q, q])
+        w = host.numpy()
+        lengths, own = [[n, q] for n in kv], [t[:-(-n // 64)] for t, n in zip(tables, kv)]
+        for rows, unit, base, warp, total, ctas, per in ((q * G, p.dec_unit, p.dec_base, p.dec_warp, p.dec_tiles, p.dec_ctas, DEC_WARPS if p.dec_rows == 8 else DEC_WARPS_WIDE),
+                                                        (p.ms_rows, p.ms_unit, p.ms_base, p.ms_warp, p.ms_tiles, p.ms_ctas, MASS_WARPS)):
+            want = []
+            for s in (0, 1):
+                for r in range(0, q * G, rows):
+                    lo, hi = keys_of(kv[s], q, G, window, r, min(q * G, r + rows))
+                    want.append((s, r, lo // 16, -(-hi // 16)))
+            check_flat(w, unit, base, warp, total, ctas, per, want, own, 64, lengths)
