@@ -96,7 +96,7 @@ class AttnArgs(C.Structure):
 class PagedPlan(C.Structure):
     _fields_ = [("struct_size", C.c_uint32)] + [(name, C.c_int32) for name in (
         "n_seqs", "n_pages", "page_tokens", "H_q", "H_kv", "d", "window", "tab_room", "renew", "total_q", "most_q",
-        "reserved", "words", "seqs", "tabs", "n_tab", "dec_units", "dec_rows", "dec_ctas", "dec_unit", "dec_base",
+        "no_mass", "words", "seqs", "tabs", "n_tab", "dec_units", "dec_rows", "dec_ctas", "dec_unit", "dec_base",
         "dec_warp", "dec_cut", "dec_tiles", "ch_units", "ch_streams", "ch_tiles", "ch_heads", "ch_whole", "ch_ctas",
         "ch_unit", "ch_order", "ch_start", "ch_seqs", "ch_img_tiles", "ch_img", "ms_units", "ms_rows", "ms_ctas",
         "ms_unit", "ms_base", "ms_warp", "ms_tiles", "ms_groups", "ms_group", "ms_tile_room", "ms_group_room")]

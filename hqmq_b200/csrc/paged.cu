@@ -32,6 +32,7 @@ int check_args(const hqmq_paged_attn_args* a, bool mass) {
   if (!(a->softmax_scale > 0.f && a->softmax_scale < INFINITY)) return HQMQ_ERR_ARG;
   if (mass) {
     if (!is_half_dtype(a->q_dtype)) return HQMQ_ERR_UNSUPPORTED;
+    if (p.no_mass) return HQMQ_ERR_CAPACITY;
     return a->mass ? HQMQ_OK : HQMQ_ERR_ARG;
   }
   if ((rc = check_pool(a->V, p)) != 0) return rc;

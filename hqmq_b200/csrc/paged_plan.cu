@@ -123,7 +123,11 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
     ch_units += um;
     img += last - first;
   }
-  if (ms_tiles > (1 << 29) || ch_tiles > (1 << 26)) return HQMQ_ERR_SHAPE;
+  if (ch_tiles > (1 << 26)) return HQMQ_ERR_SHAPE;
+  // (a prompt whose weights nobody could hold is no reason to refuse its attention)
+  const int64_t ms_blocks = blocks_of(most_rows, p.ms_rows), ms_held = ms_blocks * p.tab_room * (p.page_tokens / 16);
+  p.no_mass = std::max(ms_tiles, ms_held) > (1 << 29);
+  if (p.no_mass) ms_tiles = ms_units = ms_groups = 0;
   p.ch_units = (int)ch_units; p.ch_tiles = (int)ch_tiles; p.ch_img_tiles = (int)img;
   // the operand images of as many heads at a time as half a gigabyte holds, a divisor of the heads
   p.ch_heads = p.H_kv;
@@ -154,16 +158,15 @@ extern "C" int hqmq_paged_plan_size(hqmq_paged_plan* plan, const int32_t* kv_len
   if (p.tab_room) {
     if (n_tab > p.tab_room) return HQMQ_ERR_CAPACITY;
     // (every unit walks its sequence's tiles at most; a sequence has that many units)
-    const int64_t blocks = blocks_of(most_rows, p.ms_rows), tiles = blocks * p.tab_room * (p.page_tokens / 16);
-    if (tiles > (1 << 29)) return HQMQ_ERR_SHAPE;
+    const int64_t tiles = p.no_mass ? 0 : ms_held;
     p.ms_tile_room = (int)tiles;
-    if (ms_units) ms_most = std::max(ms_tiles, std::min(tiles, blocks * room_of(ms_units, (p.ms_rows + G - 1) / G)));
-    p.ms_group_room = p.H_q ? (int)((int64_t)p.tab_room * p.page_tokens / mass_group(p.ms_rows) + p.n_seqs) : 0;
+    if (ms_units) ms_most = std::max(ms_tiles, std::min(tiles, ms_blocks * room_of(ms_units, (p.ms_rows + G - 1) / G)));
+    p.ms_group_room = p.H_q && !p.no_mass ? (int)((int64_t)p.tab_room * p.page_tokens / mass_group(p.ms_rows) + p.n_seqs) : 0;
   }
   p.ms_ctas = (int)std::max<int64_t>(1, std::min<int64_t>(most, (ms_most + kMassWarps - 1) / kMassWarps));
   if (p.renew) {
     if (ch_units || had.ch_units) return HQMQ_ERR_UNSUPPORTED;
-    if (had.dec_units != p.dec_units || had.dec_rows != p.dec_rows || had.ms_units != p.ms_units || had.ms_rows != p.ms_rows ||
+    if (had.dec_units != p.dec_units || had.dec_rows != p.dec_rows || had.ms_units != p.ms_units || had.no_mass != p.no_mass || had.ms_rows != p.ms_rows ||
         had.total_q != p.total_q || had.most_q != p.most_q) return HQMQ_ERR_SHAPE;
     p.dec_ctas = had.dec_ctas; p.ms_ctas = had.ms_ctas;
   }
@@ -210,7 +213,7 @@ extern "C" int hqmq_paged_plan_fill(const hqmq_paged_plan* plan, const int32_t* 
     const int my_mu = mu;
     if (p.H_q && q) {
       const int rows = q * G;
-      for (int r = 0; r < rows; r += p.ms_rows, ++mu) {
+      for (int r = 0; r < rows && !p.no_mass; r += p.ms_rows, ++mu) {
         int beg, end;
         unit_keys(kv, q, G, p.window, r, std::min(rows, r + p.ms_rows), beg, end);
         int32_t* u = out + p.ms_unit + 4 * mu;
@@ -242,7 +245,7 @@ extern "C" int hqmq_paged_plan_fill(const hqmq_paged_plan* plan, const int32_t* 
         img += last - first;
       }
     }
-    if (p.H_q)
+    if (p.H_q && !p.no_mass)
       for (int t = 0; t < kv; t += mass_group(p.ms_rows)) {
         int32_t* g = out + p.ms_group + 4 * mg++;
         g[0] = s; g[1] = t; g[2] = my_mu; g[3] = mu;

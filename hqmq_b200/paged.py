@@ -366,6 +366,8 @@ def paged_attention_mass(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, tabl
         a = _attn_args(Q, pool, batch, table_K, softmax_scale, softcap, sinks, "paged_attention_mass")
         if Q.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"paged_attention_mass: Q is fp16 or bf16, not {Q.dtype}")
+        if batch.plan.no_mass:
+            raise ValueError("paged_attention_mass: the scores of all of the batch's queries have no room; weigh a prompt's last tokens in a batch of their own")
         if not -float("inf") < decay < float("inf"):
             raise ValueError(f"decay={decay}")
         a.decay, a.mass = float(decay), pool.K.c_struct().rs         # (any address: it is set below)

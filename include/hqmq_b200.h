@@ -475,7 +475,8 @@ typedef struct hqmq_paged_plan {
   int32_t renew;               /* 1: same q_lens, other kv_lens and tables for a plan sized before with tab_room; no count, place or
                                   launch changes (prompt chunks: HQMQ_ERR_UNSUPPORTED), so captured calls follow the plan's words */
   int32_t total_q;             /* rows of Q: the sum of q_lens */
-  int32_t most_q, reserved;    /* the largest q_len */
+  int32_t most_q;              /* the largest q_len */
+  int32_t no_mass;             /* 1: the scores of so many queries have no room (2^29 tiles of 16 keys); hqmq_paged_mass refuses the plan */
   /* words (4 bytes) of the plan, and in words where its parts begin */
   int32_t words, seqs, tabs, n_tab;
   /* decode: sequences of few rows */

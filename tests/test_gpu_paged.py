@@ -846,3 +846,17 @@ def test_queries_that_are_no_numbers_spoil_their_own_rows_only(q_dtype, q_lens):
         assert bool(fine[~bad[at:at + n]].all())
         assert bool(out[at:at + n][bad[at:at + n]].isnan().all())
         at += n
+
+
+def test_a_prompt_whose_weights_have_no_room():
+    n, G, d = 190_000, 16, 64
+    w = World(1, d, 24, 3, [n], outliers=None, rounds=1, page=1024, kind="randn", garbage=False)
+    b = w.batch([n], G)
+    q = (1.5 * torch.randn(n, G, d, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))).to(torch.bfloat16)
+    out = hqmq.paged_attention(q, w.pool, b, *w.tab)
+    with pytest.raises(ValueError, match="no room"):
+        hqmq.paged_attention_mass(q, w.pool, b, w.tab[0])
+    (K,), (V,) = w.dense()
+    for t in (0, 31, 5000, 100_001, n - 1):
+        o, _, bound, _ = attend64(q[t:t + 1].cpu(), K[:, :t + 1], V[:, :t + 1], G, None, None, None, d ** -0.5)
+        assert bool(((out[t:t + 1].cpu().double() - o).abs() <= bound + o.abs() * (2.0 ** -8 + 2.0 ** -18) + 1e-7).all()), t

@@ -334,3 +334,22 @@ def test_a_plan_with_room_has_the_ctas_of_the_lengths_it_may_serve(H, G, window,
                     lo, hi = keys_of(kv[s], q, G, window, r, min(q * G, r + rows))
                     want.append((s, r, lo // 16, -(-hi // 16)))
             check_flat(w, unit, base, warp, total, ctas, per, want, own, 64, lengths)
+
+
+def test_prompts_whose_weights_have_no_room_are_attended_all_the_same(built_lib):
+    n = 524288
+    pool = make_pool(n // 64, H=8)
+    table = [list(range(n // 64))]
+    b = hqmq.PagedBatch(pool, table, [n], [n], n_heads=32)
+    assert b.plan.no_mass == 1 and b.plan.ms_units == 0 and b.plan.ch_units == n // 64
+    a = _args(pool, b)
+    L = _lib.lib()
+    assert L.hqmq_paged_mass(C.byref(a), None, 0, None) == -9 and L.hqmq_paged_mass_workspace_bytes(C.byref(a)) == 0
+    assert L.hqmq_paged_attn_workspace_bytes(C.byref(a)) > 0
+    # (the room of a batch that is renewed counts as well)
+    b = hqmq.PagedBatch(pool, [[0]], [40], [32], n_heads=16, reserve_pages=1 << 24)
+    assert b.plan.no_mass == 0
+    b = hqmq.PagedBatch(pool, [[0]], [40], [32], n_heads=128, reserve_pages=1 << 24)
+    assert b.plan.no_mass == 1
+    # (the last tokens of the same prompt have weights)
+    assert hqmq.PagedBatch(pool, table, [n], [32], n_heads=32).plan.no_mass == 0
