@@ -115,7 +115,7 @@ def _int_array(x, what: str) -> np.ndarray:
         raise TypeError(f"hqmq_b200: {what} are integers")
     if a.size and (int(a.min()) < -(1 << 31) or int(a.max()) >= 1 << 31):
         raise ValueError(f"{what} out of range")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    return np.array(a, dtype=np.int32, order="C")     # (a copy: the caller's array may count on)
 
 
 class PagedBatch:

@@ -353,3 +353,14 @@ def test_prompts_whose_weights_have_no_room_are_attended_all_the_same(built_lib)
     assert b.plan.no_mass == 1
     # (the last tokens of the same prompt have weights)
     assert hqmq.PagedBatch(pool, table, [n], [32], n_heads=32).plan.no_mass == 0
+
+
+def test_a_batch_keeps_its_lengths_when_the_callers_arrays_change():
+    pool = make_pool()
+    kv, q, tables = np.array([100, 90], np.int32), torch.tensor([1, 2], dtype=torch.int32), np.array([[1, 2], [3, 2]], np.int32)
+    b = hqmq.PagedBatch(pool, tables, kv, q)
+    kv += 40
+    q.zero_()
+    tables[1, 1] = 5
+    assert b.kv_lens.tolist() == [100, 90] and b.q_lens.tolist() == [1, 2]
+    assert not b.stores_alone()                                          # both write page 2, as the plan on the device does
