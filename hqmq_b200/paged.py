@@ -138,11 +138,13 @@ class PagedBatch:
             raise ValueError(f"n_heads={n_heads} must be a positive multiple of the pool's {pool.H_kv} KV heads")
         if window is not None and window < 1:
             raise ValueError("window is at least 1 (None: no window)")
+        if not 0 <= reserve_pages <= 1 << 24:
+            raise ValueError(f"reserve_pages={reserve_pages}: from 0 to {1 << 24}")
         self.n_pages, self.page_tokens, self.H_kv, self.d_head, self.device = pool.n_pages, pool.page_tokens, pool.H_kv, pool.d_head, pool.device
         self.n_heads, self.window = n_heads, window
         p = self.plan = _lib.PagedPlan()
         p.struct_size = C.sizeof(_lib.PagedPlan)
-        p.n_pages, p.page_tokens, p.H_q, p.H_kv, p.d, p.window = pool.n_pages, pool.page_tokens, n_heads or 0, pool.H_kv, pool.d_head, window or 0
+        p.n_pages, p.page_tokens, p.H_q, p.H_kv, p.d, p.window = pool.n_pages, pool.page_tokens, n_heads or 0, pool.H_kv, pool.d_head, min(window or 0, 1 << 30)
         p.tab_room = int(reserve_pages)
         host, kv, q, pages = self._lay_out(p, tables, kv_lens, q_lens)
         self._take(kv, q, pages)
@@ -368,8 +370,8 @@ def paged_attention_mass(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, tabl
             raise TypeError(f"paged_attention_mass: Q is fp16 or bf16, not {Q.dtype}")
         if batch.plan.no_mass:
             raise ValueError("paged_attention_mass: the scores of all of the batch's queries have no room; weigh a prompt's last tokens in a batch of their own")
-        if not -float("inf") < decay < float("inf"):
-            raise ValueError(f"decay={decay}")
+        if not abs(decay) <= torch.finfo(torch.float32).max:
+            raise ValueError(f"decay={decay}: a number that fp32 holds")
         a.decay, a.mass = float(decay), pool.K.c_struct().rs         # (any address: it is set below)
         nbytes = _sized(a, pool, batch, L.hqmq_paged_mass_workspace_bytes, L.hqmq_paged_mass, Q, (table_K,), sinks, "hqmq_paged_mass")
         hit = batch._keep(key, (a, C.byref(a), nbytes))

@@ -860,3 +860,11 @@ def test_a_prompt_whose_weights_have_no_room():
     for t in (0, 31, 5000, 100_001, n - 1):
         o, _, bound, _ = attend64(q[t:t + 1].cpu(), K[:, :t + 1], V[:, :t + 1], G, None, None, None, d ** -0.5)
         assert bool(((out[t:t + 1].cpu().double() - o).abs() <= bound + o.abs() * (2.0 ** -8 + 2.0 ** -18) + 1e-7).all()), t
+
+
+def test_a_decay_that_fp32_does_not_hold_is_refused():
+    w = World(1, 64, 24, 3, [40], garbage=False)
+    q = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    for decay in (1e300, -1e39, float("nan")):
+        with pytest.raises(ValueError):
+            hqmq.paged_attention_mass(q, w.pool, w.batch([1], 2), w.tab[0], decay=decay)

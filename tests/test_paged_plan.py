@@ -364,3 +364,16 @@ def test_a_batch_keeps_its_lengths_when_the_callers_arrays_change():
     tables[1, 1] = 5
     assert b.kv_lens.tolist() == [100, 90] and b.q_lens.tolist() == [1, 2]
     assert not b.stores_alone()                                          # both write page 2, as the plan on the device does
+
+
+@pytest.mark.parametrize("window", [1 << 31, (1 << 32) + 5, 1 << 40])
+def test_a_window_wider_than_any_sequence_is_no_window(window):
+    pool = make_pool()
+    data = [hqmq.PagedBatch(pool, [[1, 2, 3]], [150], [60], n_heads=4, window=w) for w in (None, window)]
+    assert torch.equal(data[0].data, data[1].data) and data[1].plan.window == 1 << 30
+
+
+@pytest.mark.parametrize("room", [-1, (1 << 24) + 1, (1 << 32) + 8])
+def test_rooms_that_no_plan_has_are_refused(room):
+    with pytest.raises(ValueError):
+        hqmq.PagedBatch(make_pool(), [[1]], [50], [1], n_heads=4, reserve_pages=room)
