@@ -104,15 +104,20 @@ class PagedKVCache:
         self._step, self._batches = (seqs, new), {}
 
     def batch(self, layer_idx: int, n_heads: Optional[int] = None) -> PagedBatch:
-        """The step's batch for a layer (made once for all layers of a window)."""
+        """The step's batch for a layer (made once for all layers of a window whose pools are alike: a device, KV heads and a head dim)."""
         if self._step is None:
             raise _lib.HqmqError("hqmq_b200: begin() a step first")
-        key = (n_heads, self.sliding_window.get(layer_idx) if n_heads else None)
+        pool = self._pools[layer_idx]
+        key = (n_heads, self.sliding_window.get(layer_idx) if n_heads else None, *self._shape(pool))
         if key not in self._batches:
             seqs, new = self._step
-            self._batches[key] = PagedBatch(self._pools[layer_idx], [self._table[i] for i in seqs], [self._len[i] for i in seqs], new,
+            self._batches[key] = PagedBatch(pool, [self._table[i] for i in seqs], [self._len[i] for i in seqs], new,
                                             n_heads=key[0], window=key[1])
         return self._batches[key]
+
+    @staticmethod
+    def _shape(pool: PagedKV):
+        return pool.device, pool.H_kv, pool.d_head
 
     def _new_pool(self, k: torch.Tensor) -> PagedKV:
         q, outl = self._inner, hasattr(self.quantizer, "median_mult")
@@ -180,10 +185,13 @@ class PagedKVCache:
         if not cut or not self._pools:
             return {}
         tables = [pages[per * k:per * (k + 1)] for k in range(len(cut))]
-        any_pool = next(iter(self._pools.values()))
-        old = PagedBatch(any_pool, [self._table[i] for i in cut], [self._len[i] for i in cut])
-        new = PagedBatch(any_pool, tables, [keep] * len(cut))
-        kept = {layer: paged_evict(pool, old, new, self._mass[layer], first=first, last=last) for layer, pool in self._pools.items()}
+        moves: dict = {}                         # old and new batch by what a batch is bound to
+        for pool in self._pools.values():
+            if self._shape(pool) not in moves:
+                moves[self._shape(pool)] = (PagedBatch(pool, [self._table[i] for i in cut], [self._len[i] for i in cut]),
+                                            PagedBatch(pool, tables, [keep] * len(cut)))
+        kept = {layer: paged_evict(pool, *moves[self._shape(pool)], self._mass[layer], first=first, last=last)
+                for layer, pool in self._pools.items()}
         for i, table in zip(cut, tables):
             self._free.extend(reversed(self._table[i]))
             self._table[i], self._len[i] = table, keep

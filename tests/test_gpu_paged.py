@@ -868,3 +868,27 @@ def test_a_decay_that_fp32_does_not_hold_is_refused():
     for decay in (1e300, -1e39, float("nan")):
         with pytest.raises(ValueError):
             hqmq.paged_attention_mass(q, w.pool, w.batch([1], 2), w.tab[0], decay=decay)
+
+
+def test_a_cache_of_layers_with_different_head_dims():
+    H, G, dims = 2, 4, (128, 64)
+    inner = hqmq.HQMQ(2, H, 24, 3, device=DEV)
+    cache = hqmq.PagedKVCache(inner, 24)
+    ids, gen = cache.add(2), torch.Generator().manual_seed(0)
+    for new in ([300, 40], [1, 2]):
+        cache.begin(ids, new)
+        for layer, d in enumerate(dims):
+            k, v = (torch.randn(sum(new), H, d, generator=gen).to(torch.bfloat16).to(DEV) for _ in (0, 1))
+            cache.update(k, v, layer)
+            q = torch.randn(sum(new), H * G, d, generator=gen).to(torch.bfloat16)
+            out = cache.attend(q.to(DEV), layer).cpu()
+            cache.weigh(q.to(DEV), layer)
+            tabs = [inner.tables(layer, i, DEV)["table16"] for i in (0, 1)]
+            at = 0
+            for s, n in zip(ids, new):
+                K, V = (dense64(host(x), t, 24, 3, cache._table[s], cache.length(s)) for x, t in zip((cache.pool(layer).K, cache.pool(layer).V), tabs))
+                o, _, bound, _ = attend64(q[at:at + n], K, V, G, None, None, None, d ** -0.5)
+                assert bool(((out[at:at + n].double() - o).abs() <= bound + o.abs() * (2.0 ** -8 + 2.0 ** -18) + 1e-7).all())
+                at += n
+    kept = cache.evict(ids, keep=100)
+    assert sorted(kept) == [0, 1] and all(k.shape == (1, H, 100) for k in kept.values()) and [cache.length(s) for s in ids] == [100, 42]

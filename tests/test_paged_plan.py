@@ -377,3 +377,16 @@ def test_a_window_wider_than_any_sequence_is_no_window(window):
 def test_rooms_that_no_plan_has_are_refused(room):
     with pytest.raises(ValueError):
         hqmq.PagedBatch(make_pool(), [[1]], [50], [1], n_heads=4, reserve_pages=room)
+
+
+def test_layers_of_unlike_pools_have_batches_of_their_own():
+    cache = hqmq.PagedKVCache(None, 8)
+    cache._pools.update({0: make_pool(8, H=2, d=128), 1: make_pool(8, H=2, d=64), 2: make_pool(8, H=2, d=128), 3: make_pool(8, H=1, d=64)})
+    a, = cache.add()
+    cache.begin([a], [100])
+    got = [(cache.batch(layer, 4), cache.batch(layer)) for layer in range(4)]
+    for layer, pair in enumerate(got):
+        for b in pair:
+            pool = cache.pool(layer)
+            assert (b.d_head, b.H_kv, b.device, b.plan.d, b.plan.H_kv) == (pool.d_head, pool.H_kv, pool.device, pool.d_head, pool.H_kv)
+    assert got[0][0] is got[2][0] and got[0][1] is got[2][1] and got[0][0] is not got[1][0]
