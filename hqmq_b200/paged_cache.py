@@ -81,13 +81,18 @@ class PagedKVCache:
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence is named twice")
 
-    def _take(self, n: int) -> List[int]:
+    def _next_pages(self, n: int) -> List[int]:
+        """The next free pages, without weights; they stay free until ``_hand_out``, so that what raises in between leaves all as it was."""
         if n > len(self._free):
             raise _lib.HqmqError(f"hqmq_b200: {n} pages wanted, {len(self._free)} of {self.n_pages} free")
-        pages = [self._free.pop() for _ in range(n)]
-        for mass in self._mass.values():         # (a page's earlier tokens leave no weight)
-            mass[torch.tensor(pages, device=mass.device)] = 0.0
+        pages = self._free[len(self._free) - n:][::-1]
+        if pages:
+            for mass in self._mass.values():     # (a page's earlier tokens leave no weight)
+                mass[torch.tensor(pages, device=mass.device)] = 0.0
         return pages
+
+    def _hand_out(self, n: int) -> None:
+        del self._free[len(self._free) - n:]
 
     def begin(self, seqs: Sequence[int], new_tokens: Sequence[int]) -> None:
         """The next forward pass: every one of ``seqs`` gets so many new tokens.  ``update`` and ``attend`` of all layers follow."""
@@ -96,7 +101,8 @@ class PagedKVCache:
         if len(seqs) != len(new) or not seqs or min(new) < 0:
             raise ValueError(f"{len(seqs)} sequences and {len(new)} counts of new tokens")
         more = [-(-(self._len[i] + n) // self.page_tokens) - len(self._table[i]) for i, n in zip(seqs, new)]
-        pages = self._take(sum(more)) if sum(more) else []
+        pages = self._next_pages(sum(more))
+        self._hand_out(sum(more))
         for i, n, m in zip(seqs, new, more):
             self._table[i] += pages[:m]
             pages = pages[m:]
@@ -180,10 +186,10 @@ class PagedKVCache:
             raise _lib.HqmqError(f"hqmq_b200: no weights of layers {missing} (weigh() first)")
         cut = [int(i) for i in seqs if self._len[i] > keep]
         per = -(-keep // self.page_tokens)
-        pages = self._take(per * len(cut)) if self._pools else []      # (raises with nothing changed)
-        self._step, self._batches = None, {}
         if not cut or not self._pools:
+            self._step, self._batches = None, {}
             return {}
+        pages = self._next_pages(per * len(cut))  # (the tokens move to free pages: until all have, raising leaves everything as it was)
         tables = [pages[per * k:per * (k + 1)] for k in range(len(cut))]
         moves: dict = {}                         # old and new batch by what a batch is bound to
         for pool in self._pools.values():
@@ -192,6 +198,8 @@ class PagedKVCache:
                                             PagedBatch(pool, tables, [keep] * len(cut)))
         kept = {layer: paged_evict(pool, *moves[self._shape(pool)], self._mass[layer], first=first, last=last)
                 for layer, pool in self._pools.items()}
+        self._hand_out(len(pages))
+        self._step, self._batches = None, {}
         for i, table in zip(cut, tables):
             self._free.extend(reversed(self._table[i]))
             self._table[i], self._len[i] = table, keep

@@ -390,3 +390,29 @@ def test_layers_of_unlike_pools_have_batches_of_their_own():
             pool = cache.pool(layer)
             assert (b.d_head, b.H_kv, b.device, b.plan.d, b.plan.H_kv) == (pool.d_head, pool.H_kv, pool.device, pool.d_head, pool.H_kv)
     assert got[0][0] is got[2][0] and got[0][1] is got[2][1] and got[0][0] is not got[1][0]
+
+
+def test_a_cache_whose_call_fails_half_way_loses_no_page():
+    cache = hqmq.PagedKVCache(None, 16)
+    cache._pools.update({0: make_pool(16, d=128), 1: make_pool(16, d=64)})
+    cache._mass.update({layer: pool.new_mass() for layer, pool in cache._pools.items()})
+    a, b = cache.add(2)
+    cache.begin([a, b], [200, 300])
+    state = lambda: (list(cache._free), {i: list(t) for i, t in cache._table.items()}, dict(cache._len), cache._step)
+    before = state()
+    with pytest.raises(_lib.HqmqError):                                  # (these pools are no CUDA memory)
+        cache.evict([a, b], keep=100)
+    assert state() == before
+
+    class Busy:                                                          # (a copy to the device inside a graph's capture)
+        device = "cpu"
+
+        def __setitem__(self, *_):
+            raise RuntimeError("capturing")
+
+    cache._mass[1] = Busy()
+    for call in (lambda: cache.begin([a], [200]), lambda: cache.evict([b], keep=100)):
+        with pytest.raises(RuntimeError):
+            call()
+        assert state() == before
+    assert cache.free_pages == 16 - 4 - 5
