@@ -96,13 +96,15 @@ class PagedKV:
         """Zeroed weights, one per token, page and KV head (see ``paged_attention_mass``)."""
         return torch.zeros(self.n_pages, self.H_kv, self.page_tokens, dtype=torch.float32, device=self.device)
 
-    def check(self) -> None:
+    def check(self, pages: Optional[Sequence[int]] = None) -> None:
         """Synchronise and raise if a page's side buffer was too small for the outliers it was given (rows and flags are complete
-        then, but values beyond the capacity were dropped and read as 0)."""
+        then, but values beyond the capacity were dropped and read as 0).  ``pages``: those that hold tokens (None: all)."""
+        at = None if pages is None else torch.tensor(list(pages), dtype=torch.int64, device=self.device)
         for name, pk in (("K", self.K), ("V", self.V)):
-            if pk.with_outliers and int(pk.out_count.max()) > pk.out_cap:
-                raise _lib.HqmqError(f"hqmq_b200: the outliers of a page of {name} overflowed ({int(pk.out_count.max())} > "
-                                     f"{pk.out_cap} chunks); raise out_cap")
+            if pk.with_outliers and (at is None or at.numel()):
+                most = int((pk.out_count if at is None else pk.pages("out_count")[at]).max())
+                if most > pk.out_cap:
+                    raise _lib.HqmqError(f"hqmq_b200: the outliers of a page of {name} overflowed ({most} > {pk.out_cap} chunks); raise out_cap")
 
 
 def _int_array(x, what: str) -> np.ndarray:

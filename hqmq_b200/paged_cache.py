@@ -37,6 +37,7 @@ class PagedKVCache:
         self._pools: Dict[int, PagedKV] = {}
         self._mass: Dict[int, torch.Tensor] = {}
         self._step: Optional[Tuple[List[int], List[int]]] = None
+        self._updated: set = set()               # layers whose new tokens of the step are stored
         self._batches: dict = {}
 
     @property
@@ -107,7 +108,7 @@ class PagedKVCache:
             self._table[i] += pages[:m]
             pages = pages[m:]
             self._len[i] += n
-        self._step, self._batches = (seqs, new), {}
+        self._step, self._batches, self._updated = (seqs, new), {}, set()
 
     def batch(self, layer_idx: int, n_heads: Optional[int] = None) -> PagedBatch:
         """The step's batch for a layer (made once for all layers of a window whose pools are alike: a device, KV heads and a head dim)."""
@@ -151,6 +152,7 @@ class PagedKVCache:
         k, v = (x.transpose(0, 1).unsqueeze(0) for x in (key_states, value_states))
         self.quantizer.encode_pair(k, v, layer_idx, *pair)
         paged_store(pool, *pair, self.batch(layer_idx))
+        self._updated.add(layer_idx)
         return pool
 
     def attend(self, query_states: torch.Tensor, layer_idx: int, softmax_scale: Optional[float] = None,
@@ -206,12 +208,20 @@ class PagedKVCache:
         return kept
 
     def check(self) -> None:
-        """Synchronise and raise if a side buffer overflowed, or an update gave up on a bounded wait of the encoder."""
+        """Synchronise and raise if the side buffer of a page that is held overflowed, or an update gave up on a bounded wait of the encoder
+        (its tokens have a scale of NaN).  Of a step under way, a layer's new tokens count from its ``update`` on."""
         for layer, pool in self._pools.items():
+            late = dict(zip(*self._step)) if self._step and layer not in self._updated else {}
+            lens = {i: self._len[i] - late.get(i, 0) for i in self._table}
+            held = [(p, min(self.page_tokens, lens[i] - k * self.page_tokens)) for i, t in self._table.items()
+                    for k, p in enumerate(t[:-(-lens[i] // self.page_tokens)])]
+            if not held:
+                continue
             try:
-                pool.check()
+                pool.check([p for p, _ in held])
             except _lib.HqmqError as e:
                 raise _lib.HqmqError(f"{e} (layer {layer}: raise outlier_capacity)") from None
-            held = [p for i, t in self._table.items() for p in t[:self._len[i] // self.page_tokens]]
-            if held and bool(torch.stack([x.pages("rs")[torch.tensor(held, device=pool.device)].isnan().any() for x in (pool.K, pool.V)]).any()):
+            pages, tokens = torch.tensor(held, device=pool.device).unbind(1)
+            live = torch.arange(self.page_tokens, device=pool.device) < tokens.view(-1, 1, 1)      # (rows behind them are of another life)
+            if any(bool((x.pages("rs")[pages].isnan() & live).any()) for x in (pool.K, pool.V)):
                 raise _lib.HqmqError(f"hqmq_b200: an update of layer {layer} gave up on a bounded wait")

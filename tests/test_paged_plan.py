@@ -416,3 +416,57 @@ def test_a_cache_whose_call_fails_half_way_loses_no_page():
             call()
         assert state() == before
     assert cache.free_pages == 16 - 4 - 5
+
+
+def _checked_cache(lens, updated=True):
+    cache = hqmq.PagedKVCache(None, 12)
+    pool = cache._pools[0] = make_pool(12, outliers_K=True, outliers_V=True, out_cap=8)
+    for pk in (pool.K, pool.V):                                          # (what recycled pages may hold)
+        pk.pages("rs").fill_(float("nan"))
+        pk.pages("out_count").fill_(1 << 20)
+    ids = cache.add(len(lens))
+    cache.begin(ids, lens)
+    for i in ids:
+        for k, p in enumerate(cache._table[i]):
+            for pk in (pool.K, pool.V):
+                pk.pages("rs")[p, :, :min(64, lens[ids.index(i)] - 64 * k)] = 1.0
+                pk.pages("out_count")[p] = 8
+    if updated:
+        cache._updated = {0}
+    return cache, pool, ids
+
+
+@pytest.mark.parametrize("lens,token", [([63], 62), ([1, 200], 199), ([64, 65], 64), ([130], 5)])
+@pytest.mark.parametrize("plane", ["K", "V"])
+def test_check_looks_at_every_token_that_is_held(lens, token, plane):
+    cache, pool, ids = _checked_cache(lens)
+    cache.check()
+    getattr(pool, plane).pages("rs")[cache._table[ids[-1]][token // 64], 1, token % 64] = float("nan")
+    with pytest.raises(_lib.HqmqError, match="bounded wait"):
+        cache.check()
+    cache.drop([ids[-1]])
+    cache.check()
+
+
+@pytest.mark.parametrize("plane", ["K", "V"])
+def test_check_forgets_the_overflows_of_pages_that_are_free(plane):
+    cache, pool, (a, b) = _checked_cache([100, 40])
+    getattr(pool, plane).pages("out_count")[cache._table[b][0], 1] = 9
+    with pytest.raises(_lib.HqmqError, match="overflowed"):
+        cache.check()
+    with pytest.raises(_lib.HqmqError, match="overflowed"):
+        pool.check()
+    cache.drop([b])
+    cache.check()
+    pool.check(cache._table[a])
+    cache.drop([a])
+    cache.check()
+
+
+def test_check_in_the_middle_of_a_step():
+    cache, pool, (a, b) = _checked_cache([100, 40])
+    cache.begin([a, b], [60, 1])                                         # a page of an earlier life, and rows of one
+    cache.check()
+    cache._updated.add(0)
+    with pytest.raises(_lib.HqmqError):
+        cache.check()
