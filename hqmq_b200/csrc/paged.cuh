@@ -46,7 +46,7 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-constexpr int kDecWarps = 16, kDecWarpsWide = 8;     // warps of a decode CTA, for up to 8 and up to 16 rows
+constexpr int kDecWarps = 16, kDecWarpsWide = 8;     // warps of a decode CTA, for up to 8 and up to 32 rows
 constexpr int kMassWarps = 12;
 constexpr int kMassRowsWide = 32;                    // rows of a unit of the weights where a sequence has more than 8
 // Tokens of a CTA of the weights' second kernel: of 8 rows a token has 32 bytes of scores per unit, of 32 rows 128 (512 tokens either way:

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
   extern __shared__ __align__(16) unsigned char smem_raw[];
   uint32_t* hist = reinterpret_cast<uint32_t*>(smem_raw);         // [3][2048]
   uint32_t* pub = hist + 3 * 2048;                                // heavier, equal: what other CTAs read
-  uint32_t* wsum = pub + 4;                                       // [2][16]
+  uint32_t* wsum = pub + 4;                                       // [2][kSelWarps]
   uint32_t* pick = wsum + 2 * kSelWarps;                          // bin, left
   uint32_t* keys = pick + 4;
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
@@ -439,7 +439,7 @@ extern "C" int hqmq_paged_evict(const hqmq_paged_evict_args* a, void* stream) {
   while (C < 8 && units * C * 2 <= 148 && a->longest >= 2 * C * 2048) C *= 2;
   while (C < 8 && (a->longest + C - 1) / C + 32 > kSelCached) C *= 2;
   const int per = ((a->longest + C - 1) / C + 31) & ~31;
-  p.cached = per <= kSelCached ? per : 0;
+  p.cached = per <= kSelCached ? per : kSelCached;      // (a sequence that does not fit reads its weights again, the others of the call need not)
   const size_t smem = (3 * 2048 + 4 + 2 * kSelWarps + 4 + (size_t)p.cached) * 4;
   cudaStream_t st = (cudaStream_t)stream;
   HQMQ_CHECK_CUDA(raise_smem_limit((const void*)&evict_select_kernel, smem));

@@ -892,3 +892,37 @@ def test_a_cache_of_layers_with_different_head_dims():
                 at += n
     kept = cache.evict(ids, keep=100)
     assert sorted(kept) == [0, 1] and all(k.shape == (1, H, 100) for k in kept.values()) and [cache.length(s) for s in ids] == [100, 42]
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+def test_eviction_of_a_sequence_longer_than_shared_memory_holds(kind):
+    """More than eight CTAs' weights (327680), beside short sequences of the same call."""
+    kv, keep, first, last, page = [340_001, 700, 12_345], [20_000, 100, 12_345], 4, 16, 1024
+    need = [-(-n // page) for n in kv + keep]
+    order = list(range(sum(need)))
+    random.Random(0).shuffle(order)
+    cuts = np.cumsum([0] + need)
+    tables = [order[a:z] for a, z in zip(cuts, cuts[1:])]
+    pool = hqmq.PagedKV(sum(need), 1, 64, 24, 3, DEV, page_tokens=page)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for pk in (pool.K, pool.V):
+        pk.pages("codes").random_(0, 256, generator=g)
+        pk.pages("rs").uniform_(generator=g)
+    mass = torch.rand(sum(need), 1, page, device=DEV, generator=g)
+    if kind == "ties":
+        mass = (mass * 4).round()
+    before = [{k: v.cpu() for k, v in pk.planes().items()} for pk in (pool.K, pool.V)]
+    was = mass.cpu()
+    kept = hqmq.paged_evict(pool, hqmq.PagedBatch(pool, tables[:3], kv), hqmq.PagedBatch(pool, tables[3:], keep), mass, first=first, last=last).cpu()
+    now = mass.cpu()
+    for s, (n, k) in enumerate(zip(kv, keep)):
+        flat = torch.cat([was[p, 0] for p in tables[s]])[:n].double().numpy()
+        mid = np.argsort(-flat[first:n - last], kind="stable")[:k - first - last] + first
+        want = np.sort(np.concatenate([np.arange(first), mid, np.arange(n - last, n)])) if k < n else np.arange(n)
+        assert kept[s, 0, :k].tolist() == want.tolist() and bool((kept[s, 0, k:] == -1).all())
+        src = torch.tensor(tables[s])[torch.from_numpy(want) // page], torch.from_numpy(want) % page
+        dst = torch.tensor(tables[3 + s])[torch.arange(k) // page], torch.arange(k) % page
+        for x, y in zip((pool.K, pool.V), before):
+            for name in ("codes", "rs"):
+                assert torch.equal(x.pages(name).cpu()[dst[0], 0, dst[1]], y[name][src[0], 0, src[1]])
+        assert torch.equal(now[dst[0], 0, dst[1]], was[src[0], 0, src[1]])
