@@ -107,7 +107,8 @@ __global__ void __launch_bounds__(256, 4) paged_expand_kernel(const PagedExpandP
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           const float y = bits16_to_float((uint16_t)(w4[x >> 1] >> (16 * (x & 1))), pk.scale_dtype);
-          if (t + x < t_end) big = fmaxf(big, fabsf(y));
+          // (an infinite scale is its own key's: relative to it the others would be zeros, for queries that do not see it, too)
+          if (t + x < t_end && fabsf(y) < INFINITY) big = fmaxf(big, fabsf(y));
         }
       }
 #pragma unroll

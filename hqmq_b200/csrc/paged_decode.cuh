@@ -297,7 +297,7 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
       for (int nt = 0; nt < 2; ++nt) {
         const int t = nt * 8 + r;
         if constexpr (IB != 0) ld.template load_span<FL::KW, FL::LK>(kw[nt], sp + t * ROW, j, true);
-        ksc[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt);
+        ksc[nt] = key_scale(bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt));
         vsc[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsv)[t], p.sdt) * p.vfac;
       }
 #pragma unroll

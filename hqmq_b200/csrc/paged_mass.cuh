@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kMassWarps * 32, 1) paged_scores_kernel(const 
       for (int nt = 0; nt < 2; ++nt) {
         const int t = nt * 8 + r;
         if constexpr (IB != 0) ld.template load_span<FL::KW, FL::LK>(kw[nt], sp + t * ROW, j, true);
-        rs[nt] = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt);
+        rs[nt] = key_scale(bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[t], p.sdt));
       }
       uint32_t kcols = 0u, fk_t = 0u, before = 0u;
       bool wide = false;

@@ -246,6 +246,10 @@ __device__ __forceinline__ float load_query(uint32_t (*qb)[2], const QueryView& 
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
+// A key's scale as its score is multiplied by: an infinite one is no number (the key's values are infinite of either sign, so a score is
+// none; times an infinity it could be minus infinity, a weight of zero).
+__device__ __forceinline__ float key_scale(float x) { return fmaf(x, 0.f, x); }
+
 // tanh(x): for |x| <= 1/2 as x times a cubic in x^2 through its values at the Chebyshev nodes of [0, 1/4] (within 5e-7 of the value,
 // however small: a cap far above the scores leaves them as they are), beyond as 1 - 2 / (e^2x + 1).
 __device__ __forceinline__ float tanh_of(float x) {

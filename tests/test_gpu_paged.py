@@ -926,3 +926,35 @@ def test_eviction_of_a_sequence_longer_than_shared_memory_holds(kind):
             for name in ("codes", "rs"):
                 assert torch.equal(x.pages(name).cpu()[dst[0], 0, dst[1]], y[name][src[0], 0, src[1]])
         assert torch.equal(now[dst[0], 0, dst[1]], was[src[0], 0, src[1]])
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("q_lens,token", [([1, 8], 85), ([33, 60], 50), ([150, 90], 2)])
+def test_a_key_that_is_no_number_spoils_the_queries_that_see_it_only(value, q_lens, token):
+    w = World(1, 128, 96, 4, [200, 90])
+    K, V = w.dense()
+    w.pool.K.pages("rs")[w.tables[1][token // 64], 0, token % 64] = value
+    q = queries(w, q_lens, 4, torch.bfloat16)
+    out = hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab).cpu()
+    at = 0
+    for s, n in enumerate(q_lens):
+        o, _, bound, _ = attend64(q[at:at + n], K[s], V[s], 4, None, None, None, 128 ** -0.5)
+        fine = (out[at:at + n].double() - o).abs() <= bound + o.abs() * (2.0 ** -8 + 2.0 ** -18) + 1e-7
+        first = max(0, token - (w.kv[s] - n)) if s else n                        # the first query that sees the key
+        assert bool(fine[:first].all()) and bool(out[at + first:at + n].isnan().all()), s
+        at += n
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_weights_beside_a_key_that_is_no_number(value):
+    """A sequence whose queries see it has no weights; the other one has its own."""
+    w = World(1, 128, 96, 4, [200, 90])
+    K, V = w.dense()
+    w.pool.K.pages("rs")[w.tables[1][0], 0, 30] = value
+    for q_lens in ([1, 1], [12, 3]):
+        q = queries(w, q_lens, 4, torch.bfloat16)
+        mass = hqmq.paged_attention_mass(q.to(DEV), w.pool, w.batch(q_lens, 4), w.tab[0]).cpu()
+        _, m, _, bound = attend64(q[:q_lens[0]], K[0], V[0], 4, None, None, None, 128 ** -0.5)
+        got = [torch.cat([mass[p] for p in t], 1)[:, :n].double() for t, n in zip(w.tables, w.kv)]
+        assert bool(((got[0] - m).abs() <= bound + m * (2.0 ** -20 + 4 * q_lens[0] * 2.0 ** -24)).all())
+        assert bool(got[1].isnan().all())
