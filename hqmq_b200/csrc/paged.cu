@@ -112,11 +112,14 @@ int decode_launch(const hqmq_paged_attn_args* a, void* ws, cudaStream_t st) {
   // entries: what that reaches lies in the block's shared memory, too)
   const size_t any = (size_t)4 << p.ib;
   size_t tk = table, tv = table;
-  p.ext = outl && has_ext(p.ib) && compiled_fields(p.ib, a->K.radius_bits) && table + (size_t)warps * kExtK * 8 <= any;
-  if (p.ext) { tk += (size_t)warps * kExtK * 8; tv += (size_t)warps * kExtV * 8; }
+  const int room = (int)((any - table) / 8) / warps;           // (any >= table: an index has the bits of the codebook)
+  if (outl && has_ext(p.ib) && compiled_fields(p.ib, a->K.radius_bits) && room >= kExtLeast) {
+    p.ext_k = std::min(room, kPayK); p.ext_v = std::min(room, kPayV);
+    tk += (size_t)warps * p.ext_k * 8; tv += (size_t)warps * p.ext_v * 8;
+  }
   auto need = [&](int rk, int rv) { return std::max(rings + (tk << rk) + (tv << rv), std::max(any << rk, (tk << rk) + (any << rv))); };
   auto fits = [&](int rk, int rv) { return rk <= 4 && rv <= 4 && need(rk, rv) <= kSmemMax; };
-  if (p.ext && !fits(0, 0)) { p.ext = 0; tk = tv = table; }
+  if (p.ext_k && !fits(0, 0)) { p.ext_k = p.ext_v = 0; tk = tv = table; }
   if (!fits(0, 0)) return HQMQ_ERR_UNSUPPORTED;
   // (replicas of the tables against bank conflicts, K first)
   for (bool more = true; more;) {

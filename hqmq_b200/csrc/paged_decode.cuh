@@ -33,14 +33,17 @@ struct DecodeParams {
   float qmaxf, vfac;             // 1 / qmax
   int sdt, pay_bf16;             // type of the scales; whether the flagged chunks' values are bf16 (else fp16)
   const int4* seqs; const int4* units; const int* base; const int* warps; const int4* cuts; const int* tabs; const int* hdr;
-  int ctas, fused, ext;          // fused: the CTAs of a head are a cluster; ext: the tables have entries of every warp's own
+  int ctas, fused, ext_k, ext_v; // fused: the CTAs of a head are a cluster; entries of every warp's own that the tables have (0: none)
   float* parts;                  // [CTA][warps][2][part], then [CTA][2][part]
   uint2* wide;                   // [CTA][warps][K, V][16 N]: values of a tile with more flagged chunks than a stage holds
 };
 
 // Values of flagged chunks as table entries: where the index bits of a field leave room behind the codebook (2^(bits - 1) sign-folded
-// entries; 896 of them at S = 96, 1792 at 192), every warp has this many entries of K's table and of V's to itself.
-constexpr int kExtK = 36, kExtV = 24;
+// entries; 896 of them at S = 96, 1792 at 192), the warps share it out, up to the entries that a tile has staged: 56 and 32 of K's and V's at
+// S = 96 with 16 warps, 64 and 32 at 192.  Less than kExtLeast would not take one chunk column that is flagged in every token.  A tile with more
+// has products of their own, as where there is no room.  (16 x 8k, 8 heads of 128, S = 96, one to four such columns in K: 98, 102, 106
+// and 118 us; with 36 and 24 entries and tiles with more through global memory 98, 102, 145 and 167.)
+constexpr int kExtLeast = 16;
 __host__ __device__ constexpr bool has_ext(int ib) { return ib == 12 || ib == 13; }
 // Field c of a row: IB + RB bits, the row's words the writing lane's own.
 template <int IB, int RB>
@@ -120,15 +123,15 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
   using FL = FastLoader<N, IB ? IB : 12, IB ? RB : 4, true>;
   constexpr int NKS = Geo<N>::NKS, NVG = Geo<N>::NVG, NOT = 2 * NVG;
   constexpr int NW = NB == 1 ? kDecWarps : kDecWarpsWide, THREADS = NW * 32, PART = part_floats<N, NB>();
-  const bool ext = OUTL && has_ext(IB) && p.ext != 0;
+  const bool ext = OUTL && has_ext(IB) && p.ext_k != 0;
   const int ROW = IB ? row_bytes_of<N, IB, RB>() : p.row_bytes;
   const TileLayout L = tile_layout(ROW, true, OUTL);
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const uint32_t strideK = 8u << p.repk, strideV = 8u << p.repv;
   unsigned char* tblK = smem_raw;
-  unsigned char* tblV = smem_raw + (size_t)((p.table_rows >> 1) + (ext ? NW * kExtK : 0)) * strideK;
+  unsigned char* tblV = smem_raw + (size_t)((p.table_rows >> 1) + (ext ? NW * p.ext_k : 0)) * strideK;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 3, r = lane >> 2;
-  unsigned char* rings = tblV + (size_t)((p.table_rows >> 1) + (ext ? NW * kExtV : 0)) * strideV;
+  unsigned char* rings = tblV + (size_t)((p.table_rows >> 1) + (ext ? NW * p.ext_v : 0)) * strideV;
   unsigned char* ring = rings + (size_t)warp * kTileStages * L.bytes;
   const uint32_t ring32 = smem_u32(ring);
   // (of 32 rows, a warp's queries are 8 KB in shared memory, as the fragments that a lane reads: registers hold the accumulators)
@@ -227,23 +230,24 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
         if (__any_sync(0xffffffffu, fl != 0u)) {
           const uint32_t own = __popc(fl);
           before = counts_before(own, lane);
-          if (!ext) {
+          const bool as_entries = ext && __all_sync(0xffffffffu, before + own <= (uint32_t)(lane < 16 ? p.ext_k : p.ext_v));
+          if (!as_entries) {
             kcols = __reduce_or_sync(0xffffffffu, lane < 16 ? fl : 0u);
             vcols = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : fl);
+            wide = __any_sync(0xffffffffu, before + own > (uint32_t)(lane < 16 ? kPayK : kPayV));
           }
-          wide = __any_sync(0xffffffffu, before + own > (uint32_t)(lane < 16 ? (ext ? kExtK : kPayK) : (ext ? kExtV : kPayV)));
           // every lane its token's values, in place
           const float rs = bits16_to_float(reinterpret_cast<const uint16_t*>(sp + L.rsk)[lane], p.sdt);
           const float inv = rs != 0.f ? __fdividef(p.qmaxf, rs) : 0.f;
           const bool bf = p.pay_bf16 != 0;
           auto operand = [&](uint2 v) { return make_uint2(scaled_pair(v.x, inv, bf), scaled_pair(v.y, inv, bf)); };
           uint2* e = reinterpret_cast<uint2*>(sp + L.pay + (lane < 16 ? 0 : kPayK * 8)) + before;
-          if (ext && !wide) {
+          if (as_entries) {
             // Entries behind the codebook are this warp's: the value goes where the lane that decodes the chunk will look, and the chunk's
             // field in the staged row becomes that entry's, times one.
             const bool of_v = lane >= 16;
             const int tok = lane & 15;
-            uint32_t entry = (uint32_t)(p.table_rows >> 1) + (of_v ? warp * kExtV : warp * kExtK) + before;
+            uint32_t entry = (uint32_t)(p.table_rows >> 1) + (of_v ? warp * p.ext_v : warp * p.ext_k) + before;
             const uint32_t stride = of_v ? strideV : strideK, mask = (stride >> 3) - 1u;
             uint32_t dst = (of_v ? (uint32_t)(tblV - smem_raw) : 0u) + entry * stride;
             unsigned char* row = sp + (of_v ? L.v : 0) + tok * ROW;
@@ -266,8 +270,6 @@ __global__ void __launch_bounds__((NB == 1 ? kDecWarps : kDecWarpsWide) * 32, 1)
           } else if (!wide) {
             for (uint32_t x = 0; x < own; ++x, ++e) *e = operand(*e);
           } else {
-            kcols = __reduce_or_sync(0xffffffffu, lane < 16 ? fl : 0u);
-            vcols = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : fl);
             const int64_t ph = *reinterpret_cast<const int*>(sp + L.off + 16);
             const hqmq_packed& pk = lane < 16 ? p.pool.K : p.pool.V;
             uint2* far = my_wide() + (lane < 16 ? 0 : 16 * N) + before;

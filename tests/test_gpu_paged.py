@@ -958,3 +958,18 @@ def test_weights_beside_a_key_that_is_no_number(value):
         got = [torch.cat([mass[p] for p in t], 1)[:, :n].double() for t, n in zip(w.tables, w.kv)]
         assert bool(((got[0] - m).abs() <= bound + m * (2.0 ** -20 + 4 * q_lens[0] * 2.0 ** -24)).all())
         assert bool(got[1].isnan().all())
+
+
+@pytest.mark.parametrize("d,S,rb", [(128, 96, 4), (64, 96, 4), (128, 192, 6)])
+@pytest.mark.parametrize("channels", [1, 2, 3, 4, 5])
+def test_chunk_columns_that_most_tokens_have_flagged(d, S, rb, channels):
+    """About 13 to 70 flagged chunks a tile, in K and V: as many as a warp has table entries for, as are staged, and more."""
+    w = World(1, d, S, rb, [300, 90, 17], rounds=1, kind="randn", garbage=False)
+    x = [make_kv("randn", (1, 1, 407, d), 5 + i, torch.bfloat16) for i in (0, 1)]
+    for y in x:
+        y[..., torch.arange(channels) * 8 + 3] *= 40.0
+    pair = [w.quant.encode(y.to(DEV), 0, i) for i, y in enumerate(x)]
+    hqmq.paged_store(w.pool, *pair, hqmq.PagedBatch(w.pool, w.tables, w.kv, w.kv))
+    for q_lens in ([1, 1, 1], [4, 3, 1], [8, 2, 1]):
+        q = queries(w, q_lens, 4, torch.bfloat16)
+        check_attend(w, hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab), q, q_lens, 4)
