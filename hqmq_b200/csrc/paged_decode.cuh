@@ -9,11 +9,11 @@
 //     without room, fields of any width), or a tile has more than the warp has entries, they are products of their own behind
 //     the others': a lane, which owns 2 tokens x N / 4 chunks of K and 4 x N / 8 of V, finds its values by counting the flags before them.
 //     (16 sequences of 16 to 32 k tokens, two outlier channels a head in K: values put into the fragments by branches 381 us, products of
-//     their own 316, table entries 268; 169 without outliers.  Repeated passes of the main products for a tile with too many, in place of the
+//     their own 316, table entries 269; 173 without outliers.  Repeated passes of the main products for a tile with too many, in place of the
 //     products of their own, took 277 to 299; without either the kernel would take 254);
 //   - V's scales enter P relative to the largest one seen, a power of two that the accumulators are rescaled by like by the maximum, so
 //     that values of any size keep their bits.
-// What bounds it: instructions, 1013 a tile with those outliers and 680 without, at 61 to 62 % of the issue slots (chains of look-up,
+// What bounds it: instructions, 1004 a tile with those outliers and about 690 without, at 60 to 62 % of the issue slots (chains of look-up,
 // multiply, product in 16 warps of 128 registers).
 #pragma once
 #include "attn_tma.cuh"

@@ -301,6 +301,9 @@ def paged_attention(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, table_K: 
     the last ones).  ``softcap``: scores become softcap * tanh(score / softcap).  ``sinks`` (H_q): a logit per head that takes part in the
     softmax and has no value.  ``table_K`` / ``table_V``: the quantizer's fp16 tables, as in ``fused_attention_packed``.
 
+    Operands are 16-bit as in the framework's other attention calls: queries (every row relative to a power of two of its own), decoded keys and
+    values and the softmax weights have 11 bits, whatever the types of Q and ``out``; products are summed in fp32.
+
     Sequences with few rows (new tokens times heads per KV head up to 32) are read in place; the pages of prompt chunks are decoded
     once per call into operand tiles for the tensor cores, half a gigabyte at a time."""
     if Q.stride(-1) != 1:
@@ -397,8 +400,8 @@ def paged_attention_mass(Q: torch.Tensor, pool: PagedKV, batch: PagedBatch, tabl
 def paged_store(pool: PagedKV, K: PackedKV, V: PackedKV, batch: PagedBatch) -> None:
     """Encoded keys and values (``HQMQ.encode`` of (1, H_kv, total_q, d), tokens in the order of the batch's queries) become the last
     ``q_len`` tokens of their sequences.  What the pages held from the first of them on is gone: a sequence whose drafted tokens were
-    rejected goes on with a batch of its shorter length, and storing a step twice stores it once.  Pages that are written belong to one
-    sequence."""
+    rejected goes on with a batch of its shorter length, and storing a step twice stores it once (weights that its tokens had, see
+    ``paged_attention_mass``, are the caller's to reset).  Pages that are written belong to one sequence."""
     _belongs(pool, batch, "paged_store")
     for name, src, dst in (("K", K, pool.K), ("V", V, pool.V)):
         if src.B != 1 or src.T < batch.total_q or (src.H, src.n_chunks, src.S, src.radius_bits) != (dst.H, dst.n_chunks, dst.S, dst.radius_bits):
