@@ -973,3 +973,53 @@ def test_chunk_columns_that_most_tokens_have_flagged(d, S, rb, channels):
     for q_lens in ([1, 1, 1], [4, 3, 1], [8, 2, 1]):
         q = queries(w, q_lens, 4, torch.bfloat16)
         check_attend(w, hqmq.paged_attention(q.to(DEV), w.pool, w.batch(q_lens, 4), *w.tab), q, q_lens, 4)
+
+
+def test_captured_steps_store_and_attend():
+    """A step captured once and replayed: its tokens are stored where the renewed batch says, whatever warm-up calls stored before."""
+    H, G, d, B = 2, 4, 128, 2
+    q = hqmq.HQMQ(1, H, 96, 4, device=DEV)
+    quant = hqmq.with_outlier_extraction(q, C=1.5)
+    tab = [q.tables(0, i, DEV)["table16"] for i in (0, 1)]
+    pools = [hqmq.PagedKV(12, H, d, 96, 4, DEV, outliers_K=True, outliers_V=True, out_cap=64 * 32) for _ in (0, 1)]
+    tables, kv, n_new = [[3, 1, 7], [0, 5, 9]], [61, 20], [1, 2]
+    x = [make_kv("spiky", (1, H, sum(kv), d), i, torch.bfloat16).to(DEV) for i in (0, 1)]
+    first = [q.new_cache(1, sum(kv), d, DEV, scale_dtype=torch.bfloat16, with_outliers=True, out_dtype=torch.bfloat16) for _ in (0, 1)]
+    quant.encode_pair(*x, 0, *first)
+    for pool in pools:
+        hqmq.paged_store(pool, *first, hqmq.PagedBatch(pool, tables, kv, kv))
+    pair = [q.new_cache(1, sum(n_new), d, DEV, scale_dtype=torch.bfloat16, with_outliers=True, out_dtype=torch.bfloat16) for _ in (0, 1)]
+    fresh = lambda seed: [make_kv("spiky", (1, H, sum(n_new), d), seed + i, torch.bfloat16).to(DEV) for i in (0, 1)]
+    quant.encode_pair(*fresh(50), 0, *pair)
+    Q = torch.randn(sum(n_new), H * G, d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    batch = hqmq.PagedBatch(pools[0], tables, [n + m for n, m in zip(kv, n_new)], n_new, n_heads=H * G, reserve_pages=12)
+    out = torch.empty_like(Q)
+
+    def step():
+        hqmq.paged_store(pools[0], *pair, batch)
+        hqmq.paged_attention(Q, pools[0], batch, *tab, out=out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(6):                                                   # (over the end of a page and of blocks)
+        kv = [n + m for n, m in zip(kv, n_new)]
+        new = [q.new_cache(1, sum(n_new), d, DEV, scale_dtype=torch.bfloat16, with_outliers=True, out_dtype=torch.bfloat16) for _ in (0, 1)]
+        quant.encode_pair(*fresh(60 + 2 * i), 0, *new)
+        for a, b in zip(pair, new):
+            for name in ("codes", "rs", "flags", "out_off", "out_vals"):
+                getattr(a, name).copy_(getattr(b, name))
+        batch.renew(tables, kv)
+        graph.replay()
+        eager = hqmq.PagedBatch(pools[1], tables, kv, n_new, n_heads=H * G)
+        hqmq.paged_store(pools[1], *new, eager)
+        want = hqmq.paged_attention(Q, pools[1], eager, *tab)
+        torch.cuda.synchronize()
+        _same_contents(*pools, tables, kv)
+        assert float((out.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
